@@ -15,14 +15,17 @@ from dataclasses import dataclass
 
 from . import _lib
 from ._lib import (STATUS_OK, STATUS_INVALID_ARGUMENT, STATUS_UNSUPPORTED, STATUS_MISALIGNED,
-                   STATUS_NO_SM100, STATUS_DEVICE_TIMEOUT, FaTilingInfo)
+                   STATUS_NO_SM100, STATUS_DEVICE_TIMEOUT, STATUS_BAD_REQUEST, STATUS_OUT_OF_PAGES,
+                   STATUS_WORKSPACE, FaTilingInfo)
+from .paged import PagedPlan, PagedShape, paged_attention, paged_plan, rotary_append, rotary_embed
 
 __all__ = [
     "AttentionShape", "FaError", "default_scale", "attention_flops", "sm100_supported",
     "launch_attention_sm100", "launch_attention_sm100_slabs", "query_sm100", "sm100_hbm_bytes",
     "sm100_min_bytes", "attention_forward", "attention_forward_host", "device_status",
     "STATUS_OK", "STATUS_INVALID_ARGUMENT", "STATUS_UNSUPPORTED", "STATUS_MISALIGNED",
-    "STATUS_NO_SM100", "STATUS_DEVICE_TIMEOUT",
+    "STATUS_NO_SM100", "STATUS_DEVICE_TIMEOUT", "STATUS_BAD_REQUEST", "STATUS_OUT_OF_PAGES", "STATUS_WORKSPACE",
+    "PagedShape", "PagedPlan", "paged_plan", "paged_attention", "rotary_embed", "rotary_append",
 ]
 
 

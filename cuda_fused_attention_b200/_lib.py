@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/fa_sm100.h (libfa_sm100.so, built in-tree).
+"""ctypes binding of the C ABI in include/ (libfa_sm100.so, built in-tree).
 
 This is the exact binding a Python caller of the reference's launch API would
 write; it carries no compute of its own. If the library is missing the import
@@ -21,8 +21,11 @@ STATUS_DEVICE_TIMEOUT = 1007
 STATUS_HOST_ALLOC = 1008
 STATUS_BUILD_MISMATCH = 1009
 STATUS_STATIC_TOO_LARGE = 1010
+STATUS_BAD_REQUEST = 1011
+STATUS_OUT_OF_PAGES = 1012
+STATUS_WORKSPACE = 1013
 
-#: Every symbol include/fa_sm100.h declares, with (restype, argtypes).
+#: Every symbol the headers in include/ declare, with (restype, argtypes).
 _VP = ctypes.c_void_p
 _I = ctypes.c_int
 _LL = ctypes.c_longlong
@@ -46,6 +49,13 @@ SIGNATURES = {
     "fa_sm100_release_staging": (_I, []),
     "fa_sm100_fwd_host_static": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP]),
     "fa_sm100_static_staging_bytes": (ctypes.c_size_t, []),
+    "fa_sm100_paged_schedule_bytes": (ctypes.c_size_t, [_I]),
+    "fa_sm100_paged_plan": (_I, [_VP, _VP, _VP, _VP, _I, _VP, _VP]),
+    "fa_sm100_rotary": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _VP, _VP, _I, _VP, _I, _I, _I, _VP]),
+    "fa_sm100_rotary_append": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _VP, _LL, _VP, _VP,
+                                    _I, _VP, _I, _I, _VP]),
+    "fa_sm100_paged_fwd": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_size_t, _VP]),
+    "fa_sm100_paged_workspace_bytes": (ctypes.c_size_t, [_VP]),
 }
 
 
@@ -55,6 +65,14 @@ class FaTilingInfo(ctypes.Structure):
         "supported", "block_size", "tile_kv", "rows_per_block", "shared_bytes_per_block",
         "registers_per_thread", "local_bytes_per_thread", "max_blocks_per_sm",
         "device_shared_bytes_per_sm", "shared_limited_blocks_per_sm")]
+
+
+class FaPagedPlan(ctypes.Structure):
+    """Layout of FaPagedPlan (include/fa_sm100_paged.h)."""
+    _fields_ = [(name, ctypes.c_int) for name in (
+        "num_seqs", "total_tokens", "max_new", "num_pages", "table_width", "table_stride", "heads", "kv_heads",
+        "head_dim", "page_size", "causal", "reserved")] + [(name, ctypes.c_void_p) for name in (
+            "query_start", "kv_lens", "positions", "slots", "block_table", "free_cursor", "schedule")]
 
 
 _lock = threading.Lock()

@@ -4,7 +4,7 @@
 
 compiles cuda_fused_attention_b200/csrc/*.cu with nvcc for sm_100a only into
 cuda_fused_attention_b200/lib/libfa_sm100.so. The library exports the C ABI of
-include/fa_sm100.h and the C++ API of include/flash_attention_sm100.h; the CUDA
+include/fa_sm100.h and include/fa_sm100_paged.h and the C++ API of include/flash_attention_sm100.h; the CUDA
 runtime is linked statically and the driver is reached only through
 cudaGetDriverEntryPoint, so the .so needs nothing but libc/libstdc++ and the
 NVIDIA driver at run time.
@@ -24,7 +24,8 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libfa_sm100.so")
 DEBUG_LIB_PATH = os.path.join(LIB_DIR, "libfa_sm100_debug.so")
-SOURCES = ["fa_sm100.cu", "fa_sm100_host.cu", "fa_sm100_api.cu", "fa_sm100_static.cu"]
+SOURCES = ["fa_sm100.cu", "fa_sm100_host.cu", "fa_sm100_api.cu", "fa_sm100_static.cu",
+           "fa_sm100_plan.cu", "fa_sm100_paged.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

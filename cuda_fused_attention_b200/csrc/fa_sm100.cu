@@ -59,6 +59,7 @@
 
 #include "fa_sm100.h"
 #include "fa_sm100_internal.h"
+#include "fa_sm100_paged.cuh"
 #include "fa_sm100_ptx.cuh"
 
 namespace fa_sm100 {
@@ -1489,8 +1490,18 @@ int fa_sm100_device_status(unsigned int* detail)
     const unsigned int zero = 0;
     err = cudaMemcpyToSymbol(g_fa_error_word, &zero, sizeof(zero));
     if (err != cudaSuccess) return static_cast<int>(err);
+    // The paged-cache operators keep words of their own: what they recorded joins this one.
+    unsigned int plan_word = 0, paged_word = 0;
+    int status = fa_sm100_internal::take_plan_error(&plan_word);
+    if (status == FA_STATUS_OK) status = fa_sm100_internal::take_paged_attention_error(&paged_word);
+    if (status != FA_STATUS_OK) return status;
+    const unsigned int paged = plan_word | paged_word;
+    if (word == 0 || (paged & 1u) == 0) word |= paged;
+    else word |= paged & ~0xFF00u;      // one wait site only
     if (detail != nullptr) *detail = word;
-    return word ? FA_STATUS_DEVICE_TIMEOUT : FA_STATUS_OK;
+    if (word & 1u) return FA_STATUS_DEVICE_TIMEOUT;
+    if (word & FA_ERROR_OUT_OF_PAGES) return FA_STATUS_OUT_OF_PAGES;
+    return word ? FA_STATUS_BAD_REQUEST : FA_STATUS_OK;
 }
 
 int fa_sm100_debug_read(float* out, size_t floats)
@@ -1521,6 +1532,9 @@ const char* fa_sm100_status_string(int status)
         case FA_STATUS_HOST_ALLOC: return "staging allocation failed";
         case FA_STATUS_BUILD_MISMATCH: return "kernel built with fewer registers than its warpgroup split needs";
         case FA_STATUS_STATIC_TOO_LARGE: return "slab larger than the fixed staging of fa_sm100_fwd_host_static";
+        case FA_STATUS_BAD_REQUEST: return "a length, page id or slot on the device was out of range";
+        case FA_STATUS_OUT_OF_PAGES: return "the free list was shorter than the pages a step needed";
+        case FA_STATUS_WORKSPACE: return "workspace too small";
         default: break;
     }
     if (status > 0 && status < 1000) return cudaGetErrorString(static_cast<cudaError_t>(status));

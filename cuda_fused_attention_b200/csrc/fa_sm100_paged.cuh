@@ -1,0 +1,88 @@
+// What the paged-cache translation units share: the geometry of attention work
+// and how a linear range of it maps back to requests.
+//
+// A request with n new tokens and a group of G query heads per K/V head has n * G query
+// rows per K/V head (row = token * G + head in group). Requests of at most kNarrowRows rows
+// go to the narrow kernel, whose unit of work is a 64-key tile; all others to the wide
+// kernel, whose unit is a 128-key tile of a block of 2 * tokens_per_tile(G) tokens.
+#pragma once
+
+#include <cstdint>
+
+#include "fa_sm100_paged.h"
+
+namespace fa_sm100 {
+
+constexpr int kNarrowRows = 16;
+constexpr int kNarrowKeys = 64;
+constexpr int kWideRows = 128;      // query rows of one tile (tensor-memory lanes)
+constexpr int kWideKeys = 128;
+static_assert(kWideKeys == 128, "floor_sum_128 counts key tiles");
+
+// plan->schedule: narrow_start[num_seqs + 1], then wide_start[num_seqs + 1]: prefix sums of the
+// requests' units for one K/V head.
+__host__ __device__ inline long long* narrow_starts(long long* schedule, int) { return schedule; }
+__host__ __device__ inline long long* wide_starts(long long* schedule, int num_seqs) { return schedule + num_seqs + 1; }
+
+__host__ __device__ inline int tokens_per_tile(int group) { return kWideRows / group; }
+__host__ __device__ inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// sum over 0 <= i < n of floor((a * i + b) / 128), a, b >= 0. The terms' sum is exact without the
+// floors; what the floors drop, (a * i + b) mod 128, repeats with period P = 128 / gcd(a, 128), and
+// over one period takes each value that is b modulo the gcd once. So P - 1 terms at most are added up.
+__host__ __device__ inline long long floor_sum_128(long long n, long long a, long long b)
+{
+    long long g = 128;
+    while (a % g) g >>= 1;
+    const long long period = 128 / g;
+    long long dropped = n / period * (period * (b % g) + g * (period * (period - 1) / 2));
+    for (long long i = 0; i < n % period; ++i) dropped += (a * i + b) & 127;
+    return (n * b + a * (n * (n - 1) / 2) - dropped) / 128;
+}
+
+// Key tiles of token block u (of `span` tokens) of a request with `cached` + `n` tokens.
+__host__ __device__ inline long long wide_tiles_of(long long u, long long span, long long cached, long long n, bool causal)
+{
+    const long long end = (u + 1) * span < n ? (u + 1) * span : n;
+    return ceil_div(cached + (causal ? end : n), kWideKeys);
+}
+
+// Key tiles of the request's first `blocks` token blocks.
+__host__ __device__ inline long long wide_tiles_through(long long blocks, long long span, long long cached, long long n,
+                                                        bool causal)
+{
+    if (blocks <= 0) return 0;
+    if (!causal) return blocks * ceil_div(cached + n, kWideKeys);
+    const long long whole = n / span < blocks ? n / span : blocks;      // blocks that end at (u + 1) * span
+    const long long sum = floor_sum_128(whole, span, cached + span + kWideKeys - 1);
+    return sum + (blocks > whole ? ceil_div(cached + n, kWideKeys) : 0);
+}
+
+// Last b in [0, num_seqs) with start[b] <= y, for start[0] = 0 <= y < start[num_seqs].
+__device__ inline int find_request(const long long* start, int num_seqs, long long y)
+{
+    int lo = 0, hi = num_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (start[mid] <= y) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+}  // namespace fa_sm100
+
+namespace fa_sm100_internal {
+
+// The device error word of a paged translation unit on the current device: read (synchronous)
+// and cleared. Returns a cudaError_t; *word receives the bits.
+int take_plan_error(unsigned int* word);
+int take_paged_attention_error(unsigned int* word);
+
+int validate_plan(const FaPagedPlan* plan);
+bool page_size_supported(int page_size);
+
+// cudaError_t or FA_STATUS_*: the current device, its SM count, and that it is compute capability 10.x.
+int current_sm100(int* device, int* sm_count);
+
+}  // namespace fa_sm100_internal

@@ -1,0 +1,555 @@
+// Paged-cache plan and rotary kernels (sm_100a): block tables and slot maps built
+// from request lengths, rotary positions, and the write of K and V to cache slots.
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <climits>
+#include <cstdint>
+
+#include "fa_sm100_paged.h"
+#include "fa_sm100_paged.cuh"
+
+namespace fa_sm100 {
+
+__device__ unsigned int g_plan_error_word;
+
+__device__ __forceinline__ void record_plan_error(unsigned int bits) { atomicOr(&g_plan_error_word, bits); }
+
+// =============================================================================
+// Plan
+// =============================================================================
+// Three prefix sums over the requests (new tokens, new pages, attention units), then one slot
+// per new token and one table entry per new page. The bytes are few (16 per request, 8 per token,
+// 8 per new page), so the time is launch and latency: everything is one launch. Every CTA runs
+// the scan over all requests, 512 at a time, and after each 512 serves its share of their tokens
+// and pages, found by binary search in shared memory; the CTAs never wait for one another. A new
+// page's id is taken from the free list, not from the table that another CTA may be writing.
+constexpr int kPlanThreads = 512;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanTokensPerCta = 2048;     // tokens per CTA before another CTA is launched
+
+struct PlanParams {
+    FaPagedPlan plan;
+    const int* cached;
+    const int* fresh;               // new_lens
+    const int* free_pages;
+    int num_free;
+    const int* free_start;
+};
+
+struct PlanSums {
+    long long tokens, pages, narrow, wide;
+};
+
+__device__ __forceinline__ long long warp_inclusive(long long v, int lane)
+{
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long other = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += other;
+    }
+    return v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads)
+plan_kernel(const PlanParams p)
+{
+    const FaPagedPlan& plan = p.plan;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const int ps = plan.page_size;
+    const int shift = __ffs(ps) - 1;
+    const int group = plan.heads / plan.kv_heads;
+    const long long span = 2LL * tokens_per_tile(group);
+    const bool first_cta = blockIdx.x == 0;
+
+    __shared__ PlanSums warp_sums[kPlanWarps];
+    __shared__ int s_start[kPlanThreads + 1];       // packed row of each request of this round
+    __shared__ int s_page[kPlanThreads + 1];        // new pages before each request of this round
+    __shared__ int s_cached[kPlanThreads];          // cached tokens, -1 for a request with invalid lengths
+    long long* narrow = narrow_starts(plan.schedule, plan.num_seqs);
+    long long* wide = wide_starts(plan.schedule, plan.num_seqs);
+
+    const long long free_start = p.free_start ? *p.free_start : 0;
+    PlanSums carry = {0, 0, 0, 0};
+    for (int base = 0; base < plan.num_seqs; base += kPlanThreads) {
+        const int b = base + tid;
+        long long cached = 0, n = 0, need = 0, narrow_units = 0, wide_units = 0;
+        bool valid = false;
+        if (b < plan.num_seqs) {
+            cached = p.cached[b];
+            n = p.fresh[b];
+            valid = cached >= 0 && n >= 0 && n <= plan.total_tokens && n <= plan.max_new &&
+                    cached + n <= static_cast<long long>(plan.table_width) * ps;
+            if (!valid && first_cta) record_plan_error(FA_ERROR_BAD_LENGTH);
+            // A request with invalid lengths keeps its place on the token axis if that is known.
+            if (n < 0) n = 0;
+            if (n > plan.total_tokens) n = plan.total_tokens;
+        }
+        if (valid) {
+            const long long kv = cached + n;
+            need = ((kv + ps - 1) >> shift) - ((cached + ps - 1) >> shift);
+        }
+        PlanSums sum;
+        sum.tokens = warp_inclusive(n, lane);
+        sum.pages = warp_inclusive(need, lane);
+        // The tokens of requests past total_tokens have no rows: such a request gets no work.
+        if (lane == 31) warp_sums[warp] = {sum.tokens, sum.pages, 0, 0};
+        __syncthreads();
+        long long tokens_before = carry.tokens + sum.tokens - n, pages_before = carry.pages + sum.pages - need;
+        long long round_tokens = 0, round_pages = 0;
+        for (int w = 0; w < kPlanWarps; ++w) {
+            if (w < warp) {
+                tokens_before += warp_sums[w].tokens;
+                pages_before += warp_sums[w].pages;
+            }
+            round_tokens += warp_sums[w].tokens;
+            round_pages += warp_sums[w].pages;
+        }
+        const long long total = plan.total_tokens;
+        const bool fits = tokens_before + n <= total;
+        if (!fits && first_cta && b < plan.num_seqs) record_plan_error(FA_ERROR_BAD_LENGTH);
+        if (valid && fits && n > 0) {
+            if (n * group <= kNarrowRows) narrow_units = ceil_div(cached + n, kNarrowKeys);
+            else wide_units = wide_tiles_through(ceil_div(n, span), span, cached, n, plan.causal != 0);
+        }
+        s_start[tid] = static_cast<int>(tokens_before < total ? tokens_before : total);
+        s_page[tid] = static_cast<int>(pages_before - carry.pages < INT_MAX ? pages_before - carry.pages : INT_MAX);
+        s_cached[tid] = valid && fits ? static_cast<int>(cached) : -1;
+        if (tid == 0) {
+            const long long end = carry.tokens + round_tokens;
+            s_start[kPlanThreads] = static_cast<int>(end < total ? end : total);
+            s_page[kPlanThreads] = static_cast<int>(round_pages < INT_MAX ? round_pages : INT_MAX);
+        }
+        if (first_cta) {
+            // Only one CTA writes the per-request arrays, so only it needs the units' sums.
+            sum.narrow = warp_inclusive(narrow_units, lane);
+            sum.wide = warp_inclusive(wide_units, lane);
+            __syncthreads();
+            if (lane == 31) { warp_sums[warp].narrow = sum.narrow; warp_sums[warp].wide = sum.wide; }
+            __syncthreads();
+            long long narrow_before = carry.narrow + sum.narrow - narrow_units;
+            long long wide_before = carry.wide + sum.wide - wide_units;
+            for (int w = 0; w < kPlanWarps; ++w) {
+                if (w < warp) {
+                    narrow_before += warp_sums[w].narrow;
+                    wide_before += warp_sums[w].wide;
+                }
+                carry.narrow += warp_sums[w].narrow;
+                carry.wide += warp_sums[w].wide;
+            }
+            if (b < plan.num_seqs) {
+                plan.query_start[b] = s_start[tid];
+                plan.kv_lens[b] = valid && fits ? static_cast<int>(cached + n) : 0;
+                narrow[b] = narrow_before;
+                wide[b] = wide_before;
+            }
+        }
+        __syncthreads();
+
+        // This round's tokens: t in [s_start[0], s_start[last]), a contiguous share per CTA.
+        const int first = s_start[0], count = s_start[kPlanThreads] - first;
+        const int share = (count + gridDim.x - 1) / static_cast<int>(gridDim.x);
+        const int lo = first + static_cast<int>(min(static_cast<long long>(share) * blockIdx.x, static_cast<long long>(count)));
+        const int hi = min(first + count, lo + share);
+        for (int t = lo + tid; t < hi; t += kPlanThreads) {
+            int r = 0;
+#pragma unroll
+            for (int step = kPlanThreads / 2; step > 0; step >>= 1)
+                if (s_start[r + step] <= t) r += step;
+            const int cached_r = s_cached[r];
+            const long long pos = static_cast<long long>(cached_r) + (t - s_start[r]);
+            int slot = -1;
+            if (cached_r >= 0 && pos < static_cast<long long>(plan.table_width) * ps) {
+                const int index = static_cast<int>(pos >> shift);
+                const int have = static_cast<int>((static_cast<long long>(cached_r) + ps - 1) >> shift);
+                int page = -1;
+                if (index < have) {
+                    page = plan.block_table[static_cast<long long>(base + r) * plan.table_stride + index];
+                    if (page < 0 || page >= plan.num_pages) {
+                        record_plan_error(FA_ERROR_BAD_PAGE);
+                        page = -1;
+                    }
+                } else {
+                    // A free page that is missing or outside the cache is recorded where it is handed out.
+                    const long long from = free_start + carry.pages + s_page[r] + (index - have);
+                    if (from >= 0 && from < p.num_free) page = p.free_pages[from];
+                    if (page < 0 || page >= plan.num_pages) page = -1;
+                }
+                if (page >= 0) slot = page * ps + static_cast<int>(pos & (ps - 1));
+            }
+            plan.positions[t] = cached_r >= 0 ? static_cast<int>(pos) : 0;
+            plan.slots[t] = slot;
+        }
+
+        // This round's new pages.
+        const int pages = s_page[kPlanThreads];
+        for (int k = blockIdx.x * kPlanThreads + tid; k < pages; k += gridDim.x * kPlanThreads) {
+            int r = 0;
+#pragma unroll
+            for (int step = kPlanThreads / 2; step > 0; step >>= 1)
+                if (s_page[r + step] <= k) r += step;
+            if (s_cached[r] < 0) continue;
+            const int have = static_cast<int>((static_cast<long long>(s_cached[r]) + ps - 1) >> shift);
+            const long long from = free_start + carry.pages + k;
+            if (from < 0 || from >= p.num_free) {
+                record_plan_error(FA_ERROR_OUT_OF_PAGES);
+                continue;
+            }
+            const int page = p.free_pages[from];
+            if (page < 0 || page >= plan.num_pages) {
+                record_plan_error(FA_ERROR_BAD_PAGE);
+                continue;
+            }
+            plan.block_table[static_cast<long long>(base + r) * plan.table_stride + have + (k - s_page[r])] = page;
+        }
+        carry.tokens += round_tokens;
+        carry.pages += round_pages;
+        __syncthreads();
+    }
+
+    if (first_cta && tid == 0) {
+        plan.query_start[plan.num_seqs] =
+            static_cast<int>(carry.tokens < plan.total_tokens ? carry.tokens : plan.total_tokens);
+        narrow[plan.num_seqs] = carry.narrow;
+        wide[plan.num_seqs] = carry.wide;
+        *plan.free_cursor = static_cast<int>(free_start + carry.pages);
+    }
+    // Padding rows behind the last request.
+    const long long used = carry.tokens < plan.total_tokens ? carry.tokens : plan.total_tokens;
+    for (long long t = used + blockIdx.x * kPlanThreads + tid; t < plan.total_tokens; t += gridDim.x * kPlanThreads) {
+        plan.positions[t] = 0;
+        plan.slots[t] = -1;
+    }
+}
+
+// =============================================================================
+// Rotary positions, and the append of K and V
+// =============================================================================
+// A thread owns eight pairs (16 elements, two 16-byte accesses) of one token and walks over
+// heads: the eight angles are computed once, in registers, and serve every head it visits. The
+// rest is a stream: each element is read once and written once. An angle is a position times a
+// frequency; far positions need more than 24 bits of it, so the product is taken in turns
+// (1 / 2 pi) in 64 bits, its whole turns dropped there, and only the rest goes to sincospif.
+constexpr int kRotaryThreads = 256;
+constexpr int kMaxAxes = 4;
+
+struct RotaryParams {
+    const __nv_bfloat16* src[3];        // q, k, v (x alone: q)
+    __nv_bfloat16* dst[3];
+    long long src_token[3], src_head[3], src_batch;
+    long long dst_token[3], dst_head[3], dst_batch;     // k, v of an append: dst_token is the row stride
+    long long dst_page[3];
+    int rows[3];                        // heads of each
+    int batch, tokens;
+    int units;                          // 16-element units per row
+    int rotary_dim;
+    int head_split;                     // threads that share a token's heads
+    const int* positions;
+    long long position_axis, position_batch;
+    const float* inv_freq;
+    int section_end[kMaxAxes];
+    const int* slots;
+    int page_shift;
+    long long num_slots;
+    float sign;                         // -1: inverse rotation
+};
+
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8])
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&f)[8])
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 pair = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&pair);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <bool kAppend, bool kInterleaved>
+__global__ void __launch_bounds__(kRotaryThreads)
+rotary_kernel(const RotaryParams p)
+{
+    const long long index = static_cast<long long>(blockIdx.x) * kRotaryThreads + threadIdx.x;
+    const int unit = static_cast<int>(index % p.units);
+    const long long rest = index / p.units;
+    const long long flat = rest % (static_cast<long long>(p.tokens) * p.batch);
+    const int part = static_cast<int>(rest / (static_cast<long long>(p.tokens) * p.batch));
+    if (part >= p.head_split) return;
+    const int batch = static_cast<int>(flat / p.tokens);
+    const int token = static_cast<int>(flat - static_cast<long long>(batch) * p.tokens);
+
+    long long slot = 0;
+    if (kAppend) {
+        slot = p.slots[token];
+        if (slot < 0) return;
+        if (slot >= p.num_slots) {
+            record_plan_error(FA_ERROR_BAD_PAGE);
+            return;
+        }
+    }
+
+    const int half = p.rotary_dim / 2;
+    const int rotating = p.rotary_dim / 16;
+    const bool turns = unit < rotating;
+    // The unit's two 8-element pieces: the two halves of its pairs, or 16 neighbours.
+    const int lo = turns && !kInterleaved ? 8 * unit : 16 * unit;
+    const int hi = turns && !kInterleaved ? half + 8 * unit : 16 * unit + 8;
+
+    float c[8], s[8];
+    if (turns) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int pair = 8 * unit + i;
+            int axis = 0;
+#pragma unroll
+            for (int a = 0; a < kMaxAxes - 1; ++a) axis += pair >= p.section_end[a] ? 1 : 0;
+            const int position = p.positions[axis * p.position_axis + batch * p.position_batch + token];
+            const double turn = static_cast<double>(position) * static_cast<double>(p.inv_freq[pair]) *
+                                0.15915494309189533577;
+            const float part_turn = static_cast<float>(turn - rint(turn));
+            sincospif(2.0f * part_turn, &s[i], &c[i]);
+            s[i] *= p.sign;
+        }
+    }
+
+    const int rows = p.rows[0] + (kAppend ? p.rows[1] + p.rows[2] : 0);
+    for (int row = part; row < rows; row += p.head_split) {
+        int which = 0, head = row;
+        if (kAppend) {
+            if (head >= p.rows[0]) { head -= p.rows[0]; which = 1; }
+            if (which == 1 && head >= p.rows[1]) { head -= p.rows[1]; which = 2; }
+        }
+        const __nv_bfloat16* src = p.src[which] + batch * p.src_batch + token * p.src_token[which] + head * p.src_head[which];
+        __nv_bfloat16* dst = p.dst[which] + head * p.dst_head[which];
+        if (kAppend && which > 0)
+            dst += (slot >> p.page_shift) * p.dst_page[which] + (slot & ((1LL << p.page_shift) - 1)) * p.dst_token[which];
+        else
+            dst += batch * p.dst_batch + token * p.dst_token[which];
+        uint4 x0 = *reinterpret_cast<const uint4*>(src + (kAppend && which == 2 ? 16 * unit : lo));
+        uint4 x1 = *reinterpret_cast<const uint4*>(src + (kAppend && which == 2 ? 16 * unit + 8 : hi));
+        if (turns && !(kAppend && which == 2)) {
+            float a[8], b[8], u[8], w[8];
+            unpack8(x0, a);
+            unpack8(x1, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (kInterleaved) {
+                    const int q = 2 * (i & 3);
+                    const float e = i < 4 ? a[q] : b[q], o = i < 4 ? a[q + 1] : b[q + 1];
+                    const float re = e * c[i] - o * s[i], im = o * c[i] + e * s[i];
+                    if (i < 4) { u[q] = re; u[q + 1] = im; }
+                    else { w[q] = re; w[q + 1] = im; }
+                } else {
+                    u[i] = a[i] * c[i] - b[i] * s[i];
+                    w[i] = b[i] * c[i] + a[i] * s[i];
+                }
+            }
+            x0 = pack8(u);
+            x1 = pack8(w);
+        }
+        *reinterpret_cast<uint4*>(dst + (kAppend && which == 2 ? 16 * unit : lo)) = x0;
+        *reinterpret_cast<uint4*>(dst + (kAppend && which == 2 ? 16 * unit + 8 : hi)) = x1;
+    }
+}
+
+}  // namespace fa_sm100
+
+// =============================================================================
+// Host side
+// =============================================================================
+namespace {
+
+using namespace fa_sm100;
+
+bool multiple_of_8(const long long* strides, int count)
+{
+    for (int i = 0; i < count; ++i)
+        if (strides[i] & 7) return false;
+    return true;
+}
+
+bool misaligned(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) != 0; }
+
+int fill_sections(RotaryParams& params, const int* sections, int axes, int rotary_dim)
+{
+    int end = 0;
+    for (int a = 0; a < kMaxAxes; ++a) {
+        if (a < axes) {
+            if (sections[a] < 0 || sections[a] > rotary_dim / 2) return FA_STATUS_INVALID_ARGUMENT;
+            end += sections[a];
+        }
+        params.section_end[a] = end;
+    }
+    return end == rotary_dim / 2 ? FA_STATUS_OK : FA_STATUS_INVALID_ARGUMENT;
+}
+
+template <bool kAppend>
+int launch_rotary(RotaryParams& params, bool interleaved, cudaStream_t stream)
+{
+    int device = 0, sms = 0;
+    const int status = fa_sm100_internal::current_sm100(&device, &sms);
+    if (status != FA_STATUS_OK) return status;
+    const long long tokens = static_cast<long long>(params.tokens) * params.batch;
+    const int rows = params.rows[0] + (kAppend ? params.rows[1] + params.rows[2] : 0);
+    if (tokens == 0 || rows == 0) return FA_STATUS_OK;
+    // Heads are shared out until the threads fill the GPU once (2048 per SM): few tokens are then
+    // served in one go, and many tokens keep the angles of a thread in use for all heads.
+    const long long per_split = tokens * params.units;
+    long long split = (2048LL * sms + per_split - 1) / per_split;
+    params.head_split = static_cast<int>(split < rows ? split : rows);
+    const long long blocks = (per_split * params.head_split + kRotaryThreads - 1) / kRotaryThreads;
+    if (blocks > INT_MAX) return FA_STATUS_INVALID_ARGUMENT;
+    if (interleaved) rotary_kernel<kAppend, true><<<static_cast<unsigned>(blocks), kRotaryThreads, 0, stream>>>(params);
+    else rotary_kernel<kAppend, false><<<static_cast<unsigned>(blocks), kRotaryThreads, 0, stream>>>(params);
+    return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace
+
+namespace fa_sm100_internal {
+
+int take_plan_error(unsigned int* word)
+{
+    cudaError_t err = cudaMemcpyFromSymbol(word, g_plan_error_word, sizeof(*word));
+    const unsigned int zero = 0;
+    if (err == cudaSuccess && *word != 0) err = cudaMemcpyToSymbol(g_plan_error_word, &zero, sizeof(zero));
+    return static_cast<int>(err);
+}
+
+}  // namespace fa_sm100_internal
+
+extern "C" {
+
+size_t fa_sm100_paged_schedule_bytes(int num_seqs)
+{
+    return num_seqs < 0 ? 0 : 2 * (static_cast<size_t>(num_seqs) + 1) * sizeof(long long);
+}
+
+int fa_sm100_paged_plan(const FaPagedPlan* plan, const int* cached_lens, const int* new_lens, const int* free_pages,
+                        int num_free, const int* free_start, void* stream)
+{
+    int status = fa_sm100_internal::validate_plan(plan);
+    if (status != FA_STATUS_OK) return status;
+    if (num_free < 0 || (num_free > 0 && free_pages == nullptr)) return FA_STATUS_INVALID_ARGUMENT;
+    if (plan->num_seqs > 0 && (cached_lens == nullptr || new_lens == nullptr)) return FA_STATUS_INVALID_ARGUMENT;
+    int device = 0, sms = 0;
+    status = fa_sm100_internal::current_sm100(&device, &sms);
+    if (status != FA_STATUS_OK) return status;
+    PlanParams params{*plan, cached_lens, new_lens, free_pages, num_free, free_start};
+    long long blocks = ceil_div(plan->total_tokens, kPlanTokensPerCta);
+    if (blocks < 1) blocks = 1;
+    if (blocks > sms) blocks = sms;
+    plan_kernel<<<static_cast<unsigned>(blocks), kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(params);
+    return static_cast<int>(cudaGetLastError());
+}
+
+int fa_sm100_rotary(const void* x, const long long* x_strides, void* out, const long long* out_strides, int batch,
+                    int heads, int seq_len, int head_dim, const int* positions, const long long* position_strides,
+                    const float* inv_freq, int rotary_dim, const int* sections, int axes, int interleaved, int inverse,
+                    void* stream)
+{
+    if (batch < 0 || heads < 0 || seq_len < 0 || x_strides == nullptr || out_strides == nullptr ||
+        position_strides == nullptr || sections == nullptr || axes < 1 || axes > kMaxAxes)
+        return FA_STATUS_INVALID_ARGUMENT;
+    if (head_dim != 64 && head_dim != 128) return FA_STATUS_UNSUPPORTED;
+    if (rotary_dim <= 0 || rotary_dim > head_dim || rotary_dim % 16) return FA_STATUS_INVALID_ARGUMENT;
+    RotaryParams params{};
+    const int status = fill_sections(params, sections, axes, rotary_dim);
+    if (status != FA_STATUS_OK) return status;
+    if (batch == 0 || heads == 0 || seq_len == 0) return FA_STATUS_OK;
+    if (x == nullptr || out == nullptr || positions == nullptr || inv_freq == nullptr) return FA_STATUS_INVALID_ARGUMENT;
+    if (misaligned(x) || misaligned(out) || !multiple_of_8(x_strides, 3) || !multiple_of_8(out_strides, 3))
+        return FA_STATUS_MISALIGNED;
+    params.src[0] = static_cast<const __nv_bfloat16*>(x);
+    params.dst[0] = static_cast<__nv_bfloat16*>(out);
+    params.src_batch = x_strides[0];
+    params.src_head[0] = x_strides[1];
+    params.src_token[0] = x_strides[2];
+    params.dst_batch = out_strides[0];
+    params.dst_head[0] = out_strides[1];
+    params.dst_token[0] = out_strides[2];
+    params.rows[0] = heads;
+    params.batch = batch;
+    params.tokens = seq_len;
+    params.units = head_dim / 16;
+    params.rotary_dim = rotary_dim;
+    params.positions = positions;
+    params.position_axis = position_strides[0];
+    params.position_batch = position_strides[1];
+    params.inv_freq = inv_freq;
+    params.sign = inverse ? -1.0f : 1.0f;
+    return launch_rotary<false>(params, interleaved != 0, static_cast<cudaStream_t>(stream));
+}
+
+int fa_sm100_rotary_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache, void* v_cache,
+                           const long long* strides, int tokens, int heads, int kv_heads, int head_dim, int page_size,
+                           int num_pages, const int* positions, long long position_stride, const int* slots,
+                           const float* inv_freq, int rotary_dim, const int* sections, int axes, int interleaved,
+                           void* stream)
+{
+    if (tokens < 0 || heads < 1 || kv_heads < 1 || strides == nullptr || sections == nullptr || axes < 1 ||
+        axes > kMaxAxes || num_pages < 0)
+        return FA_STATUS_INVALID_ARGUMENT;
+    if (head_dim != 64 && head_dim != 128) return FA_STATUS_UNSUPPORTED;
+    if (!fa_sm100_internal::page_size_supported(page_size)) return FA_STATUS_UNSUPPORTED;
+    if (static_cast<long long>(num_pages) * page_size > INT_MAX) return FA_STATUS_INVALID_ARGUMENT;
+    if (rotary_dim <= 0 || rotary_dim > head_dim || rotary_dim % 16) return FA_STATUS_INVALID_ARGUMENT;
+    RotaryParams params{};
+    const int status = fill_sections(params, sections, axes, rotary_dim);
+    if (status != FA_STATUS_OK) return status;
+    if (tokens == 0) return FA_STATUS_OK;
+    if (q == nullptr || k == nullptr || v == nullptr || q_out == nullptr || k_cache == nullptr || v_cache == nullptr ||
+        positions == nullptr || slots == nullptr || inv_freq == nullptr)
+        return FA_STATUS_INVALID_ARGUMENT;
+    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(q_out) || misaligned(k_cache) ||
+        misaligned(v_cache) || !multiple_of_8(strides, 14))
+        return FA_STATUS_MISALIGNED;
+    params.src[0] = static_cast<const __nv_bfloat16*>(q);
+    params.src[1] = static_cast<const __nv_bfloat16*>(k);
+    params.src[2] = static_cast<const __nv_bfloat16*>(v);
+    params.dst[0] = static_cast<__nv_bfloat16*>(q_out);
+    params.dst[1] = static_cast<__nv_bfloat16*>(k_cache);
+    params.dst[2] = static_cast<__nv_bfloat16*>(v_cache);
+    params.src_token[0] = strides[0];
+    params.src_head[0] = strides[1];
+    params.dst_token[0] = strides[2];
+    params.dst_head[0] = strides[3];
+    params.src_token[1] = strides[4];
+    params.src_head[1] = strides[5];
+    params.src_token[2] = strides[6];
+    params.src_head[2] = strides[7];
+    params.dst_page[1] = strides[8];
+    params.dst_head[1] = strides[9];
+    params.dst_token[1] = strides[10];
+    params.dst_page[2] = strides[11];
+    params.dst_head[2] = strides[12];
+    params.dst_token[2] = strides[13];
+    params.rows[0] = heads;
+    params.rows[1] = kv_heads;
+    params.rows[2] = kv_heads;
+    params.batch = 1;
+    params.tokens = tokens;
+    params.units = head_dim / 16;
+    params.rotary_dim = rotary_dim;
+    params.positions = positions;
+    params.position_axis = position_stride;
+    params.inv_freq = inv_freq;
+    params.slots = slots;
+    params.page_shift = __builtin_ctz(static_cast<unsigned>(page_size));
+    params.num_slots = static_cast<long long>(num_pages) * page_size;
+    params.sign = 1.0f;
+    return launch_rotary<true>(params, interleaved != 0, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

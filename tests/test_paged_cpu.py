@@ -1,0 +1,178 @@
+"""Refusals of the paged-cache operators, made on the host before any CUDA call."""
+import ctypes
+
+import pytest
+import torch
+
+import cuda_fused_attention_b200 as fa
+from cuda_fused_attention_b200 import _lib
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load()
+
+
+def _i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def _bf16(*shape):
+    return torch.zeros(shape, dtype=torch.bfloat16)
+
+
+def _plan(**changes):
+    plan = _lib.FaPagedPlan()
+    values = dict(num_seqs=2, total_tokens=4, max_new=4, num_pages=8, table_width=4, table_stride=4, heads=8, kv_heads=2,
+                  head_dim=128, page_size=16, causal=1, query_start=0x1000, kv_lens=0x1000, positions=0x1000,
+                  slots=0x1000, block_table=0x1000, free_cursor=0x1000, schedule=0x1000)
+    for name, value in {**values, **changes}.items():
+        setattr(plan, name, value)
+    return plan
+
+
+BAD_PLANS = [
+    (dict(head_dim=96), 1002), (dict(page_size=8), 1002), (dict(page_size=48), 1002), (dict(page_size=512), 1002),
+    (dict(heads=7), 1001), (dict(heads=0), 1001), (dict(kv_heads=0), 1001), (dict(heads=129, kv_heads=1), 1002),
+    (dict(num_seqs=-1), 1001), (dict(total_tokens=-1), 1001), (dict(max_new=-1), 1001), (dict(num_pages=-1), 1001),
+    (dict(table_width=-1), 1001), (dict(table_stride=3), 1001), (dict(num_pages=2 ** 27), 1001),
+    (dict(table_width=2 ** 27, table_stride=2 ** 27), 1001), (dict(query_start=None), 1001), (dict(kv_lens=None), 1001),
+    (dict(positions=None), 1001), (dict(slots=None), 1001), (dict(block_table=None), 1001),
+    (dict(free_cursor=None), 1001), (dict(schedule=None), 1001)]
+
+
+@pytest.mark.parametrize("changes,status", BAD_PLANS, ids=lambda v: str(v))
+def test_c_plan_refusals(lib, changes, status):
+    plan = ctypes.byref(_plan(**changes))
+    assert lib.fa_sm100_paged_plan(plan, 0x1000, 0x1000, 0x1000, 4, None, None) == status
+    strides = (ctypes.c_longlong * 10)(*[128] * 10)
+    assert lib.fa_sm100_paged_fwd(plan, 0x1000, 0x1000, 0x1000, 0x1000, strides, 0x1000, 1 << 40, None) == status
+
+
+def test_c_refusals(lib):
+    plan = ctypes.byref(_plan())
+    good = (ctypes.c_longlong * 10)(*[128] * 10)
+    odd = (ctypes.c_longlong * 10)(*[128] * 9, 132)
+    assert lib.fa_sm100_paged_plan(None, 0x1000, 0x1000, 0x1000, 4, None, None) == 1001
+    assert lib.fa_sm100_paged_plan(plan, None, 0x1000, 0x1000, 4, None, None) == 1001
+    assert lib.fa_sm100_paged_plan(plan, 0x1000, None, 0x1000, 4, None, None) == 1001
+    assert lib.fa_sm100_paged_plan(plan, 0x1000, 0x1000, None, 4, None, None) == 1001
+    assert lib.fa_sm100_paged_plan(plan, 0x1000, 0x1000, 0x1000, -1, None, None) == 1001
+    fwd = lib.fa_sm100_paged_fwd
+    assert fwd(None, 0x1000, 0x1000, 0x1000, 0x1000, good, None, 0, None) == 1001
+    for i in range(4):
+        assert fwd(plan, *[None if j == i else 0x1000 for j in range(4)], good, None, 0, None) == 1001
+        assert fwd(plan, *[0x1008 if j == i else 0x1000 for j in range(4)], good, None, 0, None) == 1003
+    assert fwd(plan, 0x1000, 0x1000, 0x1000, 0x1000, None, None, 0, None) == 1001
+    assert fwd(plan, 0x1000, 0x1000, 0x1000, 0x1000, odd, None, 0, None) == 1003
+    assert fwd(ctypes.byref(_plan(total_tokens=0)), None, None, None, None, good, None, 0, None) == 0
+    assert lib.fa_sm100_paged_schedule_bytes(3) == 64 and lib.fa_sm100_paged_schedule_bytes(-1) == 0
+
+
+def test_c_rotary_refusals(lib):
+    three, two = (ctypes.c_longlong * 3)(*[128] * 3), (ctypes.c_longlong * 2)(8, 0)
+    odd = (ctypes.c_longlong * 3)(128, 128, 68)
+    sections = (ctypes.c_int * 4)(16, 24, 24, 0)
+
+    def call(x=0x1000, xs=three, out=0x1000, batch=1, dim=128, positions=0x1000, freq=0x1000, rot=128, axes=3, sec=sections):
+        return lib.fa_sm100_rotary(x, xs, out, three, batch, 2, 3, dim, positions, two, freq, rot, sec, axes, 0, 0, None)
+
+    assert call(batch=0) == 0
+    assert call(dim=80) == 1002
+    for bad in (dict(x=None), dict(out=None), dict(positions=None), dict(freq=None), dict(xs=None), dict(sec=None),
+                dict(batch=-1), dict(rot=130), dict(rot=24), dict(rot=0), dict(axes=0), dict(axes=5), dict(axes=2),
+                dict(rot=64), dict(sec=(ctypes.c_int * 4)(-8, 48, 24, 0))):
+        assert call(**bad) == 1001, bad
+    assert call(x=0x1008) == 1003 and call(xs=odd) == 1003
+
+    strides = (ctypes.c_longlong * 14)(*[128] * 14)
+
+    def append(ptrs=(0x1000,) * 6, s=strides, tokens=2, heads=4, dim=128, page=16, pages=8, slots=0x1000):
+        return lib.fa_sm100_rotary_append(*ptrs, s, tokens, heads, 2, dim, page, pages, 0x1000, 2, slots, 0x1000, 128,
+                                          sections, 3, 0, None)
+
+    assert append(tokens=0) == 0
+    assert append(dim=32) == 1002 and append(page=24) == 1002
+    for i in range(6):
+        assert append(ptrs=[None if j == i else 0x1000 for j in range(6)]) == 1001
+        assert append(ptrs=[0x1002 if j == i else 0x1000 for j in range(6)]) == 1003
+    assert append(slots=None) == 1001 and append(s=None) == 1001 and append(tokens=-1) == 1001
+    assert append(heads=0) == 1001 and append(pages=2 ** 28) == 1001 and append(pages=-1) == 1001
+    assert append(s=(ctypes.c_longlong * 14)(*[128] * 13, 4)) == 1003
+
+
+@pytest.mark.parametrize("args", [(8, 3, 64, 16), (0, 1, 64, 16), (8, 0, 64, 16), (129, 1, 64, 16), (8, 8, 80, 16),
+                                  (8, 8, 64, 24), (8, 8, 64, 8)])
+def test_shape_refusals(args):
+    with pytest.raises(ValueError):
+        fa.PagedShape(*args)
+
+
+def test_python_refusals():
+    shape = fa.PagedShape(8, 2, 64, 16)
+    good = dict(cached_lens=_i32(2), new_lens=_i32(2), block_table=_i32(2, 4), free_pages=_i32(3), total_tokens=5,
+                shape=shape, num_pages=9)
+    for change, error in [
+            (dict(cached_lens=_i32(2).long()), TypeError), (dict(cached_lens=_i32(2, 1)), ValueError),
+            (dict(new_lens=_i32(3)), ValueError), (dict(new_lens=_i32(4)[::2]), ValueError),
+            (dict(block_table=_i32(3, 4)), ValueError), (dict(block_table=_i32(8)), ValueError),
+            (dict(block_table=_i32(4, 2).t()), ValueError), (dict(block_table=_i32(1, 4).expand(2, 4)), ValueError),
+            (dict(free_pages=_i32(3).float()), TypeError), (dict(free_cursor=_i32(2)), ValueError),
+            (dict(total_tokens=-1), ValueError), (dict(num_pages=-1), ValueError), (dict(max_new=-1), ValueError),
+            (dict(num_pages=2 ** 28), ValueError), (dict(total_tokens=2 ** 31), ValueError),
+            ({}, TypeError)]:        # CPU tensors: no silent CPU path
+        with pytest.raises(error):
+            fa.paged_plan(**{**good, **change})
+
+    freq, positions = torch.ones(32), _i32(7)
+    good = dict(x=_bf16(2, 3, 7, 64), positions=positions, inv_freq=freq)
+    for change, error in [
+            (dict(x=_bf16(3, 7, 64)), ValueError), (dict(x=_bf16(2, 3, 7, 32)), ValueError),
+            (dict(x=torch.zeros(2, 3, 7, 64)), TypeError), (dict(x=_bf16(2, 3, 64, 64).transpose(2, 3)), ValueError),
+            (dict(x=_bf16(2, 3, 7, 68)[..., :64]), ValueError), (dict(positions=_i32(8)), ValueError),
+            (dict(positions=_i32(7).long()), TypeError), (dict(positions=_i32(2, 7)), ValueError),
+            (dict(positions=_i32(1, 3, 7)), ValueError), (dict(positions=_i32(7, 1).t()[:, ::1].expand(1, 7)[:, :0]), ValueError),
+            (dict(inv_freq=torch.ones(12)), ValueError), (dict(inv_freq=torch.ones(40)), ValueError),
+            (dict(inv_freq=torch.ones(32).half()), TypeError), (dict(inv_freq=torch.ones(0)), ValueError),
+            (dict(sections=(16, 15)), ValueError), (dict(sections=(16, 17)), ValueError),
+            (dict(sections=(-1, 33)), ValueError), (dict(sections=()), ValueError),
+            (dict(sections=(8, 8, 8, 4, 4)), ValueError), ({}, TypeError)]:
+        with pytest.raises(error):
+            fa.rotary_embed(**{**good, **change})
+
+    good = dict(q=_bf16(5, 4, 64), k=_bf16(5, 2, 64), v=_bf16(5, 2, 64), k_cache=_bf16(3, 2, 16, 64),
+                v_cache=_bf16(3, 2, 16, 64), positions=_i32(5), slots=_i32(5), inv_freq=freq)
+    for change, error in [
+            (dict(q=_bf16(5, 4, 128)), ValueError), (dict(q=_bf16(5, 256)), ValueError), (dict(k=_bf16(4, 2, 64)), ValueError),
+            (dict(v=_bf16(5, 3, 64)), ValueError), (dict(v_cache=_bf16(3, 2, 32, 64)), ValueError),
+            (dict(k_cache=_bf16(3, 2, 24, 64), v_cache=_bf16(3, 2, 24, 64)), ValueError),
+            (dict(k_cache=_bf16(1, 2, 16, 64).expand(3, 2, 16, 64)), ValueError), (dict(slots=_i32(4)), ValueError),
+            (dict(slots=_i32(5).long()), TypeError), (dict(positions=_i32(1, 4)), ValueError),
+            (dict(positions=_i32(2, 5)), ValueError), ({}, TypeError)]:
+        with pytest.raises(error):
+            fa.rotary_append(**{**good, **change})
+
+    plan = fa.paged.PagedPlan(2, 5, shape, torch.device("cpu"))
+    plan.c.num_pages = 3
+    good = dict(q=_bf16(5, 8, 64), k_cache=_bf16(3, 2, 16, 64), v_cache=_bf16(3, 2, 16, 64), plan=plan)
+    for change, error in [
+            (dict(q=_bf16(4, 8, 64)), ValueError), (dict(q=torch.zeros(5, 8, 64)), TypeError),
+            (dict(k_cache=_bf16(4, 2, 16, 64)), ValueError), (dict(v_cache=_bf16(3, 2, 16, 128)), ValueError),
+            (dict(v_cache=_bf16(3, 2, 16, 72)[..., 4:68]), ValueError), ({}, TypeError)]:
+        with pytest.raises(error):
+            fa.paged_attention(**{**good, **change})
+
+
+def test_plan_views_are_the_struct_s_pointers():
+    plan = fa.paged.PagedPlan(3, 7, fa.PagedShape(8, 2, 64, 16), torch.device("cpu"))
+    for name, size in (("query_start", 4), ("kv_lens", 3), ("positions", 7), ("slots", 7), ("free_cursor", 1)):
+        view = getattr(plan, name)
+        assert view.data_ptr() == getattr(plan.c, name) and view.shape == (size,) and view.dtype == torch.int32
+    end = plan.free_cursor.data_ptr() + 4
+    assert end <= plan._buffer.data_ptr() + 8 * plan._buffer.numel()
+    assert plan.c.query_start == plan.c.schedule + _lib.load().fa_sm100_paged_schedule_bytes(3)
+
+
+def test_status_strings(lib):
+    for code in (fa.STATUS_BAD_REQUEST, fa.STATUS_OUT_OF_PAGES, fa.STATUS_WORKSPACE):
+        assert b"unknown" not in lib.fa_sm100_status_string(code)
