@@ -1082,18 +1082,12 @@ int prepare_device(int device)
 // read as zero and are clipped on store.
 int make_map(CUtensorMap* map, const void* ptr, long long slabs, int seq_len, int head_dim)
 {
-    EncodeTiledFn fn = encode_fn();
-    if (fn == nullptr) return FA_STATUS_DRIVER_ENTRY;
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(seq_len),
                                 static_cast<cuuint64_t>(slabs)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_dim) * 2u,
                                    static_cast<cuuint64_t>(seq_len) * static_cast<cuuint64_t>(head_dim) * 2u};
     const cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(kBlockM), 1u};
-    const cuuint32_t elem_strides[3] = {1u, 1u, 1u};
-    const CUresult res = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box,
-                            elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return res == CUDA_SUCCESS ? FA_STATUS_OK : FA_STATUS_TENSOR_MAP;
+    return fa_sm100_internal::encode_map(map, ptr, 3, dims, strides, box);
 }
 
 // The four tensor maps of a call depend only on the base pointers and the shape, so a
@@ -1342,6 +1336,19 @@ int forward(const void* q, const void* k, const void* v, void* o, int batch, int
 }  // namespace
 
 namespace fa_sm100_internal {
+
+int encode_map(CUtensorMap* map, const void* ptr, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+               const cuuint32_t* box)
+{
+    EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return FA_STATUS_DRIVER_ENTRY;
+    const cuuint32_t elem_strides[5] = {1u, 1u, 1u, 1u, 1u};
+    const CUresult res = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank),
+                            const_cast<void*>(ptr), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return res == CUDA_SUCCESS ? FA_STATUS_OK : FA_STATUS_TENSOR_MAP;
+}
 
 int forward_without_workspace(const void* q, const void* k, const void* v, void* o, int batch, int heads,
                               int seq_len, int head_dim, int causal, void* stream)

@@ -3,6 +3,7 @@
 // -fvisibility=hidden and these carry no FA_API).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 namespace fa_sm100_internal {
@@ -20,5 +21,10 @@ int forward_without_workspace(const void* q, const void* k, const void* v, void*
 // on it, so a timeout of a launch that another caller made at the same time
 // can be reported here instead of there.
 int take_error_word(cudaStream_t stream, unsigned int* word);
+
+// Encodes a bf16 tensor map (128-byte swizzle, zero fill out of range; strides in bytes, of
+// dimensions 1 to rank - 1). FA_STATUS_OK, FA_STATUS_DRIVER_ENTRY or FA_STATUS_TENSOR_MAP.
+int encode_map(CUtensorMap* map, const void* ptr, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+               const cuuint32_t* box);
 
 }  // namespace fa_sm100_internal
