@@ -27,6 +27,7 @@ struct PagedParams {
     long long k_page, k_head, k_row, v_page, v_head, v_row;
     int page_shift;
     float scale_log2;
+    float* wide_partial;        // the same of the wide kernel's blocks
     float* partial;             // parts of items that cross a border between CTAs' ranges
 };
 
@@ -470,51 +471,675 @@ combine_narrow_kernel(const __grid_constant__ PagedParams p, int ctas)
         *reinterpret_cast<uint32_t*>(out + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
 }
 
-// One warp per query row: a lane holds D / 32 elements of q and of the accumulator.
+// =============================================================================
+// Wide kernel: requests of more than 16 query rows per K/V head (chunks of tokens)
+// =============================================================================
+// The query rows of a K/V head (token * group + head in group) are taken 128 at a time as the M
+// of tcgen05 products, so that all heads of a group share each K/V tile; a block is two such
+// tiles (256 rows) that ping-pong between two softmax warpgroups, as in the dense kernel. The
+// arithmetic is 4 D operations per (row, key) against 4 D bytes per key and block, so the tensor
+// pipe and the exponentials bound it, not memory. The work of all requests, K/V heads and blocks
+// is one line of 128-key tiles (request, head, block, key) of which each of the grid's CTAs (one
+// per SM, persistent) takes an equal stretch; blocks that cross a border are merged from parts by
+// combine_wide_kernel. Within a CTA the K/V ring runs on across blocks, the first products of a
+// block overlap the epilogue of the one before.
+//
+// Warps: 0-3 and 4-7 softmax, O correction and epilogue of Q tile 0 and 1 (one thread per row);
+// 8 MMA issuer; 9 TMA producer; 10 zeroes what V's last page holds behind the last key (a weight
+// of zero does not silence a NaN); 11 walks the line and hands out the segments.
+// Tensor memory, barriers per key tile, register split and the lazily moved exponent base are
+// those of the dense kernel (fa_sm100.cu). P is rounded to bf16 for the product with V.
+constexpr int kWideThreads = 384;
+constexpr int kWideMinTiles = 2;        // tiles a CTA takes at least
+constexpr uint32_t kWideRegsLaunch = 168, kWideRegsSoftmax = 216, kWideRegsOther = 72;
+static_assert(2 * 128 * kWideRegsSoftmax + 128 * kWideRegsOther <= kWideThreads * kWideRegsLaunch,
+              "the warpgroup register split must fit in the registers the CTA launches with");
+
+enum WideSite : uint32_t {
+    kSiteWideSched = 40, kSiteWideQ = 41, kSiteWideK = 42, kSiteWideV = 43, kSiteWideP = 44, kSiteWideEmpty = 45,
+    kSiteWideS = 46, kSiteWideO = 47, kSiteWideTail = 48,
+};
+
 template <int D>
-__global__ void __launch_bounds__(128)
-paged_rows_kernel(const PagedParams p)
+struct WideCfg {
+    static constexpr int kSub = D / 64;                         // 64-column swizzle blocks per row
+    static constexpr int kSubBytes = kWideRows * 128;
+    static constexpr int kTileBytes = kSub * kSubBytes;         // one Q, K or V tile
+    static constexpr int kStages = D == 128 ? 4 : 8;
+    static constexpr int kRingOff = 2 * kTileBytes;
+    static constexpr int kBarOff = kRingOff + kStages * kTileBytes;
+    static constexpr int kBarQFull = 0, kBarQEmpty = 1;
+    static constexpr int kBarKvFull = 2, kBarKvEmpty = 2 + kStages;
+    static constexpr int kBarSFull = 2 + 2 * kStages;           // per Q tile from here
+    static constexpr int kBarPHalf = kBarSFull + 2;
+    static constexpr int kBarPFull = kBarPHalf + 2;
+    static constexpr int kBarPvHalf = kBarPFull + 2;
+    static constexpr int kBarOFull = kBarPvHalf + 2;
+    static constexpr int kBarTail = kBarOFull + 2;              // per ring slot: a V tile to be zeroed in part has landed
+    static constexpr int kBarDrain = kBarTail + kStages;
+    static constexpr int kBarSchedFull = kBarDrain + 1;
+    static constexpr int kBarSchedEmpty = kBarSchedFull + 2;
+    static constexpr int kNumBars = kBarSchedEmpty + 2;
+    static constexpr int kMiscOff = kBarOff + kNumBars * 8;     // tensor memory base, abort flag
+    static constexpr int kSegOff = (kMiscOff + 8 + 15) / 16 * 16;
+    static constexpr int kSmemBytes = kSegOff + 2 * 64 + 1024;
+    static constexpr uint32_t kColS0 = 0, kColS1 = 128, kColO0 = 256, kColO1 = 256 + D;
+    static constexpr uint32_t kIdescQK = make_idesc_bf16(kWideRows, kWideKeys, false);
+    static constexpr uint32_t kIdescPV = make_idesc_bf16(kWideRows, D, true);
+    // A part: per Q tile O as [D / 4][128 rows] of float4, then 128 maxima and 128 sums.
+    static constexpr int kPartTileFloats = kWideRows * (D + 2);
+    static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
+
+// A stretch of one block inside a CTA's range.
+struct WideSegment {
+    int b, h;
+    int token0;             // packed row of the block's first token
+    int tokens;             // tokens of the block, at most 2 * tokens_per_tile
+    int pos0;               // position of its first token
+    int kv;                 // keys of the request
+    int tile, count;        // key tiles [tile, tile + count) of the block; count 0 ends the walk
+    int part;               // place of its part, -1: the whole block, written directly
+    int zero_from, zero_to; // rows of the last V tile that must read as zero ([0, 0): none)
+    int reserved;
+    long long first, last;  // the block's tiles on the line (combine)
+};
+static_assert(sizeof(WideSegment) == 64, "segment slots");
+
+__device__ inline WideSegment wide_segment(const FaPagedPlan& plan, const long long* start, long long x, long long end)
 {
-    constexpr int E = D / 32;
-    const FaPagedPlan& plan = p.plan;
-    const int lane = threadIdx.x % 32;
-    const long long row = (static_cast<long long>(blockIdx.x) * 128 + threadIdx.x) / 32;
-    const int token = static_cast<int>(row / plan.heads);
-    const int head = static_cast<int>(row % plan.heads);
-    if (token >= plan.query_start[plan.num_seqs]) return;
-    int lo = 0, hi = plan.num_seqs - 1;
+    WideSegment s;
+    s.b = find_request(start, plan.num_seqs, x / plan.kv_heads);
+    const long long tiles = start[s.b + 1] - start[s.b], base = start[s.b] * plan.kv_heads;
+    s.h = static_cast<int>((x - base) / tiles);
+    const long long head_first = base + s.h * tiles;
+    const int n = plan.query_start[s.b + 1] - plan.query_start[s.b];
+    s.kv = plan.kv_lens[s.b];
+    const int cached = s.kv - n;
+    const int span = 2 * tokens_per_tile(plan.heads / plan.kv_heads);
+    const bool causal = plan.causal != 0;
+    int lo = 0, hi = (n - 1) / span;        // last block whose tiles begin at or before x
     while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (plan.query_start[mid] <= token) lo = mid;
+        const int mid = (lo + hi + 1) >> 1;
+        if (head_first + wide_tiles_through(mid, span, cached, n, causal) <= x) lo = mid;
         else hi = mid - 1;
     }
-    const int start = plan.query_start[lo], n = plan.query_start[lo + 1] - start, kv = plan.kv_lens[lo];
-    if (kv < n || n * (plan.heads / plan.kv_heads) <= kNarrowRows) return;
-    const int keys = plan.causal ? kv - n + (token - start) + 1 : kv;
-    const int kv_head = head / (plan.heads / plan.kv_heads);
-    float q[E], acc[E] = {}, m = -INFINITY, l = 0.0f;
-    for (int e = 0; e < E; ++e) q[e] = __bfloat162float(p.q[token * p.q_token + head * p.q_head + lane * E + e]);
-    for (int j = 0; j < keys; ++j) {
-        const int page = plan.block_table[static_cast<long long>(lo) * plan.table_stride + (j >> p.page_shift)];
-        if (page < 0 || page >= plan.num_pages) {
-            atomicOr(&g_paged_error_word, FA_ERROR_BAD_PAGE);
-            return;
-        }
-        const int r = j & ((1 << p.page_shift) - 1);
-        const __nv_bfloat16* k = p.k + page * p.k_page + kv_head * p.k_head + r * p.k_row + lane * E;
-        const __nv_bfloat16* v = p.v + page * p.v_page + kv_head * p.v_head + r * p.v_row + lane * E;
-        float dot = 0.0f;
-        for (int e = 0; e < E; ++e) dot += q[e] * __bfloat162float(k[e]);
-        for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-        const float s = dot * p.scale_log2;
-        const float top = fmaxf(m, s);
-        const float keep = exp2f(m - top), w = exp2f(s - top);
-        l = l * keep + w;
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * keep + w * __bfloat162float(v[e]);
-        m = top;
+    s.first = head_first + wide_tiles_through(lo, span, cached, n, causal);
+    s.last = s.first + wide_tiles_of(lo, span, cached, n, causal);
+    s.token0 = plan.query_start[s.b] + lo * span;
+    s.tokens = min(span, n - lo * span);
+    s.pos0 = cached + lo * span;
+    s.tile = static_cast<int>(x - s.first);
+    s.count = static_cast<int>((s.last < end ? s.last : end) - x);
+    s.part = -1;
+    s.reserved = 0;
+    // Behind the last key: rows of the last page (pages behind it are zero-filled by the copy).
+    const int v0 = (s.tile + s.count - 1) * kWideKeys;
+    const int held = (s.kv + plan.page_size - 1) / plan.page_size * plan.page_size;
+    s.zero_from = s.kv - v0;
+    s.zero_to = min(kWideKeys, held - v0);
+    if (s.zero_from >= s.zero_to) s.zero_from = s.zero_to = 0;
+    return s;
+}
+
+__device__ __forceinline__ long long wide_share(long long total, int ctas)
+{
+    const long long even = (total + ctas - 1) / ctas;
+    return even > kWideMinTiles ? even : kWideMinTiles;
+}
+
+template <int D>
+__device__ __forceinline__ void wide_issue_qk(uint32_t d_tmem, uint32_t q_saddr, uint32_t k_saddr)
+{
+    using C = WideCfg<D>;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off = static_cast<uint32_t>((kk >> 2) * C::kSubBytes + (kk & 3) * 32);
+        umma_ss(d_tmem, make_smem_desc(q_saddr + off, 16, 1024), make_smem_desc(k_saddr + off, 16, 1024), C::kIdescQK,
+                kk > 0 ? 1u : 0u);
     }
-    for (int e = 0; e < E; ++e)
-        p.o[token * p.o_token + head * p.o_head + lane * E + e] = __float2bfloat16_rn(acc[e] / l);
+}
+
+template <int D, int kFirst, int kLast>
+__device__ __forceinline__ void wide_issue_pv(uint32_t d_tmem, uint32_t p_tmem, uint32_t v_saddr, bool accumulate)
+{
+    using C = WideCfg<D>;
+#pragma unroll
+    for (int kk = kFirst; kk < kLast; ++kk)
+        umma_ts(d_tmem, p_tmem + static_cast<uint32_t>(kk * 8),
+                make_smem_desc(v_saddr + static_cast<uint32_t>(kk * 16 * 128), C::kSubBytes, 1024), C::kIdescPV,
+                (accumulate || kk > 0) ? 1u : 0u);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kWideThreads, 1)
+paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedParams p)
+{
+    using C = WideCfg<D>;
+    const FaPagedPlan& plan = p.plan;
+    const long long* start = wide_starts(plan.schedule, plan.num_seqs);
+    const long long total = start[plan.num_seqs] * plan.kv_heads;
+    const long long share = wide_share(total, gridDim.x);
+    const long long begin = share * blockIdx.x;
+    if (begin >= total) return;
+    const long long end = begin + share < total ? begin + share : total;
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (base - raw);
+    const uint32_t ring = base + C::kRingOff;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
+    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + C::kMiscOff + 4);
+    WideSegment* segments = reinterpret_cast<WideSegment*>(smem + C::kSegOff);
+    auto bar = [&](int index) -> uint32_t { return base + C::kBarOff + static_cast<uint32_t>(index) * 8u; };
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    constexpr int kMma = 8, kLoad = 9, kTail = 10;
+    constexpr int kReaders = 11;            // warps that read a segment slot
+
+    if (warp == 0) {
+        for (int i = lane; i < C::kNumBars; i += 32) {
+            uint32_t count = 1;
+            if (i >= C::kBarPHalf && i < C::kBarPvHalf) count = 128;
+            if (i >= C::kBarSchedEmpty) count = kReaders;
+            mbar_init(bar(i), count);
+        }
+        if (lane == 0) *abort_flag = 0u;
+        fence_mbarrier_init();
+    }
+    if (warp == kMma) {
+        tmem_alloc(smem_u32(tmem_slot), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int group = plan.heads / plan.kv_heads;
+    const int per_tile = tokens_per_tile(group);
+
+    // Takes segment number sg: every lane of a reading warp gets the values. False: gave up.
+    auto take_segment = [&](int sg, WideSegment& s) -> bool {
+        if (!__all_sync(0xffffffffu, wait_paged(bar(C::kBarSchedFull + (sg & 1)), (sg >> 1) & 1, abort_flag, kSiteWideSched)))
+            return false;
+        s = segments[sg & 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::kBarSchedEmpty + (sg & 1)));
+        return true;
+    };
+
+    if (warp >= kMma) {
+        regs_decrease<kWideRegsOther>();
+        if (warp == kLoad) {
+            // ======================= TMA producer ==============================
+            const int rows = plan.page_size < kWideKeys ? plan.page_size : kWideKeys;
+            const int pages = kWideKeys / rows;
+            const bool active = lane < pages * C::kSub;
+            const int page_of_tile = lane / C::kSub, block = lane % C::kSub;
+            const uint32_t offset = static_cast<uint32_t>(block * C::kSubBytes + page_of_tile * rows * 128);
+            int ri = 0;                 // ring index of the next K or V tile
+            int q_loads = 0;
+            uint32_t tail_slots = 0, tail_parity = 0;      // slots whose latest load went by the tail warp; their phases
+            bool ok = true;
+            WideSegment s;
+            for (int sg = 0; ok; ++sg) {
+                ok = take_segment(sg, s);
+                if (!ok || s.count == 0) break;
+                if (sg > 0 && !__all_sync(0xffffffffu, wait_paged(bar(C::kBarQEmpty), (sg - 1) & 1, abort_flag, kSiteWideQ))) {
+                    ok = false;
+                    break;
+                }
+                const int tiles = s.tokens > per_tile ? 2 : 1;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(bar(C::kBarQFull), static_cast<uint32_t>(tiles * C::kSub * 128 * group * per_tile));
+                    for (int t = 0; t < tiles; ++t)
+                        for (int sub = 0; sub < C::kSub; ++sub)
+                            tma_load_3d(base + t * C::kTileBytes + sub * C::kSubBytes, &tm_q, bar(C::kBarQFull), sub * 64,
+                                        s.h * group, s.token0 + t * per_tile);
+                }
+                ++q_loads;
+                const int* table = plan.block_table + static_cast<long long>(s.b) * plan.table_stride;
+                const int held = (s.kv + plan.page_size - 1) >> p.page_shift;
+                auto page_at = [&](int tile) -> int {
+                    // num_pages is out of the map's range: such a box reads as zeros.
+                    const int i = ((tile * kWideKeys) >> p.page_shift) + page_of_tile;
+                    if (!active || i >= held) return plan.num_pages;
+                    const int page = __ldg(table + i);
+                    if (page >= 0 && page < plan.num_pages) return page;
+                    atomicOr(&g_paged_error_word, FA_ERROR_BAD_PAGE);
+                    return plan.num_pages;
+                };
+                int page = page_at(s.tile);
+                for (int i = 0; ok && i < s.count; ++i) {
+                    const int row = pages > 1 ? 0 : ((s.tile + i) * kWideKeys) & (plan.page_size - 1);
+                    for (int kv = 0; kv < 2; ++kv, ++ri) {
+                        const int slot = ri % C::kStages, use = ri / C::kStages;
+                        if (use > 0 && !__all_sync(0xffffffffu, wait_paged(bar(C::kBarKvEmpty + slot), (use - 1) & 1,
+                                                                           abort_flag, kSiteWideEmpty))) {
+                            ok = false;
+                            break;
+                        }
+                        // A V tile to be zeroed in part lands on the tail warp's barrier, and that warp then
+                        // completes the slot's.
+                        const bool tail = kv == 1 && i + 1 == s.count && s.zero_to > s.zero_from;
+                        const uint32_t landed = bar((tail ? C::kBarTail : C::kBarKvFull) + slot);
+                        tail_slots = tail ? tail_slots | (1u << slot) : tail_slots & ~(1u << slot);
+                        if (tail) tail_parity ^= 1u << slot;
+                        if (lane == 0) mbar_arrive_expect_tx(landed, C::kTileBytes);
+                        __syncwarp();
+                        if (active)
+                            tma_load_4d(ring + slot * C::kTileBytes + offset, kv ? &tm_v : &tm_k, landed, block * 64, row,
+                                        s.h, page);
+                    }
+                    if (ok && i + 1 < s.count) page = page_at(s.tile + i + 1);
+                }
+            }
+            if (!ok && lane == 0) {
+                if (q_loads > 0) drain_paged(bar(C::kBarQFull), (q_loads - 1) & 1);
+                for (int i = ri > C::kStages ? ri - C::kStages : 0; i < ri; ++i) {
+                    const int slot = i % C::kStages;
+                    if (tail_slots >> slot & 1u) drain_paged(bar(C::kBarTail + slot), (tail_parity >> slot & 1u) ^ 1u);
+                    else drain_paged(bar(C::kBarKvFull + slot), (i / C::kStages) & 1);
+                }
+            }
+        } else if (warp == kMma) {
+            // ======================= MMA issuer ================================
+            const uint32_t t_s0 = tmem_base + C::kColS0, t_s1 = tmem_base + C::kColS1;
+            const uint32_t t_o0 = tmem_base + C::kColO0, t_o1 = tmem_base + C::kColO1;
+            const uint32_t sq0 = base, sq1 = base + C::kTileBytes;
+            auto slot_addr = [&](int i) -> uint32_t { return ring + (i % C::kStages) * C::kTileBytes; };
+            auto empty_bar = [&](int i) -> uint32_t { return bar(C::kBarKvEmpty + i % C::kStages); };
+            int ri = 0, c0 = 0, c1 = 0;
+            bool ok = true;
+            WideSegment s;
+            auto wait = [&](int index, uint32_t parity, uint32_t site) {
+                return wait_paged(bar(index), parity & 1u, abort_flag, site);
+            };
+            auto wait_ring = [&](int i, uint32_t site) {
+                return wait_paged(bar(C::kBarKvFull + i % C::kStages), (i / C::kStages) & 1, abort_flag, site);
+            };
+            for (int sg = 0; ok; ++sg) {
+                ok = take_segment(sg, s);
+                if (!ok || s.count == 0) break;
+                if (lane == 0) {
+                    const bool two = s.tokens > per_tile;
+                    ok = wait(C::kBarQFull, sg, kSiteWideQ) && wait_ring(ri, kSiteWideK);
+                    if (ok) {
+                        tc_fence_after();
+                        wide_issue_qk<D>(t_s0, sq0, slot_addr(ri));
+                        umma_commit(bar(C::kBarSFull + 0));
+                        if (two) {
+                            wide_issue_qk<D>(t_s1, sq1, slot_addr(ri));
+                            umma_commit(bar(C::kBarSFull + 1));
+                        }
+                        umma_commit(empty_bar(ri));
+                        if (s.count == 1) umma_commit(bar(C::kBarQEmpty));
+                    }
+                    for (int j = 0; ok && j < s.count; ++j) {
+                        const int vi = ri + 2 * j + 1, ki = vi + 1;
+                        const bool more = j + 1 < s.count;
+                        if (!wait_ring(vi, kSiteWideV)) { ok = false; break; }
+                        if (!wait(C::kBarPHalf + 0, c0 + j, kSiteWideP)) { ok = false; break; }
+                        tc_fence_after();
+                        wide_issue_pv<D, 0, 4>(t_o0, t_s0, slot_addr(vi), j > 0);
+                        umma_commit(bar(C::kBarPvHalf + 0));
+                        if (!wait(C::kBarPFull + 0, c0 + j, kSiteWideP)) { ok = false; break; }
+                        tc_fence_after();
+                        wide_issue_pv<D, 4, 8>(t_o0, t_s0, slot_addr(vi), true);
+                        if (!more) umma_commit(bar(C::kBarOFull + 0));
+                        if (more) {
+                            if (!wait_ring(ki, kSiteWideK)) { ok = false; break; }
+                            tc_fence_after();
+                            wide_issue_qk<D>(t_s0, sq0, slot_addr(ki));
+                            umma_commit(bar(C::kBarSFull + 0));
+                        }
+                        if (two) {
+                            if (!wait(C::kBarPHalf + 1, c1 + j, kSiteWideP)) { ok = false; break; }
+                            tc_fence_after();
+                            wide_issue_pv<D, 0, 4>(t_o1, t_s1, slot_addr(vi), j > 0);
+                            umma_commit(bar(C::kBarPvHalf + 1));
+                            if (!wait(C::kBarPFull + 1, c1 + j, kSiteWideP)) { ok = false; break; }
+                            tc_fence_after();
+                            wide_issue_pv<D, 4, 8>(t_o1, t_s1, slot_addr(vi), true);
+                            if (!more) umma_commit(bar(C::kBarOFull + 1));
+                        }
+                        umma_commit(empty_bar(vi));
+                        if (more) {
+                            if (two) {
+                                wide_issue_qk<D>(t_s1, sq1, slot_addr(ki));
+                                umma_commit(bar(C::kBarSFull + 1));
+                            }
+                            umma_commit(empty_bar(ki));
+                            if (j + 2 == s.count) umma_commit(bar(C::kBarQEmpty));
+                        }
+                    }
+                    ri += 2 * s.count;
+                    c0 += s.count;
+                    if (two) c1 += s.count;
+                }
+                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            }
+            if (lane == 0) {
+                // Every MMA issued above must finish before tensor memory is released.
+                umma_commit(bar(C::kBarDrain));
+                drain_paged(bar(C::kBarDrain), 0);
+            }
+            __syncwarp();
+        } else if (warp == kTail) {
+            // ======================= zeroes behind the last key ================
+            int ri = 0;
+            uint32_t parity = 0;
+            WideSegment s;
+            for (int sg = 0; take_segment(sg, s) && s.count > 0; ++sg) {
+                if (s.zero_to > s.zero_from) {
+                    const int vi = ri + 2 * s.count - 1, slot = vi % C::kStages;
+                    if (!__all_sync(0xffffffffu, wait_paged(bar(C::kBarTail + slot), parity >> slot & 1u, abort_flag, kSiteWideTail)))
+                        break;
+                    parity ^= 1u << slot;
+                    const int bytes = (s.zero_to - s.zero_from) * 128;
+                    for (int sub = 0; sub < C::kSub; ++sub) {
+                        uint8_t* at = smem + C::kRingOff + slot * C::kTileBytes + sub * C::kSubBytes + s.zero_from * 128;
+                        for (int i = lane * 16; i < bytes; i += 512) *reinterpret_cast<uint4*>(at + i) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(C::kBarKvFull + slot));
+                }
+                ri += 2 * s.count;
+            }
+        } else if (lane == 0) {
+            // ======================= the walk along the line ===================
+            long long x = begin;
+            for (int sg = 0;; ++sg) {
+                if (sg > 1 && !wait_paged(bar(C::kBarSchedEmpty + (sg & 1)), ((sg >> 1) - 1) & 1, abort_flag, kSiteWideSched))
+                    break;
+                WideSegment s;
+                if (x < end) {
+                    s = wide_segment(plan, start, x, end);
+                    // A block that began before this CTA's range leaves its part in the CTA's first place, one
+                    // that goes on behind it in the second.
+                    if (s.first < begin) s.part = 2 * static_cast<int>(blockIdx.x);
+                    else if (s.last > end) s.part = 2 * static_cast<int>(blockIdx.x) + 1;
+                    x += s.count;
+                } else {
+                    s.count = 0;
+                }
+                segments[sg & 1] = s;
+                mbar_arrive(bar(C::kBarSchedFull + (sg & 1)));
+                if (s.count == 0) break;
+            }
+        }
+        __syncwarp();
+    } else {
+        // ======================= softmax / correction / epilogue ================
+        regs_increase<kWideRegsSoftmax>();
+        const int t = warp / 4;                    // Q tile of this warpgroup
+        const int quarter = warp % 4;
+        const int r = quarter * 32 + lane;         // row within the Q tile == tensor-memory lane
+        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        const uint32_t t_s = lane_base + (t == 0 ? C::kColS0 : C::kColS1);
+        const uint32_t t_o = lane_base + (t == 0 ? C::kColO0 : C::kColO1);
+        const int tok = t * per_tile + r / group;       // token of this row within its block
+        const bool in_tile = r < per_tile * group;
+        const float sl2 = p.scale_log2;
+        const uint64_t c2 = f2_pack(sl2, sl2);
+        uint32_t phase = 0;                        // parity of this tile's per-key-tile barriers
+        uint32_t o_phase = 0;
+
+        auto rescale_o = [&](float scale) {
+            const uint64_t a2 = f2_pack(scale, scale);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(t_o + static_cast<uint32_t>(c * 32), o);
+                tmem_wait_ld();
+                reg_fence32(o);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float o0, o1;
+                    f2_unpack(fmul2(f2_pack(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), a2), o0, o1);
+                    o[2 * i] = __float_as_uint(o0);
+                    o[2 * i + 1] = __float_as_uint(o1);
+                }
+                tmem_st32(t_o + static_cast<uint32_t>(c * 32), o);
+            }
+        };
+        // 64 scores on base `mb`: P as bf16 pairs to tensor memory, the 32-bit sum and the raw maximum.
+        auto exp_half = [&](const uint32_t (&lo)[32], const uint32_t (&hi)[32], float mb, float& half_sum, float& half_max,
+                            uint32_t p_tmem) {
+            const uint64_t nb2 = f2_pack(-mb, -mb);
+            uint64_t sum_a = f2_pack(0.0f, 0.0f), sum_b = f2_pack(0.0f, 0.0f);
+            float ma = fmaxf(__uint_as_float(lo[0]), __uint_as_float(lo[1])), mb_ = __uint_as_float(hi[0]);
+            uint32_t out[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const uint32_t (&src)[32] = (i < 16) ? lo : hi;
+                const int k = (i & 15) * 2;
+                if (i >= 16) mb_ = max3f(mb_, __uint_as_float(src[k]), __uint_as_float(src[k + 1]));
+                else if (i > 0) ma = max3f(ma, __uint_as_float(src[k]), __uint_as_float(src[k + 1]));
+                const uint64_t x = ffma2(f2_pack(__uint_as_float(src[k]), __uint_as_float(src[k + 1])), c2, nb2);
+                float x0, x1;
+                f2_unpack(x, x0, x1);
+                const uint64_t pr = f2_pack(ex2_approx(x0), ex2_approx(x1));
+                if (i & 1) sum_b = fadd2(sum_b, pr);
+                else sum_a = fadd2(sum_a, pr);
+                float p0, p1;
+                f2_unpack(pr, p0, p1);
+                out[i] = pack_bf16x2(p0, p1);
+                if (i == 15) tmem_st16(p_tmem, *reinterpret_cast<uint32_t (*)[16]>(&out[0]));
+                if (i == 31) tmem_st16(p_tmem + 16, *reinterpret_cast<uint32_t (*)[16]>(&out[16]));
+            }
+            float sa0, sa1, sb0, sb1;
+            f2_unpack(sum_a, sa0, sa1);
+            f2_unpack(sum_b, sb0, sb1);
+            half_sum = (sa0 + sa1) + (sb0 + sb1);
+            half_max = fmaxf(ma, mb_);
+        };
+
+        bool ok = true;
+        for (int sg = 0; ok; ++sg) {
+            // The slot stays this segment's until the epilogue has read it.
+            ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarSchedFull + (sg & 1)), (sg >> 1) & 1, abort_flag, kSiteWideSched));
+            if (!ok) break;
+            const WideSegment& seg = segments[sg & 1];
+            const int count = seg.count;
+            if (count == 0) break;
+            if (t == 1 && seg.tokens <= per_tile) {     // this block has one tile
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(C::kBarSchedEmpty + (sg & 1)));
+                continue;
+            }
+            const int tile = seg.tile;
+            const int limit = plan.causal ? min(seg.pos0 + tok, seg.kv - 1) : seg.kv - 1;
+            // First key tile of the stretch that some row of this Q tile must not see all of.
+            const int mask_from = (plan.causal ? seg.pos0 + t * per_tile + 1 : seg.kv) / kWideKeys - tile;
+            float row_max = -INFINITY, row_sum = 0.0f, m_base = 0.0f;
+            for (int j = 0; j < count; ++j, phase ^= 1u) {
+                ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarSFull + t), phase, abort_flag, kSiteWideS));
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t sc[4][32];
+                tmem_ld32(t_s + 0, sc[0]);
+                tmem_ld32(t_s + 32, sc[1]);
+                tmem_ld32(t_s + 64, sc[2]);
+                tmem_ld32(t_s + 96, sc[3]);
+                tmem_wait_ld();
+                reg_fence32(sc[0]);
+                reg_fence32(sc[1]);
+                reg_fence32(sc[2]);
+                reg_fence32(sc[3]);
+                if (j >= mask_from) {
+                    const int key0 = (tile + j) * kWideKeys;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (key0 + c * 32 + i > limit) sc[c][i] = __float_as_uint(-INFINITY);
+                }
+                if (j == 0) {
+                    float mx[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float a = __uint_as_float(sc[c][0]), b = __uint_as_float(sc[c][1]);
+#pragma unroll
+                        for (int i = 2; i < 32; i += 2) {
+                            a = fmaxf(a, __uint_as_float(sc[c][i]));
+                            b = fmaxf(b, __uint_as_float(sc[c][i + 1]));
+                        }
+                        mx[c] = fmaxf(a, b);
+                    }
+                    row_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    m_base = row_max == -INFINITY ? 0.0f : row_max * sl2;
+                }
+                float o_scale = 1.0f;       // O correction owed before the first PV of this tile reads O
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float hsum, hmax;
+                    exp_half(sc[2 * h], sc[2 * h + 1], m_base, hsum, hmax, t_s + static_cast<uint32_t>(32 * h));
+                    const bool need = (hmax - row_max) * sl2 > kRebase;
+                    if (__any_sync(0xffffffffu, need)) {
+                        const float m_new = need ? hmax : row_max;
+                        const float alpha = need ? ex2_approx(row_max * sl2 - m_new * sl2) : 1.0f;
+                        row_sum *= alpha;
+                        row_max = m_new;
+                        m_base = row_max == -INFINITY ? 0.0f : row_max * sl2;
+                        if (h == 0) {
+                            o_scale = alpha;
+                        } else {
+                            // The first-half PV of this tile may be running on the old base: let it finish, then
+                            // correct O, its contribution included.
+                            ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarPvHalf + t), phase, abort_flag, kSiteWideO));
+                            if (!ok) break;
+                            tc_fence_after();
+                            rescale_o(alpha);
+                        }
+                        exp_half(sc[2 * h], sc[2 * h + 1], m_base, hsum, hmax, t_s + static_cast<uint32_t>(32 * h));
+                    }
+                    row_sum += hsum;
+                    if (h == 0) {
+                        if (j > 0 && __any_sync(0xffffffffu, o_scale != 1.0f)) rescale_o(o_scale);
+                        tmem_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(bar(C::kBarPHalf + t));
+                    }
+                }
+                if (!ok) break;
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(bar(C::kBarPFull + t));
+            }
+            if (!ok) break;
+
+            // ---- epilogue: O from tensor memory, to its rows or to this stretch's part ----
+            ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarOFull + t), o_phase, abort_flag, kSiteWideO));
+            if (!ok) break;
+            o_phase ^= 1u;
+            tc_fence_after();
+            const int part = seg.part;
+            const bool real = in_tile && tok < seg.tokens;
+            __nv_bfloat16* out = p.o + static_cast<long long>(seg.token0 + tok) * p.o_token +
+                                 static_cast<long long>(seg.h * group + r % group) * p.o_head;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(C::kBarSchedEmpty + (sg & 1)));
+            if (part < 0) {
+                const float inv = 1.0f / row_sum;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(t_o + static_cast<uint32_t>(c * 32), o);
+                    tmem_wait_ld();
+                    reg_fence32(o);
+                    if (real) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                w[i] = pack_bf16x2(__uint_as_float(o[8 * q + 2 * i]) * inv, __uint_as_float(o[8 * q + 2 * i + 1]) * inv);
+                            *reinterpret_cast<uint4*>(out + c * 32 + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                }
+            } else {
+                float* mine = p.wide_partial + (static_cast<long long>(part) * 2 + t) * C::kPartTileFloats;
+                float4* columns = reinterpret_cast<float4*>(mine);
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(t_o + static_cast<uint32_t>(c * 32), o);
+                    tmem_wait_ld();
+                    reg_fence32(o);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        columns[(c * 8 + q) * kWideRows + r] =
+                            make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]),
+                                        __uint_as_float(o[4 * q + 2]), __uint_as_float(o[4 * q + 3]));
+                }
+                mine[D * kWideRows + r] = row_max;
+                mine[D * kWideRows + kWideRows + r] = row_sum;
+            }
+        }
+        tc_fence_before();
+    }
+
+    __syncthreads();
+    if (warp == kMma) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// One block row per border between two CTAs' ranges; the first border inside a block of tokens merges
+// its parts, in their order. A thread is a query row and takes 32 columns of one Q tile.
+template <int D>
+__global__ void __launch_bounds__(kWideRows)
+combine_wide_kernel(const __grid_constant__ PagedParams p, int ctas)
+{
+    using C = WideCfg<D>;
+    const FaPagedPlan& plan = p.plan;
+    const long long* start = wide_starts(plan.schedule, plan.num_seqs);
+    const long long total = start[plan.num_seqs] * plan.kv_heads;
+    const long long share = wide_share(total, ctas);
+    const long long border = share * (blockIdx.x + 1);
+    if (border >= total) return;
+    const WideSegment s = wide_segment(plan, start, border, total);
+    if (s.first == border || s.first < border - share) return;
+    const int group = plan.heads / plan.kv_heads, per_tile = tokens_per_tile(group);
+    const int t = blockIdx.y / (D / 32), c = blockIdx.y % (D / 32), r = threadIdx.x;
+    const int tok = t * per_tile + r / group;
+    if (r >= per_tile * group || tok >= s.tokens) return;
+    const long long c0 = s.first / share, c1 = (s.last - 1) / share;
+    auto part = [&](long long cta) {
+        return p.wide_partial + ((2 * cta + (cta == c0 ? 1 : 0)) * 2 + t) * C::kPartTileFloats;
+    };
+    float top = -INFINITY;
+    for (long long cta = c0; cta <= c1; ++cta) top = fmaxf(top, part(cta)[D * kWideRows + r]);
+    float4 acc[8] = {};
+    float sum = 0.0f;
+    for (long long cta = c0; cta <= c1; ++cta) {
+        const float* at = part(cta);
+        const float m = at[D * kWideRows + r];
+        const float w = m == -INFINITY ? 0.0f : ex2_approx((m - top) * p.scale_log2);
+        sum += w * at[D * kWideRows + kWideRows + r];
+        const float4* columns = reinterpret_cast<const float4*>(at) + c * 8 * kWideRows + r;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const float4 v = columns[q * kWideRows];
+            acc[q].x += w * v.x;
+            acc[q].y += w * v.y;
+            acc[q].z += w * v.z;
+            acc[q].w += w * v.w;
+        }
+    }
+    const float inv = 1.0f / sum;
+    __nv_bfloat16* out = p.o + static_cast<long long>(s.token0 + tok) * p.o_token +
+                         static_cast<long long>(s.h * group + r % group) * p.o_head + c * 32;
+#pragma unroll
+    for (int q = 0; q < 8; q += 2)
+        *reinterpret_cast<uint4*>(out + q * 4) =
+            make_uint4(pack_bf16x2(acc[q].x * inv, acc[q].y * inv), pack_bf16x2(acc[q].z * inv, acc[q].w * inv),
+                       pack_bf16x2(acc[q + 1].x * inv, acc[q + 1].y * inv), pack_bf16x2(acc[q + 1].z * inv, acc[q + 1].w * inv));
 }
 
 }  // namespace fa_sm100
@@ -601,6 +1226,20 @@ int prepare_paged_device(int device)
         if (err == cudaSuccess)
             err = cudaFuncSetAttribute(reinterpret_cast<const void*>(paged_narrow_kernel<128>),
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, NarrowCfg<128>::kSmemBytes);
+        const void* const wide[] = {reinterpret_cast<const void*>(paged_wide_kernel<64>),
+                                    reinterpret_cast<const void*>(paged_wide_kernel<128>)};
+        for (int i = 0; i < 2 && err == cudaSuccess; ++i) {
+            err = cudaFuncSetAttribute(wide[i], cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       i == 0 ? WideCfg<64>::kSmemBytes : WideCfg<128>::kSmemBytes);
+            // setmaxnreg waits forever for registers that the CTA did not launch with.
+            cudaFuncAttributes attributes{};
+            if (err == cudaSuccess) err = cudaFuncGetAttributes(&attributes, wide[i]);
+            if (err == cudaSuccess && static_cast<uint32_t>(attributes.numRegs) * kWideThreads <
+                                          2u * 128u * kWideRegsSoftmax + 128u * kWideRegsOther) {
+                state.status = FA_STATUS_BUILD_MISMATCH;
+                return;
+            }
+        }
         state.status = static_cast<int>(err);
     });
     return state.status;
@@ -611,6 +1250,25 @@ int narrow_ctas(int sms) { return kNarrowCtasPerSm * sms; }
 size_t narrow_workspace(int sms, int head_dim)
 {
     return static_cast<size_t>(narrow_ctas(sms)) * 2 * kNarrowRows * (head_dim + 2) * sizeof(float);
+}
+
+size_t wide_workspace(int sms, int head_dim)
+{
+    return static_cast<size_t>(sms) * 2 * 2 * kWideRows * (head_dim + 2) * sizeof(float);
+}
+
+// Which kernels a plan's requests can need: decided from the sizes that the host knows.
+bool may_be_narrow(const FaPagedPlan& plan) { return plan.heads / plan.kv_heads <= kNarrowRows; }
+bool may_be_wide(const FaPagedPlan& plan)
+{
+    const long long most = plan.max_new < plan.total_tokens ? plan.max_new : plan.total_tokens;
+    return most * (plan.heads / plan.kv_heads) > kNarrowRows;
+}
+
+size_t workspace_bytes_of(const FaPagedPlan& plan, int sms)
+{
+    return (may_be_narrow(plan) ? narrow_workspace(sms, plan.head_dim) : 0) +
+           (may_be_wide(plan) ? wide_workspace(sms, plan.head_dim) : 0);
 }
 
 // A cache as [page][head][row][D]: boxes of 64 columns by `rows` rows of one head of one page.
@@ -635,6 +1293,17 @@ int launch_narrow(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const PagedP
     return static_cast<int>(cudaGetLastError());
 }
 
+template <int D>
+int launch_wide(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const PagedParams& params,
+                int sms, cudaStream_t stream)
+{
+    paged_wide_kernel<D><<<sms, kWideThreads, WideCfg<D>::kSmemBytes, stream>>>(tm_q, tm_k, tm_v, params);
+    cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return static_cast<int>(err);
+    combine_wide_kernel<D><<<dim3(sms - 1, 2 * (D / 32)), kWideRows, 0, stream>>>(params, sms);
+    return static_cast<int>(cudaGetLastError());
+}
+
 }  // namespace
 
 extern "C" {
@@ -645,7 +1314,7 @@ size_t fa_sm100_paged_workspace_bytes(const FaPagedPlan* plan)
     if (fa_sm100_internal::validate_plan(plan) != FA_STATUS_OK ||
         fa_sm100_internal::current_sm100(&device, &sms) != FA_STATUS_OK)
         return 0;
-    return narrow_workspace(sms, plan->head_dim);
+    return workspace_bytes_of(*plan, sms);
 }
 
 int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cache, const void* v_cache, void* o,
@@ -666,8 +1335,10 @@ int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cac
     status = fa_sm100_internal::current_sm100(&device, &sms);
     if (status != FA_STATUS_OK) return status;
     if ((status = prepare_paged_device(device)) != FA_STATUS_OK) return status;
-    if (workspace_bytes < narrow_workspace(sms, plan->head_dim)) return FA_STATUS_WORKSPACE;
-    if (workspace == nullptr || plan->num_pages == 0) return FA_STATUS_INVALID_ARGUMENT;
+    if (plan->num_pages == 0) return FA_STATUS_INVALID_ARGUMENT;
+    const size_t needed = workspace_bytes_of(*plan, sms);
+    if (workspace_bytes < needed) return FA_STATUS_WORKSPACE;
+    if (needed > 0 && workspace == nullptr) return FA_STATUS_INVALID_ARGUMENT;
     if (reinterpret_cast<uintptr_t>(workspace) & 15u) return FA_STATUS_MISALIGNED;
     PagedParams params{};
     params.plan = *plan;
@@ -687,20 +1358,39 @@ int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cac
     params.v_row = strides[9];
     params.page_shift = __builtin_ctz(static_cast<unsigned>(plan->page_size));
     params.scale_log2 = fa_default_scale(plan->head_dim) * 1.4426950408889634f;
-    params.partial = static_cast<float*>(workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     CUtensorMap tm_k, tm_v;
-    if ((status = cache_map(&tm_k, k_cache, *plan, strides + 4, kNarrowKeys)) != FA_STATUS_OK) return status;
-    if ((status = cache_map(&tm_v, v_cache, *plan, strides + 7, kNarrowKeys)) != FA_STATUS_OK) return status;
-    status = plan->head_dim == 64 ? launch_narrow<64>(tm_k, tm_v, params, sms, s)
-                                  : launch_narrow<128>(tm_k, tm_v, params, sms, s);
-    if (status != FA_STATUS_OK) return status;
-    const long long rows = static_cast<long long>(plan->total_tokens) * plan->heads;
-    const long long blocks = (rows + 3) / 4;
-    if (blocks > INT_MAX) return FA_STATUS_INVALID_ARGUMENT;
-    if (plan->head_dim == 64) paged_rows_kernel<64><<<static_cast<unsigned>(blocks), 128, 0, s>>>(params);
-    else paged_rows_kernel<128><<<static_cast<unsigned>(blocks), 128, 0, s>>>(params);
-    return static_cast<int>(cudaGetLastError());
+    int map_rows = 0;           // rows of a box of the two maps; they serve both kernels where pages are that short
+    auto cache_maps = [&](int rows) -> int {
+        rows = plan->page_size < rows ? plan->page_size : rows;
+        if (rows == map_rows) return FA_STATUS_OK;
+        map_rows = rows;
+        const int made = cache_map(&tm_k, k_cache, *plan, strides + 4, rows);
+        return made != FA_STATUS_OK ? made : cache_map(&tm_v, v_cache, *plan, strides + 7, rows);
+    };
+    char* work = static_cast<char*>(workspace);
+    if (may_be_wide(*plan)) {
+        params.wide_partial = reinterpret_cast<float*>(work);
+        work += wide_workspace(sms, plan->head_dim);
+        CUtensorMap tm_q;
+        const int group = plan->heads / plan->kv_heads;
+        const cuuint64_t dims[3] = {static_cast<cuuint64_t>(plan->head_dim), static_cast<cuuint64_t>(plan->heads),
+                                    static_cast<cuuint64_t>(plan->total_tokens)};
+        const cuuint64_t bytes[2] = {static_cast<cuuint64_t>(params.q_head) * 2u, static_cast<cuuint64_t>(params.q_token) * 2u};
+        const cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(tokens_per_tile(group))};
+        if ((status = fa_sm100_internal::encode_map(&tm_q, q, 3, dims, bytes, box)) != FA_STATUS_OK) return status;
+        if ((status = cache_maps(kWideKeys)) != FA_STATUS_OK) return status;
+        status = plan->head_dim == 64 ? launch_wide<64>(tm_q, tm_k, tm_v, params, sms, s)
+                                      : launch_wide<128>(tm_q, tm_k, tm_v, params, sms, s);
+        if (status != FA_STATUS_OK) return status;
+    }
+    if (may_be_narrow(*plan)) {
+        params.partial = reinterpret_cast<float*>(work);
+        if ((status = cache_maps(kNarrowKeys)) != FA_STATUS_OK) return status;
+        status = plan->head_dim == 64 ? launch_narrow<64>(tm_k, tm_v, params, sms, s)
+                                      : launch_narrow<128>(tm_k, tm_v, params, sms, s);
+    }
+    return status;
 }
 
 }  // extern "C"
