@@ -67,14 +67,6 @@ class FaTilingInfo(ctypes.Structure):
         "device_shared_bytes_per_sm", "shared_limited_blocks_per_sm")]
 
 
-class FaPagedPlan(ctypes.Structure):
-    """Layout of FaPagedPlan (include/fa_sm100_paged.h)."""
-    _fields_ = [(name, ctypes.c_int) for name in (
-        "num_seqs", "total_tokens", "max_new", "num_pages", "table_width", "table_stride", "heads", "kv_heads",
-        "head_dim", "page_size", "causal", "reserved")] + [(name, ctypes.c_void_p) for name in (
-            "query_start", "kv_lens", "positions", "slots", "block_table", "free_cursor", "schedule")]
-
-
 _lock = threading.Lock()
 _lib = None
 
@@ -86,6 +78,8 @@ def library_path():
 def load():
     """Load libfa_sm100.so once and attach the signatures. Raises if it is missing."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             path = library_path()

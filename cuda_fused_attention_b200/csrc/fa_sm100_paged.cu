@@ -141,6 +141,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const long long total = start[plan.num_seqs] * plan.kv_heads;
     const long long share = narrow_share(total, gridDim.x);
     const long long begin = share * blockIdx.x;
+    grid_dependents_launch();
     if (begin >= total) return;
     const long long end = begin + share < total ? begin + share : total;
 
@@ -427,7 +428,8 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 }
 
 // One block per border between two CTAs' ranges; the first border inside an item merges the item's
-// parts, in their order, one warp per row.
+// parts, in their order, one warp per row. It is launched while the narrow kernel still runs
+// (programmatic dependent launch) and finds its item meanwhile.
 template <int D>
 __global__ void __launch_bounds__(kNarrowRows * 32)
 combine_narrow_kernel(const __grid_constant__ PagedParams p, int ctas)
@@ -438,34 +440,64 @@ combine_narrow_kernel(const __grid_constant__ PagedParams p, int ctas)
     const long long total = start[plan.num_seqs] * plan.kv_heads;
     const long long share = narrow_share(total, ctas);
     const long long border = share * (blockIdx.x + 1);
-    if (border >= total) return;
-    const NarrowSegment s = narrow_segment(plan, start, border, total);
-    if (s.first == border || s.first < border - share) return;
     const int row = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int token0 = plan.query_start[s.b], n = plan.query_start[s.b + 1] - token0;
-    const int group = plan.heads / plan.kv_heads;
-    if (row >= n * group) return;
-    const long long c0 = s.first / share, c1 = (s.last - 1) / share;
-    // The first part ends its CTA's range; the others begin theirs.
-    auto part = [&](long long c) { return p.partial + (2 * c + (c == c0 ? 1 : 0)) * C::kPartFloats; };
-    float top = -INFINITY;
-    for (long long c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, part(c)[16 * D + row]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    int count = 0;                          // parts of this block's item (0: none to merge here)
+    const float* first = nullptr;           // the first ends its CTA's range; the others begin theirs
+    __nv_bfloat16* out = nullptr;
     constexpr int E = D / 32;
-    float acc[E] = {}, sum = 0.0f;
-#pragma unroll 4
-    for (long long c = c0; c <= c1; ++c) {
-        const float* at = part(c);
-        const float m = at[16 * D + row];
-        const float w = m == -INFINITY ? 0.0f : ex2_approx((m - top) * p.scale_log2);
-        sum += w * at[16 * D + 16 + row];
+    constexpr long long kNext = 2LL * C::kPartFloats;
+    if (border < total) {
+        const NarrowSegment s = narrow_segment(plan, start, border, total);
+        const int token0 = plan.query_start[s.b], n = plan.query_start[s.b + 1] - token0;
+        const int group = plan.heads / plan.kv_heads;
+        if (s.first != border && s.first >= border - share && row < n * group) {
+            const long long c0 = s.first / share;
+            count = static_cast<int>((s.last - 1) / share - c0) + 1;
+            first = p.partial + (2 * c0 + 1) * C::kPartFloats;
+            const int tok = row / group;
+            out = p.o + (token0 + tok) * p.o_token + (s.h * group + row - tok * group) * p.o_head + lane * E;
+        }
+    }
+    grid_dependency_wait();
+    if (count == 0) return;
+    auto part = [&](int i) { return i == 0 ? first : first + i * kNext - C::kPartFloats; };
+    // 32 parts at a time: a lane reads one part's maximum and sum, then all lanes add up its columns.
+    float top = -INFINITY, sum = 0.0f, acc[E] = {};
+    for (int i0 = 0; i0 < count; i0 += 32) {
+        const int mine = i0 + lane;
+        const float m = mine < count ? part(mine)[16 * D + row] : -INFINITY;
+        const float l = mine < count ? part(mine)[16 * D + 16 + row] : 0.0f;
+        float high = fmaxf(m, top);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += w * at[row * D + lane * E + e];
+        for (int d = 16; d > 0; d >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+        const float keep = top == -INFINITY ? 0.0f : ex2_approx((top - high) * p.scale_log2);
+        const float w = m == -INFINITY ? 0.0f : ex2_approx((m - high) * p.scale_log2);
+        float wl = w * l;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) wl += __shfl_xor_sync(0xffffffffu, wl, d);
+        sum = sum * keep + wl;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= keep;
+        top = high;
+        const int here = min(32, count - i0);
+#pragma unroll 8
+        for (int i = 0; i < here; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const float* at = part(i0 + i) + row * D + lane * E;
+            if constexpr (E == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(at);
+                acc[0] += wi * v.x;
+                acc[1] += wi * v.y;
+                acc[2] += wi * v.z;
+                acc[3] += wi * v.w;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(at);
+                acc[0] += wi * v.x;
+                acc[1] += wi * v.y;
+            }
+        }
     }
     const float inv = 1.0f / sum;
-    const int tok = row / group;
-    __nv_bfloat16* out = p.o + (token0 + tok) * p.o_token + (s.h * group + row - tok * group) * p.o_head + lane * E;
 #pragma unroll
     for (int e = 0; e < E; e += 2)
         *reinterpret_cast<uint32_t*>(out + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
@@ -622,6 +654,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const long long total = start[plan.num_seqs] * plan.kv_heads;
     const long long share = wide_share(total, gridDim.x);
     const long long begin = share * blockIdx.x;
+    grid_dependents_launch();
     if (begin >= total) return;
     const long long end = begin + share < total ? begin + share : total;
 
@@ -1091,7 +1124,8 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 }
 
 // One block row per border between two CTAs' ranges; the first border inside a block of tokens merges
-// its parts, in their order. A thread is a query row and takes 32 columns of one Q tile.
+// its parts, in their order. A thread is a query row and takes 32 columns of one Q tile. Launched while
+// the wide kernel still runs, as combine_narrow_kernel.
 template <int D>
 __global__ void __launch_bounds__(kWideRows)
 combine_wide_kernel(const __grid_constant__ PagedParams p, int ctas)
@@ -1102,13 +1136,17 @@ combine_wide_kernel(const __grid_constant__ PagedParams p, int ctas)
     const long long total = start[plan.num_seqs] * plan.kv_heads;
     const long long share = wide_share(total, ctas);
     const long long border = share * (blockIdx.x + 1);
-    if (border >= total) return;
-    const WideSegment s = wide_segment(plan, start, border, total);
-    if (s.first == border || s.first < border - share) return;
     const int group = plan.heads / plan.kv_heads, per_tile = tokens_per_tile(group);
     const int t = blockIdx.y / (D / 32), c = blockIdx.y % (D / 32), r = threadIdx.x;
     const int tok = t * per_tile + r / group;
-    if (r >= per_tile * group || tok >= s.tokens) return;
+    WideSegment s;
+    bool merges = false;
+    if (border < total) {
+        s = wide_segment(plan, start, border, total);
+        merges = s.first != border && s.first >= border - share && r < per_tile * group && tok < s.tokens;
+    }
+    grid_dependency_wait();
+    if (!merges) return;
     const long long c0 = s.first / share, c1 = (s.last - 1) / share;
     auto part = [&](long long cta) {
         return p.wide_partial + ((2 * cta + (cta == c0 ? 1 : 0)) * 2 + t) * C::kPartTileFloats;
@@ -1282,6 +1320,23 @@ int cache_map(CUtensorMap* map, const void* ptr, const FaPagedPlan& plan, const 
     return fa_sm100_internal::encode_map(map, ptr, 4, dims, bytes, box);
 }
 
+// Launches a kernel that may start before the one in front of it in the stream is done; it waits for
+// that one itself (grid_dependency_wait).
+template <typename... Args>
+int launch_early(void (*kernel)(Args...), dim3 grid, int threads, cudaStream_t stream, Args... args)
+{
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.stream = stream;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&config, kernel, args...));
+}
+
 template <int D>
 int launch_narrow(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const PagedParams& params, int sms, cudaStream_t stream)
 {
@@ -1289,8 +1344,7 @@ int launch_narrow(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const PagedP
     paged_narrow_kernel<D><<<ctas, kNarrowThreads, NarrowCfg<D>::kSmemBytes, stream>>>(tm_k, tm_v, params);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return static_cast<int>(err);
-    combine_narrow_kernel<D><<<ctas - 1, kNarrowRows * 32, 0, stream>>>(params, ctas);
-    return static_cast<int>(cudaGetLastError());
+    return launch_early(combine_narrow_kernel<D>, dim3(ctas - 1), kNarrowRows * 32, stream, params, ctas);
 }
 
 template <int D>
@@ -1300,8 +1354,7 @@ int launch_wide(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensor
     paged_wide_kernel<D><<<sms, kWideThreads, WideCfg<D>::kSmemBytes, stream>>>(tm_q, tm_k, tm_v, params);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return static_cast<int>(err);
-    combine_wide_kernel<D><<<dim3(sms - 1, 2 * (D / 32)), kWideRows, 0, stream>>>(params, sms);
-    return static_cast<int>(cudaGetLastError());
+    return launch_early(combine_wide_kernel<D>, dim3(sms - 1, 2 * (D / 32)), kWideRows, stream, params, sms);
 }
 
 }  // namespace

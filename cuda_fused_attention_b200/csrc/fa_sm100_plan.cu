@@ -226,13 +226,16 @@ plan_kernel(const PlanParams p)
 // =============================================================================
 // Rotary positions, and the append of K and V
 // =============================================================================
-// A thread owns eight pairs (16 elements, two 16-byte accesses) of one token and walks over
-// heads: the eight angles are computed once, in registers, and serve every head it visits. The
-// rest is a stream: each element is read once and written once. An angle is a position times a
-// frequency; far positions need more than 24 bits of it, so the product is taken in turns
-// (1 / 2 pi) in 64 bits, its whole turns dropped there, and only the rest goes to sincospif.
+// A CTA serves a few neighbouring tokens: it first computes their angles' sines and cosines, once
+// for all heads, into shared memory, then streams the tokens' rows in units of eight pairs (two
+// 16-byte accesses), each element read once and written once; memory bounds it. An angle is a
+// position times a frequency; far positions need more than 24 bits of it, so the product is taken
+// in turns (1 / 2 pi) in 64 bits, its whole turns dropped there, and only the rest goes to
+// sincospif.
 constexpr int kRotaryThreads = 256;
 constexpr int kMaxAxes = 4;
+constexpr int kMaxTokensPerCta = 8;     // tokens that share a CTA
+constexpr int kRotaryBatch = 4;         // units a thread has in flight
 
 struct RotaryParams {
     const __nv_bfloat16* src[3];        // q, k, v (x alone: q)
@@ -242,9 +245,9 @@ struct RotaryParams {
     long long dst_page[3];
     int rows[3];                        // heads of each
     int batch, tokens;
-    int units;                          // 16-element units per row
+    int unit_shift;                     // log2 of the 16-element units per row
+    int group_shift;
     int rotary_dim;
-    int head_split;                     // threads that share a token's heads
     const int* positions;
     long long position_axis, position_batch;
     const float* inv_freq;
@@ -278,88 +281,114 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8])
 
 template <bool kAppend, bool kInterleaved>
 __global__ void __launch_bounds__(kRotaryThreads)
-rotary_kernel(const RotaryParams p)
+rotary_kernel(const __grid_constant__ RotaryParams p)
 {
-    const long long index = static_cast<long long>(blockIdx.x) * kRotaryThreads + threadIdx.x;
-    const int unit = static_cast<int>(index % p.units);
-    const long long rest = index / p.units;
-    const long long flat = rest % (static_cast<long long>(p.tokens) * p.batch);
-    const int part = static_cast<int>(rest / (static_cast<long long>(p.tokens) * p.batch));
-    if (part >= p.head_split) return;
-    const int batch = static_cast<int>(flat / p.tokens);
-    const int token = static_cast<int>(flat - static_cast<long long>(batch) * p.tokens);
+    __shared__ float2 turn[kMaxTokensPerCta][64];       // (cos, sin) of each token's pairs
+    __shared__ long long slots[kMaxTokensPerCta];
+    const int group = 1 << p.group_shift;
+    const int blocks_per_batch = (p.tokens + group - 1) >> p.group_shift;
+    const int batch = kAppend ? 0 : static_cast<int>(blockIdx.x) / blocks_per_batch;
+    const int token0 = (static_cast<int>(blockIdx.x) - batch * blocks_per_batch) << p.group_shift;
+    const int tokens = min(group, p.tokens - token0);
+    const int pairs = p.rotary_dim / 2;
 
-    long long slot = 0;
-    if (kAppend) {
-        slot = p.slots[token];
-        if (slot < 0) return;
+    if (kAppend && threadIdx.x < tokens) {
+        long long slot = p.slots[token0 + threadIdx.x];
         if (slot >= p.num_slots) {
             record_plan_error(FA_ERROR_BAD_PAGE);
-            return;
+            slot = -1;
         }
+        slots[threadIdx.x] = slot;
     }
+    for (int i = threadIdx.x; i < tokens * pairs; i += kRotaryThreads) {
+        const int tok = i / pairs, pair = i - tok * pairs;
+        int axis = 0;
+#pragma unroll
+        for (int a = 0; a < kMaxAxes - 1; ++a) axis += pair >= p.section_end[a] ? 1 : 0;
+        const int position = p.positions[axis * p.position_axis + batch * p.position_batch + token0 + tok];
+        const double turns = static_cast<double>(position) * static_cast<double>(p.inv_freq[pair]) * 0.15915494309189533577;
+        float sine, cosine;
+        sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sine, &cosine);
+        turn[tok][pair] = make_float2(cosine, p.sign * sine);
+    }
+    __syncthreads();
 
-    const int half = p.rotary_dim / 2;
+    // Neighbouring threads take the units of a row, then the rows that are neighbours in memory: the next
+    // head of a packed token, the next token of a [heads, tokens] tensor.
     const int rotating = p.rotary_dim / 16;
+    const int rows = p.rows[0] + (kAppend ? p.rows[1] + p.rows[2] : 0);
+    const int total = (kAppend ? tokens : group) * rows << p.unit_shift;
+    const int unit = threadIdx.x & ((1 << p.unit_shift) - 1);       // the same for all of a thread's items
     const bool turns = unit < rotating;
     // The unit's two 8-element pieces: the two halves of its pairs, or 16 neighbours.
     const int lo = turns && !kInterleaved ? 8 * unit : 16 * unit;
-    const int hi = turns && !kInterleaved ? half + 8 * unit : 16 * unit + 8;
-
-    float c[8], s[8];
-    if (turns) {
+    const int hi = turns && !kInterleaved ? pairs + 8 * unit : 16 * unit + 8;
+    for (int first = threadIdx.x; first < total; first += kRotaryBatch * kRotaryThreads) {
+        uint4 x0[kRotaryBatch], x1[kRotaryBatch];
+        __nv_bfloat16* dst[kRotaryBatch];
+        int tok[kRotaryBatch];                  // -1: nothing here; + 256: copied, not turned (V)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int pair = 8 * unit + i;
-            int axis = 0;
-#pragma unroll
-            for (int a = 0; a < kMaxAxes - 1; ++a) axis += pair >= p.section_end[a] ? 1 : 0;
-            const int position = p.positions[axis * p.position_axis + batch * p.position_batch + token];
-            const double turn = static_cast<double>(position) * static_cast<double>(p.inv_freq[pair]) *
-                                0.15915494309189533577;
-            const float part_turn = static_cast<float>(turn - rint(turn));
-            sincospif(2.0f * part_turn, &s[i], &c[i]);
-            s[i] *= p.sign;
-        }
-    }
-
-    const int rows = p.rows[0] + (kAppend ? p.rows[1] + p.rows[2] : 0);
-    for (int row = part; row < rows; row += p.head_split) {
-        int which = 0, head = row;
-        if (kAppend) {
-            if (head >= p.rows[0]) { head -= p.rows[0]; which = 1; }
-            if (which == 1 && head >= p.rows[1]) { head -= p.rows[1]; which = 2; }
-        }
-        const __nv_bfloat16* src = p.src[which] + batch * p.src_batch + token * p.src_token[which] + head * p.src_head[which];
-        __nv_bfloat16* dst = p.dst[which] + head * p.dst_head[which];
-        if (kAppend && which > 0)
-            dst += (slot >> p.page_shift) * p.dst_page[which] + (slot & ((1LL << p.page_shift) - 1)) * p.dst_token[which];
-        else
-            dst += batch * p.dst_batch + token * p.dst_token[which];
-        uint4 x0 = *reinterpret_cast<const uint4*>(src + (kAppend && which == 2 ? 16 * unit : lo));
-        uint4 x1 = *reinterpret_cast<const uint4*>(src + (kAppend && which == 2 ? 16 * unit + 8 : hi));
-        if (turns && !(kAppend && which == 2)) {
-            float a[8], b[8], u[8], w[8];
-            unpack8(x0, a);
-            unpack8(x1, b);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (kInterleaved) {
-                    const int q = 2 * (i & 3);
-                    const float e = i < 4 ? a[q] : b[q], o = i < 4 ? a[q + 1] : b[q + 1];
-                    const float re = e * c[i] - o * s[i], im = o * c[i] + e * s[i];
-                    if (i < 4) { u[q] = re; u[q + 1] = im; }
-                    else { w[q] = re; w[q + 1] = im; }
-                } else {
-                    u[i] = a[i] * c[i] - b[i] * s[i];
-                    w[i] = b[i] * c[i] + a[i] * s[i];
-                }
+        for (int k = 0; k < kRotaryBatch; ++k) {
+            const int item = (first + k * kRotaryThreads) >> p.unit_shift;
+            tok[k] = -1;
+            if (first + k * kRotaryThreads >= total) continue;
+            int t, head, which = 0;
+            if (kAppend) {
+                t = item / rows;
+                head = item - t * rows;
+                if (slots[t] < 0) continue;
+                if (head >= p.rows[0]) { head -= p.rows[0]; which = 1; }
+                if (which == 1 && head >= p.rows[1]) { head -= p.rows[1]; which = 2; }
+            } else {
+                t = item & (group - 1);
+                head = item >> p.group_shift;
+                if (t >= tokens) continue;
             }
-            x0 = pack8(u);
-            x1 = pack8(w);
+            const long long token = token0 + t;
+            const __nv_bfloat16* src = p.src[which] + batch * p.src_batch + token * p.src_token[which] + head * p.src_head[which];
+            __nv_bfloat16* to = p.dst[which] + head * p.dst_head[which];
+            if (kAppend && which > 0)
+                to += (slots[t] >> p.page_shift) * p.dst_page[which] + (slots[t] & ((1LL << p.page_shift) - 1)) * p.dst_token[which];
+            else
+                to += batch * p.dst_batch + token * p.dst_token[which];
+            dst[k] = to;
+            tok[k] = t + (which == 2 ? 256 : 0);
+            x0[k] = *reinterpret_cast<const uint4*>(src + (which == 2 ? 16 * unit : lo));
+            x1[k] = *reinterpret_cast<const uint4*>(src + (which == 2 ? 16 * unit + 8 : hi));
         }
-        *reinterpret_cast<uint4*>(dst + (kAppend && which == 2 ? 16 * unit : lo)) = x0;
-        *reinterpret_cast<uint4*>(dst + (kAppend && which == 2 ? 16 * unit + 8 : hi)) = x1;
+#pragma unroll
+        for (int k = 0; k < kRotaryBatch; ++k) {
+            if (tok[k] < 0) continue;
+            const bool copied = kAppend && tok[k] >= 256;
+            if (turns && !copied) {
+                const float4* cs = reinterpret_cast<const float4*>(&turn[tok[k]][8 * unit]);
+                float a[8], b[8], u[8], w[8];
+                unpack8(x0[k], a);
+                unpack8(x1[k], b);
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float4 two = cs[i / 2];       // cos, sin of pairs i and i + 1
+                    if (kInterleaved) {
+                        float(&v)[8] = i < 4 ? a : b;
+                        float(&out)[8] = i < 4 ? u : w;
+                        const int q = 2 * (i & 3);
+                        out[q] = v[q] * two.x - v[q + 1] * two.y;
+                        out[q + 1] = v[q + 1] * two.x + v[q] * two.y;
+                        out[q + 2] = v[q + 2] * two.z - v[q + 3] * two.w;
+                        out[q + 3] = v[q + 3] * two.z + v[q + 2] * two.w;
+                    } else {
+                        u[i] = a[i] * two.x - b[i] * two.y;
+                        w[i] = b[i] * two.x + a[i] * two.y;
+                        u[i + 1] = a[i + 1] * two.z - b[i + 1] * two.w;
+                        w[i + 1] = b[i + 1] * two.z + a[i + 1] * two.w;
+                    }
+                }
+                x0[k] = pack8(u);
+                x1[k] = pack8(w);
+            }
+            *reinterpret_cast<uint4*>(dst[k] + (copied ? 16 * unit : lo)) = x0[k];
+            *reinterpret_cast<uint4*>(dst[k] + (copied ? 16 * unit + 8 : hi)) = x1[k];
+        }
     }
 }
 
@@ -403,13 +432,14 @@ int launch_rotary(RotaryParams& params, bool interleaved, cudaStream_t stream)
     const long long tokens = static_cast<long long>(params.tokens) * params.batch;
     const int rows = params.rows[0] + (kAppend ? params.rows[1] + params.rows[2] : 0);
     if (tokens == 0 || rows == 0) return FA_STATUS_OK;
-    // Heads are shared out until the threads fill the GPU once (2048 per SM): few tokens are then
-    // served in one go, and many tokens keep the angles of a thread in use for all heads.
-    const long long per_split = tokens * params.units;
-    long long split = (2048LL * sms + per_split - 1) / per_split;
-    params.head_split = static_cast<int>(split < rows ? split : rows);
-    const long long blocks = (per_split * params.head_split + kRotaryThreads - 1) / kRotaryThreads;
-    if (blocks > INT_MAX) return FA_STATUS_INVALID_ARGUMENT;
+    // Tokens share a CTA (and its set-up) once the CTAs would fill the GPU without it, four per SM.
+    params.group_shift = 0;
+    while ((2 << params.group_shift) <= kMaxTokensPerCta && (tokens >> (params.group_shift + 1)) >= 4LL * sms)
+        ++params.group_shift;
+    const long long per_batch = ceil_div(params.tokens, 1LL << params.group_shift);
+    const long long blocks = per_batch * params.batch;
+    if (blocks > INT_MAX || per_batch << params.group_shift > INT_MAX || (static_cast<long long>(rows) << 7) > INT_MAX)
+        return FA_STATUS_INVALID_ARGUMENT;
     if (interleaved) rotary_kernel<kAppend, true><<<static_cast<unsigned>(blocks), kRotaryThreads, 0, stream>>>(params);
     else rotary_kernel<kAppend, false><<<static_cast<unsigned>(blocks), kRotaryThreads, 0, stream>>>(params);
     return static_cast<int>(cudaGetLastError());
@@ -482,7 +512,7 @@ int fa_sm100_rotary(const void* x, const long long* x_strides, void* out, const 
     params.rows[0] = heads;
     params.batch = batch;
     params.tokens = seq_len;
-    params.units = head_dim / 16;
+    params.unit_shift = head_dim == 64 ? 2 : 3;
     params.rotary_dim = rotary_dim;
     params.positions = positions;
     params.position_axis = position_strides[0];
@@ -540,7 +570,7 @@ int fa_sm100_rotary_append(const void* q, const void* k, const void* v, void* q_
     params.rows[2] = kv_heads;
     params.batch = 1;
     params.tokens = tokens;
-    params.units = head_dim / 16;
+    params.unit_shift = head_dim == 64 ? 2 : 3;
     params.rotary_dim = rotary_dim;
     params.positions = positions;
     params.position_axis = position_stride;

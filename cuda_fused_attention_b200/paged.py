@@ -18,7 +18,8 @@ device arrays is recorded on the device: device_status() reports it.
 No counterpart in the reference, whose attention has contiguous K and V of Q's own length.
 """
 import contextlib
-import ctypes
+import functools
+import struct
 from dataclasses import dataclass
 
 from . import _lib
@@ -27,6 +28,12 @@ __all__ = ["PagedShape", "PagedPlan", "paged_plan", "paged_attention", "rotary_e
 
 _PAGE_SIZES = (16, 32, 64, 128, 256)
 _INT_MAX = 2 ** 31 - 1
+
+# Small steps are bound by what the host does, so the calls below check their arguments in few
+# steps, look closer only at what those do not pass, and hand structs and strides to the C ABI
+# as packed bytes (a ctypes array costs several times as much).
+_PLAN = struct.Struct("12i7P")          # FaPagedPlan
+_STRIDES = {n: struct.Struct(f"{n}q").pack for n in (2, 3, 10, 14)}
 
 
 @dataclass(frozen=True)
@@ -55,44 +62,43 @@ class PagedPlan:
     free_cursor [1] are int32 views of one buffer of the plan; block_table is the caller's.
     """
 
-    def __init__(self, num_seqs, total_tokens, shape, device):
-        import torch
+    def __init__(self, num_seqs, total_tokens, shape, like):
         self.shape = shape
         self.num_seqs = num_seqs
         self.total_tokens = total_tokens
-        self.device = device
+        self.device_index = like.get_device()
         self.block_table = None
+        self.num_pages = 0
         self.causal = True
-        schedule = 2 * (num_seqs + 1)
-        words = (num_seqs + 1) + num_seqs + 2 * total_tokens + 1
-        self._buffer = torch.empty(schedule + (words + 1) // 2, dtype=torch.int64, device=device)
+        # [schedule, as 64-bit words][query_start][kv_lens][positions][slots][free_cursor]
+        self._sizes = (4 * (num_seqs + 1), num_seqs + 1, num_seqs, total_tokens, total_tokens, 1)
+        self._buffer = like.new_empty(sum(self._sizes))
         self._views = None
-        base = int(self._buffer.data_ptr())
-        at = base + 8 * schedule
-        c = self.c = _lib.FaPagedPlan()
-        c.num_seqs, c.total_tokens = num_seqs, total_tokens
-        c.heads, c.kv_heads, c.head_dim, c.page_size = shape.heads, shape.kv_heads, shape.head_dim, shape.page_size
-        c.schedule = base
-        c.query_start = at
-        c.kv_lens = at + 4 * (num_seqs + 1)
-        c.positions = c.kv_lens + 4 * num_seqs
-        c.slots = c.positions + 4 * total_tokens
-        c.free_cursor = c.slots + 4 * total_tokens
-        self._ref = ctypes.byref(c)
+        self.c = b""                    # FaPagedPlan
+        self._workspace = 0             # bytes of workspace that paged_attention needs
 
-    def _split(self):
+    def _fill(self, block_table, width, stride, num_pages, max_new, causal):
+        self.block_table, self.num_pages, self.causal = block_table, num_pages, causal
+        shape, seqs, tokens = self.shape, self.num_seqs, self.total_tokens
+        schedule = self._buffer.data_ptr()
+        start = schedule + 16 * (seqs + 1)
+        lens = start + 4 * (seqs + 1)
+        positions = lens + 4 * seqs
+        slots = positions + 4 * tokens
+        self.c = _PLAN.pack(seqs, tokens, max_new, num_pages, width, stride, shape.heads, shape.kv_heads, shape.head_dim,
+                            shape.page_size, causal, 0, start, lens, positions, slots, block_table.data_ptr(),
+                            slots + 4 * tokens, schedule)
+
+    def _view(self, index):
         if self._views is None:
-            import torch
-            b, t = self.num_seqs, self.total_tokens
-            words = self._buffer.view(torch.int32)[4 * (b + 1):]
-            self._views = words[: 2 * b + 2 + 2 * t].split([b + 1, b, t, t, 1])
-        return self._views
+            self._views = self._buffer.split_with_sizes(self._sizes)
+        return self._views[index]
 
-    query_start = property(lambda self: self._split()[0])
-    kv_lens = property(lambda self: self._split()[1])
-    positions = property(lambda self: self._split()[2])
-    slots = property(lambda self: self._split()[3])
-    free_cursor = property(lambda self: self._split()[4])
+    query_start = property(lambda self: self._view(1))
+    kv_lens = property(lambda self: self._view(2))
+    positions = property(lambda self: self._view(3))
+    slots = property(lambda self: self._view(4))
+    free_cursor = property(lambda self: self._view(5))
 
 
 def _check(status, what):
@@ -101,8 +107,8 @@ def _check(status, what):
         raise FaError(status, what)
 
 
-def _device(**tensors):
-    """The one CUDA device of the tensors."""
+def _device_error(**tensors):
+    """Raises for tensors that are not all on one CUDA device."""
     device = None
     for name, t in tensors.items():
         if t is None:
@@ -113,31 +119,49 @@ def _device(**tensors):
             device = t.device
         elif t.device != device:
             raise ValueError(f"{name} is on {t.device}, other arguments on {device}")
-    return device
+    raise ValueError("arguments are on different devices")
+
+
+@functools.lru_cache(maxsize=None)
+def _raw_stream():
+    """The function that gives a device's current stream as an integer."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw if raw is not None else lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
 @contextlib.contextmanager
-def _launching(device, stream):
-    """Make `device` current and yield the stream's handle. What is allocated inside belongs to that
+def _elsewhere(index, stream):
+    """Make device `index` current and yield the stream's handle. What is allocated inside belongs to that
     stream, so that its memory is not handed to another one while the call still uses it."""
     import torch
-    with contextlib.ExitStack() as stack:
-        if torch.cuda.current_device() != device.index:
-            stack.enter_context(torch.cuda.device(device))
+    with torch.cuda.device(index):
         if stream is None:
-            handle = int(torch.cuda.current_stream(device).cuda_stream)
-        else:
-            handle = stream if isinstance(stream, int) else int(stream.cuda_stream)
-            if handle != int(torch.cuda.current_stream(device).cuda_stream):
-                stack.enter_context(torch.cuda.stream(
-                    torch.cuda.ExternalStream(handle, device=device) if handle
-                    else torch.cuda.default_stream(device)))
-        yield handle
+            yield _raw_stream()(index)
+            return
+        handle = stream if isinstance(stream, int) else int(stream.cuda_stream)
+        if handle == _raw_stream()(index):
+            yield handle
+            return
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = (torch.cuda.ExternalStream(handle, device=index) if handle
+                      else torch.cuda.default_stream(index))
+        with torch.cuda.stream(stream):
+            yield handle
+
+
+def _launch(call, index, stream, *args):
+    """call(stream handle, *args) with device `index` current."""
+    import torch
+    if stream is None and torch.cuda.current_device() == index:
+        return call(_raw_stream()(index), *args)
+    with _elsewhere(index, stream) as handle:
+        return call(handle, *args)
 
 
 def _int32(name, t, dims):
     import torch
-    if t.dtype != torch.int32:
+    if t.dtype is not torch.int32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
     if t.dim() != dims:
         raise ValueError(f"{name} must have {dims} dimension(s), got {t.dim()}")
@@ -154,15 +178,22 @@ def _vector(name, t, size=None):
 def _rows(name, t, shape):
     """A bf16 tensor of this shape with contiguous rows on 16-byte boundaries; its strides without the last."""
     import torch
-    if t.dtype != torch.bfloat16:
+    strides = t.stride()
+    if t.dtype is torch.bfloat16 and t.shape == shape and strides[-1] == 1 and not t.data_ptr() & 15:
+        strides = strides[:-1]
+        if len(strides) == 3:
+            if not (strides[0] | strides[1] | strides[2]) & 7:
+                return strides
+        elif not (strides[0] | strides[1]) & 7:
+            return strides
+    if t.dtype is not torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
     if tuple(t.shape) != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    strides = t.stride()
-    if strides[-1] != 1:
+    if t.stride(-1) != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
     # The stride of a dimension with one element is never used.
-    strides = [s if n > 1 else shape[-1] for s, n in zip(strides[:-1], shape)]
+    strides = tuple(s if n > 1 else shape[-1] for s, n in zip(t.stride()[:-1], shape))
     for s in strides:
         if s % 8:
             raise ValueError(f"{name} has rows off 16-byte boundaries (strides {list(t.stride())})")
@@ -173,6 +204,8 @@ def _rows(name, t, shape):
 
 def _written(name, t):
     """An output (or cache) whose elements share no memory."""
+    if t.is_contiguous():
+        return t
     span = sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1)
     reach = 1
     for s, n in span:
@@ -195,16 +228,22 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, total_tokens, sha
     plan: an earlier plan of the same B, total_tokens and shape whose buffers are written again
     (for CUDA graphs). Returns the PagedPlan.
     """
-    _vector("cached_lens", cached_lens)
+    import torch
+    i32 = torch.int32
     num_seqs = cached_lens.numel()
-    _vector("new_lens", new_lens, num_seqs)
-    _vector("free_pages", free_pages)
-    _int32("block_table", block_table, 2)
-    if block_table.shape[0] != num_seqs:
-        raise ValueError(f"block_table must have {num_seqs} rows, got {block_table.shape[0]}")
-    width = block_table.shape[1]
-    if width > 1 and block_table.stride(1) != 1:
-        raise ValueError("block_table must be contiguous in its last dimension")
+    width = block_table.shape[-1] if block_table.dim() else 0
+    if not (cached_lens.dtype is i32 and new_lens.dtype is i32 and block_table.dtype is i32 and free_pages.dtype is i32
+            and cached_lens.shape == new_lens.shape == (num_seqs,) and block_table.shape == (num_seqs, width)
+            and free_pages.dim() == 1 and cached_lens.is_contiguous() and new_lens.is_contiguous()
+            and block_table.is_contiguous() and free_pages.is_contiguous()):
+        _vector("cached_lens", cached_lens)
+        _vector("new_lens", new_lens, num_seqs)
+        _vector("free_pages", free_pages)
+        _int32("block_table", block_table, 2)
+        if block_table.shape[0] != num_seqs:
+            raise ValueError(f"block_table must have {num_seqs} rows, got {block_table.shape[0]}")
+        if width > 1 and block_table.stride(1) != 1:
+            raise ValueError("block_table must be contiguous in its last dimension")
     stride = block_table.stride(0) if num_seqs > 1 else width
     if stride < width:
         raise ValueError("block_table has rows that share memory")
@@ -218,39 +257,56 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, total_tokens, sha
         raise ValueError("total_tokens must be below 2^30")
     if num_pages * shape.page_size > _INT_MAX or width * shape.page_size > _INT_MAX:
         raise ValueError("a cache, and a table row, must hold fewer than 2^31 tokens")
-    device = _device(cached_lens=cached_lens, new_lens=new_lens, block_table=block_table, free_pages=free_pages,
-                     free_cursor=free_cursor)
-    with _launching(device, stream) as handle:
-        if plan is None:
-            plan = PagedPlan(num_seqs, total_tokens, shape, device)
-        elif (plan.num_seqs, plan.total_tokens, plan.shape, plan.device) != (num_seqs, total_tokens, shape, device):
-            raise ValueError("plan was made for other sizes or another device")
-        plan.block_table = block_table
-        plan.causal = bool(causal)
-        c = plan.c
-        c.max_new, c.num_pages, c.causal = max_new, num_pages, 1 if causal else 0
-        c.table_width, c.table_stride = width, stride
-        c.block_table = block_table.data_ptr()
-        status = _lib.load().fa_sm100_paged_plan(plan._ref, cached_lens.data_ptr(), new_lens.data_ptr(),
-                                                 free_pages.data_ptr(), free_pages.numel(),
-                                                 free_cursor.data_ptr() if free_cursor is not None else None, handle)
-    _check(status, "fa_sm100_paged_plan")
+    index = cached_lens.get_device()
+    if index < 0 or not (index == new_lens.get_device() == block_table.get_device() == free_pages.get_device()) or (
+            free_cursor is not None and free_cursor.get_device() != index):
+        _device_error(cached_lens=cached_lens, new_lens=new_lens, block_table=block_table, free_pages=free_pages,
+                      free_cursor=free_cursor)
+    if plan is not None and (plan.num_seqs, plan.total_tokens, plan.shape, plan.device_index) != (
+            num_seqs, total_tokens, shape, index):
+        raise ValueError("plan was made for other sizes or another device")
+    return _launch(_plan, index, stream, cached_lens, new_lens, block_table, free_pages, total_tokens, shape, num_pages,
+                   free_cursor, causal, max_new, plan, width, stride)
+
+
+def _plan(handle, cached_lens, new_lens, block_table, free_pages, total_tokens, shape, num_pages, free_cursor, causal,
+          max_new, plan, width, stride):
+    if plan is None:
+        plan = PagedPlan(cached_lens.numel(), total_tokens, shape, cached_lens)
+    plan._fill(block_table, width, stride, num_pages, max_new, 1 if causal else 0)
+    lib = _lib.load()
+    status = lib.fa_sm100_paged_plan(plan.c, cached_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(),
+                                     free_pages.numel(), free_cursor.data_ptr() if free_cursor is not None else None,
+                                     handle)
+    if status:
+        _check(status, "fa_sm100_paged_plan")
+    plan._workspace = lib.fa_sm100_paged_workspace_bytes(plan.c)
     return plan
 
 
-def _frequencies(inv_freq, head_dim, sections):
-    import torch
-    if inv_freq.dtype != torch.float32:
-        raise TypeError(f"inv_freq must be float32, got {inv_freq.dtype}")
-    if inv_freq.dim() != 1 or not inv_freq.is_contiguous():
-        raise ValueError("inv_freq must be a contiguous vector")
-    pairs = inv_freq.numel()
-    if pairs == 0 or pairs % 8 or 2 * pairs > head_dim:
-        raise ValueError(f"inv_freq must have a multiple of 8 and at most {head_dim // 2} elements, got {pairs}")
+@functools.lru_cache(maxsize=64)
+def _sections(sections, pairs):
+    """(sections, the same packed) for a number of pairs."""
     sections = (pairs,) if sections is None else tuple(int(n) for n in sections)
     if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) != pairs:
         raise ValueError(f"sections must be 1 to 4 counts that add up to {pairs}, got {sections}")
-    return 2 * pairs, sections
+    return sections, struct.pack(f"{len(sections)}i", *sections)
+
+
+def _frequencies(inv_freq, head_dim, sections):
+    """(rotary_dim, axes, packed sections)."""
+    import torch
+    pairs = inv_freq.numel()
+    if inv_freq.dtype is not torch.float32:
+        raise TypeError(f"inv_freq must be float32, got {inv_freq.dtype}")
+    if inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous vector")
+    if pairs == 0 or pairs % 8 or 2 * pairs > head_dim:
+        raise ValueError(f"inv_freq must have a multiple of 8 and at most {head_dim // 2} elements, got {pairs}")
+    if sections is not None and not isinstance(sections, tuple):
+        sections = tuple(sections)
+    counts, packed = _sections(sections, pairs)
+    return 2 * pairs, len(counts), packed
 
 
 def rotary_embed(x, positions, inv_freq, sections=None, interleaved=False, inverse=False, out=None, stream=None):
@@ -263,42 +319,44 @@ def rotary_embed(x, positions, inv_freq, sections=None, interleaved=False, inver
     is also the gradient: dL/dx = rotary_embed(dL/dout, ..., inverse=True). out may be x.
     """
     import torch
-    if x.dim() != 4:
+    shape = x.shape
+    if len(shape) != 4:
         raise ValueError("x must be [batch, heads, seq_len, head_dim]")
-    shape = tuple(x.shape)
     batch, heads, tokens, dim = shape
-    if dim not in (64, 128):
+    if dim != 128 and dim != 64:
         raise ValueError(f"head_dim must be 64 or 128, got {dim}")
     x_strides = _rows("x", x, shape)
-    rotary_dim, sections = _frequencies(inv_freq, dim, sections)
-    if positions.dim() == 1:
-        positions = positions[None]
-    _int32("positions", positions, 3 if positions.dim() == 3 else 2)
-    expected = (len(sections), tokens) if positions.dim() == 2 else (len(sections), batch, tokens)
-    if tuple(positions.shape) != expected:
-        raise ValueError(f"positions must be {list(expected)}, got {list(positions.shape)}")
-    if tokens > 1 and positions.stride(-1) != 1:
+    rotary_dim, axes, packed = _frequencies(inv_freq, dim, sections)
+    at, step = positions.shape, positions.stride()
+    if positions.dtype is not torch.int32 or not 1 <= len(at) <= 3:
+        _int32("positions", positions, 2)
+    if len(at) == 1:
+        at, step = (1, *at), (0, *step)
+    if at != ((axes, tokens) if len(at) == 2 else (axes, batch, tokens)):
+        raise ValueError(f"positions must be {[axes, tokens]} or {[axes, batch, tokens]}, got {list(positions.shape)}")
+    if tokens > 1 and step[-1] != 1:
         raise ValueError("positions must be contiguous in their last dimension")
-    strides = (positions.stride(0), positions.stride(1) if positions.dim() == 3 else 0)
-    device = _device(x=x, positions=positions, inv_freq=inv_freq, out=out)
-    with _launching(device, stream) as handle:
-        if out is None:
-            out = torch.empty(shape, dtype=x.dtype, device=device)
-        out_strides = _rows("out", _written("out", out), shape)
-        status = _lib.load().fa_sm100_rotary(
-            x.data_ptr(), (ctypes.c_longlong * 3)(*x_strides), out.data_ptr(), (ctypes.c_longlong * 3)(*out_strides),
-            batch, heads, tokens, dim, positions.data_ptr(), (ctypes.c_longlong * 2)(*strides), inv_freq.data_ptr(),
-            rotary_dim, (ctypes.c_int * len(sections))(*sections), len(sections), 1 if interleaved else 0,
-            1 if inverse else 0, handle)
-    _check(status, "fa_sm100_rotary")
+    index = x.get_device()
+    if index < 0 or not (index == positions.get_device() == inv_freq.get_device()) or (
+            out is not None and out.get_device() != index):
+        _device_error(x=x, positions=positions, inv_freq=inv_freq, out=out)
+    return _launch(_embed, index, stream, x, x_strides, positions, step[0], step[1] if len(at) == 3 else 0, inv_freq,
+                   rotary_dim, axes, packed, interleaved, inverse, out)
+
+
+def _embed(handle, x, x_strides, positions, axis_stride, batch_stride, inv_freq, rotary_dim, axes, packed, interleaved,
+           inverse, out):
+    shape = x.shape
+    if out is None:
+        out = x.new_empty(shape)
+    pack = _STRIDES[3]
+    status = _lib.load().fa_sm100_rotary(
+        x.data_ptr(), pack(*x_strides), out.data_ptr(), pack(*_rows("out", _written("out", out), shape)), *shape,
+        positions.data_ptr(), _STRIDES[2](axis_stride, batch_stride), inv_freq.data_ptr(), rotary_dim, packed, axes,
+        1 if interleaved else 0, 1 if inverse else 0, handle)
+    if status:
+        _check(status, "fa_sm100_rotary")
     return out
-
-
-def _caches(k_cache, v_cache):
-    if k_cache.dim() != 4:
-        raise ValueError("k_cache must be [num_pages, kv_heads, page_size, head_dim]")
-    shape = tuple(k_cache.shape)
-    return shape, _rows("k_cache", k_cache, shape), _rows("v_cache", v_cache, shape)
 
 
 def rotary_append(q, k, v, k_cache, v_cache, positions, slots, inv_freq, sections=None, interleaved=False, out=None,
@@ -313,42 +371,62 @@ def rotary_append(q, k, v, k_cache, v_cache, positions, slots, inv_freq, section
     interleaved: as in rotary_embed.
     """
     import torch
-    if q.dim() != 3 or k.dim() != 3:
-        raise ValueError("q and k must be [tokens, heads, head_dim]")
-    cache_shape, k_cache_strides, v_cache_strides = _caches(_written("k_cache", k_cache), _written("v_cache", v_cache))
+    cache_shape = k_cache.shape
+    if len(cache_shape) != 4:
+        raise ValueError("k_cache must be [num_pages, kv_heads, page_size, head_dim]")
     num_pages, kv_heads, page_size, dim = cache_shape
-    tokens, heads = q.shape[0], q.shape[1]
-    if dim not in (64, 128):
+    rows = q.shape
+    if len(rows) != 3:
+        raise ValueError("q must be [tokens, heads, head_dim]")
+    tokens = rows[0]
+    if dim != 128 and dim != 64:
         raise ValueError(f"head_dim must be 64 or 128, got {dim}")
     if page_size not in _PAGE_SIZES:
         raise ValueError(f"page_size must be one of {_PAGE_SIZES}, got {page_size}")
     if num_pages * page_size > _INT_MAX:
         raise ValueError("a cache must hold fewer than 2^31 tokens")
-    q_strides = _rows("q", q, (tokens, heads, dim))
-    k_strides = _rows("k", k, (tokens, kv_heads, dim))
-    v_strides = _rows("v", v, (tokens, kv_heads, dim))
-    rotary_dim, sections = _frequencies(inv_freq, dim, sections)
-    if positions.dim() == 1:
-        positions = positions[None]
-    _int32("positions", positions, 2)
-    if tuple(positions.shape) != (len(sections), tokens):
-        raise ValueError(f"positions must be {[len(sections), tokens]}, got {list(positions.shape)}")
-    if tokens > 1 and positions.stride(1) != 1:
+    if rows[2] != dim:
+        raise ValueError(f"q must have {dim} elements per head, got {rows[2]}")
+    kv_rows = (tokens, kv_heads, dim)
+    strides = (*_rows("k", k, kv_rows), *_rows("v", v, kv_rows),
+               *_rows("k_cache", _written("k_cache", k_cache), cache_shape),
+               *_rows("v_cache", _written("v_cache", v_cache), cache_shape))
+    q_strides = _rows("q", q, rows)
+    rotary_dim, axes, packed = _frequencies(inv_freq, dim, sections)
+    at, step = positions.shape, positions.stride()
+    if positions.dtype is not torch.int32 or not 1 <= len(at) <= 2:
+        _int32("positions", positions, 2)
+    if len(at) == 1:
+        at, step = (1, *at), (0, *step)
+    if at != (axes, tokens):
+        raise ValueError(f"positions must be {[axes, tokens]}, got {list(positions.shape)}")
+    if tokens > 1 and step[1] != 1:
         raise ValueError("positions must be contiguous in their last dimension")
-    _vector("slots", slots, tokens)
-    device = _device(q=q, k=k, v=v, k_cache=k_cache, v_cache=v_cache, positions=positions, slots=slots,
-                     inv_freq=inv_freq, out=out)
-    with _launching(device, stream) as handle:
-        if out is None:
-            out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=device)
-        out_strides = _rows("out", _written("out", out), (tokens, heads, dim))
-        strides = (*q_strides, *out_strides, *k_strides, *v_strides, *k_cache_strides, *v_cache_strides)
-        status = _lib.load().fa_sm100_rotary_append(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            (ctypes.c_longlong * 14)(*strides), tokens, heads, kv_heads, dim, page_size, num_pages,
-            positions.data_ptr(), positions.stride(0), slots.data_ptr(), inv_freq.data_ptr(), rotary_dim,
-            (ctypes.c_int * len(sections))(*sections), len(sections), 1 if interleaved else 0, handle)
-    _check(status, "fa_sm100_rotary_append")
+    if not (slots.dtype is torch.int32 and slots.shape == (tokens,) and slots.is_contiguous()):
+        _vector("slots", slots, tokens)
+    index = q.get_device()
+    if index < 0 or not (index == k.get_device() == v.get_device() == k_cache.get_device() == v_cache.get_device()
+                         == positions.get_device() == slots.get_device() == inv_freq.get_device()) or (
+            out is not None and out.get_device() != index):
+        _device_error(q=q, k=k, v=v, k_cache=k_cache, v_cache=v_cache, positions=positions, slots=slots,
+                      inv_freq=inv_freq, out=out)
+    return _launch(_append, index, stream, q, k, v, k_cache, v_cache, q_strides, strides, positions, step[0], slots,
+                   inv_freq, rotary_dim, axes, packed, interleaved, out)
+
+
+def _append(handle, q, k, v, k_cache, v_cache, q_strides, strides, positions, axis_stride, slots, inv_freq, rotary_dim,
+            axes, packed, interleaved, out):
+    rows = q.shape
+    if out is None:
+        out = q.new_empty(rows)
+    num_pages, kv_heads, page_size, dim = k_cache.shape
+    status = _lib.load().fa_sm100_rotary_append(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        _STRIDES[14](*q_strides, *_rows("out", _written("out", out), rows), *strides), rows[0], rows[1], kv_heads, dim,
+        page_size, num_pages, positions.data_ptr(), axis_stride, slots.data_ptr(), inv_freq.data_ptr(), rotary_dim,
+        packed, axes, 1 if interleaved else 0, handle)
+    if status:
+        _check(status, "fa_sm100_rotary_append")
     return out
 
 
@@ -360,25 +438,27 @@ def paged_attention(q, k_cache, v_cache, plan, out=None, stream=None):
     contiguous rows; the new tokens' K and V are in them. Returns out [total_tokens, heads, head_dim]
     (out may be q); padding rows are not written.
     """
-    import torch
-    shape, c = plan.shape, plan.c
+    shape = plan.shape
     rows = (plan.total_tokens, shape.heads, shape.head_dim)
+    cache = (plan.num_pages, shape.kv_heads, shape.page_size, shape.head_dim)
     q_strides = _rows("q", q, rows)
-    cache = (c.num_pages, shape.kv_heads, shape.page_size, shape.head_dim)
-    k_strides = _rows("k_cache", k_cache, cache)
-    v_strides = _rows("v_cache", v_cache, cache)
-    device = _device(q=q, k_cache=k_cache, v_cache=v_cache, out=out)
-    if device != plan.device:
-        raise ValueError(f"plan is on {plan.device}, other arguments on {device}")
-    lib = _lib.load()
-    with _launching(device, stream) as handle:
-        if out is None:
-            out = torch.empty(rows, dtype=q.dtype, device=device)
-        out_strides = _rows("out", _written("out", out), rows)
-        size = lib.fa_sm100_paged_workspace_bytes(plan._ref)
-        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        strides = (ctypes.c_longlong * 10)(*q_strides, *out_strides, *k_strides, *v_strides)
-        status = lib.fa_sm100_paged_fwd(plan._ref, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                                        out.data_ptr(), strides, workspace.data_ptr() if size else None, size, handle)
-    _check(status, "fa_sm100_paged_fwd")
+    strides = (*_rows("k_cache", k_cache, cache), *_rows("v_cache", v_cache, cache))
+    index = plan.device_index
+    if index < 0 or not (index == q.get_device() == k_cache.get_device() == v_cache.get_device()) or (
+            out is not None and out.get_device() != index):
+        _device_error(plan=plan._buffer, q=q, k_cache=k_cache, v_cache=v_cache, out=out)
+    return _launch(_attention, index, stream, q, k_cache, v_cache, plan, q_strides, strides, rows, out)
+
+
+def _attention(handle, q, k_cache, v_cache, plan, q_strides, strides, rows, out):
+    if out is None:
+        out = q.new_empty(rows)
+    size = plan._workspace
+    workspace = q.new_empty((size + 1) // 2) if size else None
+    status = _lib.load().fa_sm100_paged_fwd(
+        plan.c, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+        _STRIDES[10](*q_strides, *_rows("out", _written("out", out), rows), *strides),
+        workspace.data_ptr() if size else None, size, handle)
+    if status:
+        _check(status, "fa_sm100_paged_fwd")
     return out

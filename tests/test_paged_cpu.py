@@ -1,5 +1,6 @@
 """Refusals of the paged-cache operators, made on the host before any CUDA call."""
 import ctypes
+import struct
 
 import pytest
 import torch
@@ -21,8 +22,16 @@ def _bf16(*shape):
     return torch.zeros(shape, dtype=torch.bfloat16)
 
 
+class FaPagedPlan(ctypes.Structure):
+    """Layout of FaPagedPlan (include/fa_sm100_paged.h)."""
+    _fields_ = [(name, ctypes.c_int) for name in (
+        "num_seqs", "total_tokens", "max_new", "num_pages", "table_width", "table_stride", "heads", "kv_heads",
+        "head_dim", "page_size", "causal", "reserved")] + [(name, ctypes.c_void_p) for name in (
+            "query_start", "kv_lens", "positions", "slots", "block_table", "free_cursor", "schedule")]
+
+
 def _plan(**changes):
-    plan = _lib.FaPagedPlan()
+    plan = FaPagedPlan()
     values = dict(num_seqs=2, total_tokens=4, max_new=4, num_pages=8, table_width=4, table_stride=4, heads=8, kv_heads=2,
                   head_dim=128, page_size=16, causal=1, query_start=0x1000, kv_lens=0x1000, positions=0x1000,
                   slots=0x1000, block_table=0x1000, free_cursor=0x1000, schedule=0x1000)
@@ -152,8 +161,8 @@ def test_python_refusals():
         with pytest.raises(error):
             fa.rotary_append(**{**good, **change})
 
-    plan = fa.paged.PagedPlan(2, 5, shape, torch.device("cpu"))
-    plan.c.num_pages = 3
+    plan = fa.paged.PagedPlan(2, 5, shape, _i32(1))
+    plan.num_pages = 3
     good = dict(q=_bf16(5, 8, 64), k_cache=_bf16(3, 2, 16, 64), v_cache=_bf16(3, 2, 16, 64), plan=plan)
     for change, error in [
             (dict(q=_bf16(4, 8, 64)), ValueError), (dict(q=torch.zeros(5, 8, 64)), TypeError),
@@ -164,13 +173,19 @@ def test_python_refusals():
 
 
 def test_plan_views_are_the_struct_s_pointers():
-    plan = fa.paged.PagedPlan(3, 7, fa.PagedShape(8, 2, 64, 16), torch.device("cpu"))
+    """The packed struct has the C layout, and the views are where its pointers say."""
+    plan = fa.paged.PagedPlan(3, 7, fa.PagedShape(8, 2, 64, 16), _i32(1))
+    table = _i32(3, 9)[:, :5]
+    plan._fill(table, 5, 9, 11, 6, 1)
+    c = FaPagedPlan.from_buffer_copy(plan.c)
+    assert len(plan.c) == ctypes.sizeof(FaPagedPlan) == struct.calcsize("12i7P")
+    assert [getattr(c, n) for n, _ in FaPagedPlan._fields_[:12]] == [3, 7, 6, 11, 5, 9, 8, 2, 64, 16, 1, 0]
     for name, size in (("query_start", 4), ("kv_lens", 3), ("positions", 7), ("slots", 7), ("free_cursor", 1)):
         view = getattr(plan, name)
-        assert view.data_ptr() == getattr(plan.c, name) and view.shape == (size,) and view.dtype == torch.int32
-    end = plan.free_cursor.data_ptr() + 4
-    assert end <= plan._buffer.data_ptr() + 8 * plan._buffer.numel()
-    assert plan.c.query_start == plan.c.schedule + _lib.load().fa_sm100_paged_schedule_bytes(3)
+        assert view.data_ptr() == getattr(c, name) and view.shape == (size,) and view.dtype == torch.int32
+    assert c.block_table == table.data_ptr() and c.schedule == plan._buffer.data_ptr()
+    assert plan.free_cursor.data_ptr() + 4 == plan._buffer.data_ptr() + 4 * plan._buffer.numel()
+    assert c.query_start == c.schedule + _lib.load().fa_sm100_paged_schedule_bytes(3)
 
 
 def test_status_strings(lib):

@@ -70,7 +70,7 @@ def test_plan_schedule(cuda_device, group, causal):
     r = Requests(cached, new, 16, cuda_device)
     plan = r.plan(fa.PagedShape(group, 1, 64, 16), causal=causal)
     torch.cuda.synchronize()
-    got = plan._buffer[: 2 * (len(new) + 1)].view(2, -1).tolist()
+    got = plan._buffer[: 4 * (len(new) + 1)].view(torch.int64).view(2, -1).tolist()
     units = np.array([_units(c, n, group, causal) for c, n in zip(cached, new)])
     want = np.concatenate([np.zeros((1, 2), np.int64), np.cumsum(units, 0)]).T.tolist()
     assert got == want
