@@ -36,37 +36,52 @@ constexpr float kRebase = 16.0f;
 
 
 // =============================================================================
-// Narrow kernel: requests of at most 16 query rows per K/V head (decode steps)
+// Narrow kernel: requests of few query rows per K/V head (decode steps, drafted tokens)
 // =============================================================================
-// Each K/V byte is used for at most 16 rows, so the cache's bytes bound it: 512 bytes a key at
-// D = 128 against 16 * 4 * 128 operations. The work of all requests and K/V heads is one line of
-// 64-key tiles (request, then head, then key), and each of the grid's CTAs (two per SM) takes an
-// equal stretch of it, whatever the requests' lengths: a request that crosses a border is merged
-// from partial results by combine_narrow_kernel. A CTA's warp 4 streams the tiles by TMA through a
-// ring that runs on across requests, page by page (a page that is absent reads as zeros); warps
-// 0-3 take 16 keys of every tile each, S = Q K^T and O += P V by warp-level matrix instructions
-// with Q, P and O in registers, a running maximum and sum per warp, and meet only at a segment's
-// end. P is rounded to bf16 for the product with V (its sum is taken before); everything else
-// that is kept is 32-bit.
+// Each K/V byte is used for at most 32 rows, so the cache's bytes bound it: 512 bytes a key at
+// D = 128 against 32 * 4 * 128 operations. The work of all requests and K/V heads is one line of
+// 64-key tiles (request, then head, then key; each item preceded by kNarrowGap idle units that stand
+// for its set-up), and each of the grid's CTAs (two per SM) takes an equal stretch of it, whatever the
+// requests' lengths: an item that crosses a border is merged from parts by combine_narrow_kernel. A
+// CTA's warp 4 streams the tiles by TMA through a ring that runs on across items, page by page (a page
+// that is absent reads as zeros), with each item's Q and description ahead of its first tile; warps
+// 0-3 take 16 keys of every tile each, S = Q K^T and O += P V by warp-level matrix instructions with
+// P and O in registers, a running maximum and sum per warp, and meet only at an item's end, in the ring
+// slot of its last tile. P is rounded to bf16 for the product with V (its sum is taken before);
+// everything else that is kept is 32-bit. MT is the number of 16-row tiles of queries.
 constexpr int kNarrowWarps = 4;
 constexpr int kNarrowThreads = (kNarrowWarps + 1) * 32;
 constexpr int kNarrowCtasPerSm = 2;
-constexpr int kNarrowMinTiles = 2;       // tiles a CTA takes at least
+constexpr int kNarrowMinTiles = 3;       // units a CTA takes at least
 constexpr unsigned long long kTimeoutNs = 1000000000ull;
 
-template <int D>
+// What the producer tells the consumers of a stretch of one (request, K/V head).
+struct NarrowItem {
+    int token0, tokens, head0, kv;      // packed row of the first token, tokens, first query head, keys
+    int tile, count;                    // key tiles [tile, tile + count); count 0 ends the walk
+    int part;                           // place of its part, -1: the whole item, written directly
+    int reserved;
+};
+
+template <int D, int MT>
 struct NarrowCfg {
     static constexpr int kTile = kNarrowKeys * D * 2;               // bytes of a K or V tile
     static constexpr int kStage = 2 * kTile;
     static constexpr int kStages = D == 128 ? 3 : 6;                // 96 KB in flight per CTA
-    static constexpr int kQuarter = D / 4;                          // columns merged at a time
-    static constexpr int kMergeStride = kQuarter + 8;               // floats; the pad spreads rows over banks
-    static constexpr int kMergeOff = kStages * kStage;
-    static constexpr int kStatsOff = kMergeOff + kNarrowWarps * kNarrowRows * kMergeStride * 4;
-    static constexpr int kBarOff = kStatsOff + 2 * kNarrowWarps * kNarrowRows * 4;
-    static constexpr int kAbortOff = kBarOff + 2 * kStages * 8;
+    static constexpr int kQSlots = D == 128 ? (MT == 1 ? 3 : 1) : (MT == 1 ? 4 : 2);
+    static constexpr int kQStride = 2 * D + 16;                     // bytes; the pad spreads rows over banks
+    static constexpr int kQBytes = 16 * MT * kQStride;
+    static constexpr int kQOff = kStages * kStage;
+    static constexpr int kStatsOff = kQOff + kQSlots * kQBytes;     // [warp][row] maxima, then sums
+    static constexpr int kStats = kNarrowWarps * 16 * MT;
+    static constexpr int kItemOff = kStatsOff + 2 * kStats * 4;
+    static constexpr int kBarOff = kItemOff + kQSlots * static_cast<int>(sizeof(NarrowItem));
+    static constexpr int kNumBars = 2 * kStages + 2 * kQSlots;
+    static constexpr int kAbortOff = kBarOff + kNumBars * 8;
     static constexpr int kSmemBytes = kAbortOff + 16 + 1024;        // slack for 1024-byte alignment
-    static constexpr int kPartFloats = kNarrowRows * (D + 2);       // O [16][D], maxima [16], sums [16]
+    static constexpr int kPartFloats = 16 * MT * (D + 2);           // O [rows][D], maxima, sums
+    static_assert(kNarrowWarps * 16 * D * 4 == kStage, "a merge of 16 rows fits one ring slot");
+    static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
 };
 
 __device__ __forceinline__ void record_paged_timeout(volatile uint32_t* abort_flag, uint32_t site)
@@ -100,42 +115,55 @@ __device__ __forceinline__ void drain_paged(uint32_t bar, uint32_t parity)
         if (global_timer_ns() - begin > kTimeoutNs) return;
 }
 
-enum PagedSite : uint32_t { kSiteNarrowFull = 32, kSiteNarrowEmpty = 33 };
+enum PagedSite : uint32_t { kSiteNarrowFull = 32, kSiteNarrowEmpty = 33, kSiteNarrowItem = 34, kSiteNarrowItemFree = 35 };
 
-// A stretch of one (request, K/V head) inside a CTA's range.
-struct NarrowSegment {
+// Where x falls on the narrow line: the item's request and head, and its tiles' place [first, last).
+struct NarrowPlace {
     int b, h;
-    long long first, last;      // the item's tiles on the line: [first, last)
-    int tile, count;            // this stretch: tiles [tile, tile + count) of the item
+    long long first, last;
 };
 
-__device__ __forceinline__ NarrowSegment narrow_segment(const FaPagedPlan& plan, const long long* start, long long x,
-                                                        long long end)
+// For one warp, all lanes with the same arguments. 32 borders are read at a time, so a thousand
+// requests take two round trips to memory.
+__device__ __forceinline__ int find_request_warp(const long long* start, int num_seqs, long long y)
 {
-    NarrowSegment s;
-    s.b = find_request(start, plan.num_seqs, x / plan.kv_heads);
-    const long long tiles = start[s.b + 1] - start[s.b], base = start[s.b] * plan.kv_heads;
-    s.h = static_cast<int>((x - base) / tiles);
-    s.first = base + s.h * tiles;
-    s.last = s.first + tiles;
-    s.tile = static_cast<int>(x - s.first);
-    s.count = static_cast<int>((s.last < end ? s.last : end) - x);
+    const int lane = threadIdx.x % 32;
+    int lo = 0, count = num_seqs;           // the last b in [lo, lo + count) with start[b] <= y
+    while (count > 1) {
+        const int step = (count + 31) / 32;
+        const int at = lo + lane * step;
+        const bool below = lane * step < count && start[at] <= y;
+        const int last = 31 - __clz(static_cast<int>(__ballot_sync(0xffffffffu, below)));
+        lo += last * step;
+        count = min(step, count - last * step);
+    }
+    return lo;
+}
+
+__device__ __forceinline__ NarrowPlace narrow_place(const FaPagedPlan& plan, const long long* start, long long x)
+{
+    NarrowPlace s;
+    s.b = find_request_warp(start, plan.num_seqs, x / plan.kv_heads);
+    const long long units = start[s.b + 1] - start[s.b], base = start[s.b] * plan.kv_heads;
+    s.h = static_cast<int>((x - base) / units);
+    s.first = base + s.h * units + kNarrowGap;
+    s.last = s.first - kNarrowGap + units;
     return s;
 }
 
-// Tiles per CTA when `total` are shared out over `ctas`.
+// Units per CTA when `total` are shared out over `ctas`.
 __device__ __forceinline__ long long narrow_share(long long total, int ctas)
 {
     const long long even = (total + ctas - 1) / ctas;
     return even > kNarrowMinTiles ? even : kNarrowMinTiles;
 }
 
-template <int D>
+template <int D, int MT>
 __global__ void __launch_bounds__(kNarrowThreads, kNarrowCtasPerSm)
 paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                     const __grid_constant__ PagedParams p)
 {
-    using C = NarrowCfg<D>;
+    using C = NarrowCfg<D, MT>;
     const FaPagedPlan& plan = p.plan;
     const long long* start = narrow_starts(plan.schedule, plan.num_seqs);
     const long long total = start[plan.num_seqs] * plan.kv_heads;
@@ -150,15 +178,20 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const uint32_t base = (raw + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (base - raw);
     volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + C::kAbortOff);
-    auto full = [&](int s) -> uint32_t { return base + C::kBarOff + static_cast<uint32_t>(s) * 8u; };
-    auto empty = [&](int s) -> uint32_t { return base + C::kBarOff + static_cast<uint32_t>(C::kStages + s) * 8u; };
+    NarrowItem* items = reinterpret_cast<NarrowItem*>(smem + C::kItemOff);
+    auto bar = [&](int i) -> uint32_t { return base + C::kBarOff + static_cast<uint32_t>(i) * 8u; };
+    auto full = [&](int s) -> uint32_t { return bar(s); };
+    auto empty = [&](int s) -> uint32_t { return bar(C::kStages + s); };
+    auto item_full = [&](int s) -> uint32_t { return bar(2 * C::kStages + s); };
+    auto item_empty = [&](int s) -> uint32_t { return bar(2 * C::kStages + C::kQSlots + s); };
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < C::kStages; ++s) {
-            mbar_init(full(s), 1);
-            mbar_init(empty(s), kNarrowWarps);
+    const int group = plan.heads / plan.kv_heads;
+    if (warp == 0) {
+        for (int i = lane; i < C::kNumBars; i += 32) {
+            const bool released = (i >= C::kStages && i < 2 * C::kStages) || i >= 2 * C::kStages + C::kQSlots;
+            mbar_init(bar(i), released ? kNarrowWarps : 1);
         }
-        *abort_flag = 0u;
+        if (lane == 0) *abort_flag = 0u;
         fence_mbarrier_init();
     }
     __syncthreads();
@@ -174,13 +207,55 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         const int is_v = (lane / kBlocks) & 1, block = lane % kBlocks;
         const uint32_t offset = static_cast<uint32_t>(is_v * C::kTile + block * kNarrowKeys * 128 + page_of_tile * rows * 128);
         const void* map = is_v ? static_cast<const void*>(&tm_v) : static_cast<const void*>(&tm_k);
-        int it = 0;
+        int it = 0, sg = 0;
         bool ok = true;
-        for (long long x = begin; x < end && ok;) {
-            const NarrowSegment s = narrow_segment(plan, start, x, end);
-            x += s.count;
-            const int* table = plan.block_table + static_cast<long long>(s.b) * plan.table_stride;
-            const int held = (plan.kv_lens[s.b] + plan.page_size - 1) >> p.page_shift;
+        for (long long x = begin; ok;) {
+            NarrowItem item{};
+            int b = 0, h = 0;
+            if (x < end) {
+                const NarrowPlace s = narrow_place(plan, start, x);
+                if (x < s.first) x = s.first;
+                const long long stop = s.last < end ? s.last : end;
+                if (x >= stop) {                // only idle units are left of this range
+                    x = s.last;
+                    continue;
+                }
+                b = s.b;
+                h = s.h;
+                item.token0 = plan.query_start[b];
+                item.tokens = plan.query_start[b + 1] - item.token0;
+                item.head0 = h * group;
+                item.kv = plan.kv_lens[b];
+                item.tile = static_cast<int>(x - s.first);
+                item.count = static_cast<int>(stop - x);
+                // An item that began before this CTA's range leaves its part in the CTA's first place, one that
+                // goes on behind it in the second.
+                item.part = s.first < begin ? 2 * static_cast<int>(blockIdx.x)
+                                            : s.last > end ? 2 * static_cast<int>(blockIdx.x) + 1 : -1;
+                x = stop;
+            }
+            const int q_slot = sg % C::kQSlots;
+            if (sg >= C::kQSlots && !__all_sync(0xffffffffu, wait_paged(item_empty(q_slot), (sg / C::kQSlots - 1) & 1, abort_flag,
+                                                                         kSiteNarrowItemFree))) {
+                ok = false;
+                break;
+            }
+            const int q_rows = item.count > 0 ? item.tokens * group : 0;
+            if (lane == 0) {
+                items[q_slot] = item;
+                mbar_arrive_expect_tx(item_full(q_slot), static_cast<uint32_t>(q_rows * 2 * D));
+            }
+            __syncwarp();
+            ++sg;
+            if (item.count == 0) break;
+            if (lane < q_rows) {
+                const int tok = lane / group;
+                bulk_load(base + C::kQOff + q_slot * C::kQBytes + lane * C::kQStride,
+                          p.q + (item.token0 + tok) * p.q_token + (item.head0 + lane - tok * group) * p.q_head, 2 * D,
+                          item_full(q_slot));
+            }
+            const int* table = plan.block_table + static_cast<long long>(b) * plan.table_stride;
+            const int held = (item.kv + plan.page_size - 1) >> p.page_shift;
             auto page_at = [&](int tile) -> int {
                 // num_pages is out of the map's range: such a box reads as zeros.
                 const int i = ((tile * kNarrowKeys) >> p.page_shift) + page_of_tile;
@@ -190,10 +265,10 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 atomicOr(&g_paged_error_word, FA_ERROR_BAD_PAGE);
                 return plan.num_pages;
             };
-            int page = page_at(s.tile);
-            for (int i = 0; i < s.count; ++i, ++it) {
+            int page = page_at(item.tile);
+            for (int i = 0; i < item.count; ++i, ++it) {
                 const int slot = it % C::kStages, use = it / C::kStages;
-                const int row = ((s.tile + i) * kNarrowKeys) & (plan.page_size - 1);
+                const int row = ((item.tile + i) * kNarrowKeys) & (plan.page_size - 1);
                 if (use > 0 && !__all_sync(0xffffffffu, wait_paged(empty(slot), (use - 1) & 1, abort_flag, kSiteNarrowEmpty))) {
                     ok = false;
                     break;
@@ -201,24 +276,26 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 if (lane == 0) mbar_arrive_expect_tx(full(slot), C::kStage);
                 __syncwarp();
                 if (active)
-                    tma_load_4d(base + slot * C::kStage + offset, map, full(slot), block * 64, pages > 1 ? 0 : row, s.h, page);
-                if (i + 1 < s.count) page = page_at(s.tile + i + 1);
+                    tma_load_4d(base + slot * C::kStage + offset, map, full(slot), block * 64, pages > 1 ? 0 : row, h, page);
+                if (i + 1 < item.count) page = page_at(item.tile + i + 1);
             }
         }
-        if (!ok && lane == 0)
+        if (!ok && lane == 0) {
             for (int i = it > C::kStages ? it - C::kStages : 0; i < it; ++i) drain_paged(full(i % C::kStages), (i / C::kStages) & 1);
+            for (int i = sg > C::kQSlots ? sg - C::kQSlots : 0; i < sg; ++i)
+                drain_paged(item_full(i % C::kQSlots), (i / C::kQSlots) & 1);
+        }
         return;
     }
 
     // ======================= consumers =========================================
+    // A warp that gave up (ok false) still walks on, so that the others' barriers complete; nothing waits then.
     constexpr int kSteps = D / 16;
     constexpr int kNTiles = D / 8;
-    float* merge = reinterpret_cast<float*>(smem + C::kMergeOff);
-    float* stats = reinterpret_cast<float*>(smem + C::kStatsOff);      // [warp][16] maxima, then [warp][16] sums
+    float* stats = reinterpret_cast<float*>(smem + C::kStatsOff);
     const int g = lane >> 2, t = lane & 3;
-    const int group = plan.heads / plan.kv_heads;
     const float sl2 = p.scale_log2;
-    // ldmatrix rows of this lane within a tile (16 keys per warp), and their swizzle term.
+    // ldmatrix rows of this lane within a tile (16 keys per warp).
     const int k_row = warp * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, k_chunk = (lane >> 3) & 1;
     const int v_row = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, v_chunk = (lane >> 4) & 1;
     auto swizzled = [](int row, int chunk) -> uint32_t {
@@ -226,101 +303,122 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     };
     int it = 0;
     bool ok = true;
-    for (long long x = begin; x < end;) {
-        const NarrowSegment s = narrow_segment(plan, start, x, end);
-        x += s.count;
-        const int token0 = plan.query_start[s.b], n = plan.query_start[s.b + 1] - token0, kv = plan.kv_lens[s.b];
-        const int rows = n * group;
-        const int head0 = s.h * group;
-        // Rows g and g + 8 of the fragments; a row that does not exist is zero and goes nowhere.
-        const int tok_a = g / group, tok_b = (g + 8) / group;
-        const int limit_a = plan.causal ? kv - n + tok_a : kv - 1, limit_b = plan.causal ? kv - n + tok_b : kv - 1;
-        const int first_limit = plan.causal ? kv - n : kv - 1;
-        const uint32_t* qa_row = reinterpret_cast<const uint32_t*>(p.q + (token0 + tok_a) * p.q_token +
-                                                                   (head0 + g - tok_a * group) * p.q_head);
-        const uint32_t* qb_row = reinterpret_cast<const uint32_t*>(p.q + (token0 + tok_b) * p.q_token +
-                                                                   (head0 + g + 8 - tok_b * group) * p.q_head);
-        uint32_t qf[kSteps][4];
+    for (int sg = 0;; ++sg) {
+        const int q_slot = sg % C::kQSlots;
+        if (ok) ok = __all_sync(0xffffffffu, wait_paged(item_full(q_slot), (sg / C::kQSlots) & 1, abort_flag, kSiteNarrowItem));
+        // All four warps leave together, or none.
+        if (!named_barrier_and(1, kNarrowWarps * 32, ok)) break;
+        const NarrowItem item = items[q_slot];
+        if (item.count == 0) break;
+        const int rows = item.tokens * group;
+        const uint32_t q_addr = base + C::kQOff + q_slot * C::kQBytes +
+                                static_cast<uint32_t>(((lane & 7) + ((lane >> 3) & 1) * 8) * C::kQStride + (lane >> 4) * 16);
+        uint32_t qf[MT == 1 ? kSteps : 1][4];
+        if constexpr (MT == 1) {
 #pragma unroll
-        for (int kk = 0; kk < kSteps; ++kk) {
-            qf[kk][0] = g < rows ? qa_row[kk * 8 + t] : 0u;
-            qf[kk][1] = g + 8 < rows ? qb_row[kk * 8 + t] : 0u;
-            qf[kk][2] = g < rows ? qa_row[kk * 8 + t + 4] : 0u;
-            qf[kk][3] = g + 8 < rows ? qb_row[kk * 8 + t + 4] : 0u;
+            for (int kk = 0; kk < kSteps; ++kk) ldmatrix_x4(q_addr + kk * 32, qf[kk]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(item_empty(q_slot));
         }
-        float o[kNTiles][4];
+        const bool upper = MT > 1 && rows > 16;         // the second 16 rows exist
+        const int first_limit = plan.causal ? item.kv - item.tokens : item.kv - 1;
+        int limit[MT][2];                               // last key of rows g and g + 8 of each row tile
 #pragma unroll
-        for (int j = 0; j < kNTiles; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-        float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.0f, l_b = 0.0f;
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                limit[mt][e] = plan.causal ? first_limit + (16 * mt + 8 * e + g) / group : first_limit;
+        float o[MT][kNTiles][4];
+        float m[MT][2], l[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            m[mt][0] = m[mt][1] = -INFINITY;
+            l[mt][0] = l[mt][1] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kNTiles; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.0f;
+        }
 
-        for (int i = 0; i < s.count; ++i, ++it) {
+        for (int i = 0; i < item.count; ++i, ++it) {
             const int slot = it % C::kStages;
             if (ok) ok = __all_sync(0xffffffffu, wait_paged(full(slot), (it / C::kStages) & 1, abort_flag, kSiteNarrowFull));
-            const int key0 = (s.tile + i) * kNarrowKeys + warp * 16;
-            if (ok && key0 < kv) {
+            const int key0 = (item.tile + i) * kNarrowKeys + warp * 16;
+            if (ok && key0 < item.kv) {
                 const uint32_t k_tile = base + slot * C::kStage, v_tile = k_tile + C::kTile;
-                float sc[2][4] = {};
+                float sc[MT][2][4] = {};
 #pragma unroll
                 for (int kk = 0; kk < kSteps; ++kk) {
                     uint32_t b[4];
                     ldmatrix_x4(k_tile + swizzled(k_row, 2 * kk + k_chunk), b);
-                    mma_16816(sc[0], qf[kk], b[0], b[1]);
-                    mma_16816(sc[1], qf[kk], b[2], b[3]);
-                }
-                if (key0 + 15 > first_limit) {
+                    if constexpr (MT == 1) {
+                        mma_16816(sc[0][0], qf[kk], b[0], b[1]);
+                        mma_16816(sc[0][1], qf[kk], b[2], b[3]);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int key = key0 + 8 * j + 2 * t + e;
-                            if (key > limit_a) sc[j][e] = -INFINITY;
-                            if (key > limit_b) sc[j][2 + e] = -INFINITY;
+                        for (int mt = 0; mt < MT; ++mt) {
+                            if (mt > 0 && !upper) continue;
+                            ldmatrix_x4(q_addr + mt * 16 * C::kQStride + kk * 32, qf[0]);
+                            mma_16816(sc[mt][0], qf[0], b[0], b[1]);
+                            mma_16816(sc[mt][1], qf[0], b[2], b[3]);
                         }
-                }
-                float top_a = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
-                float top_b = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
-#pragma unroll
-                for (int d = 1; d < 4; d <<= 1) {
-                    top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, d));
-                    top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, d));
-                }
-                // The base of a row's exponents moves only when a score exceeds it by a factor 2^16 (a weight
-                // keeps its relative precision in bf16, sums are 32-bit), so O is rarely rescaled.
-                const bool move_a = (top_a - m_a) * sl2 > kRebase, move_b = (top_b - m_b) * sl2 > kRebase;
-                if (__any_sync(0xffffffffu, move_a || move_b)) {
-                    const float keep_a = move_a ? ex2_approx((m_a - top_a) * sl2) : 1.0f;
-                    const float keep_b = move_b ? ex2_approx((m_b - top_b) * sl2) : 1.0f;
-                    if (move_a) m_a = top_a;
-                    if (move_b) m_b = top_b;
-                    l_a *= keep_a;
-                    l_b *= keep_b;
-#pragma unroll
-                    for (int j = 0; j < kNTiles; ++j) {
-                        o[j][0] *= keep_a;
-                        o[j][1] *= keep_a;
-                        o[j][2] *= keep_b;
-                        o[j][3] *= keep_b;
                     }
                 }
-                const float base_a = m_a == -INFINITY ? 0.0f : m_a * sl2, base_b = m_b == -INFINITY ? 0.0f : m_b * sl2;
-                uint32_t pf[4];
+                uint32_t pf[MT][4];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float a0 = ex2_approx(fmaf(sc[j][0], sl2, -base_a)), a1 = ex2_approx(fmaf(sc[j][1], sl2, -base_a));
-                    const float b0 = ex2_approx(fmaf(sc[j][2], sl2, -base_b)), b1 = ex2_approx(fmaf(sc[j][3], sl2, -base_b));
-                    l_a += a0 + a1;
-                    l_b += b0 + b1;
-                    pf[2 * j] = pack_bf16x2(a0, a1);
-                    pf[2 * j + 1] = pack_bf16x2(b0, b1);
+                for (int mt = 0; mt < MT; ++mt) {
+                    if (mt > 0 && !upper) continue;
+                    float(&s)[2][4] = sc[mt];
+                    if (key0 + 15 > first_limit) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (key0 + 8 * j + 2 * t + (e & 1) > limit[mt][e >> 1]) s[j][e] = -INFINITY;
+                    }
+                    float top[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        top[e] = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+#pragma unroll
+                        for (int d = 1; d < 4; d <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], d));
+                    }
+                    // The base of a row's exponents moves only when a score exceeds it by a factor 2^16 (a weight
+                    // keeps its relative precision in bf16, sums are 32-bit), so O is rarely rescaled.
+                    const bool move0 = (top[0] - m[mt][0]) * sl2 > kRebase, move1 = (top[1] - m[mt][1]) * sl2 > kRebase;
+                    if (__any_sync(0xffffffffu, move0 || move1)) {
+                        const float keep0 = move0 ? ex2_approx((m[mt][0] - top[0]) * sl2) : 1.0f;
+                        const float keep1 = move1 ? ex2_approx((m[mt][1] - top[1]) * sl2) : 1.0f;
+                        if (move0) m[mt][0] = top[0];
+                        if (move1) m[mt][1] = top[1];
+                        l[mt][0] *= keep0;
+                        l[mt][1] *= keep1;
+#pragma unroll
+                        for (int j = 0; j < kNTiles; ++j) {
+                            o[mt][j][0] *= keep0;
+                            o[mt][j][1] *= keep0;
+                            o[mt][j][2] *= keep1;
+                            o[mt][j][3] *= keep1;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float base_e = m[mt][e] == -INFINITY ? 0.0f : m[mt][e] * sl2;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const float w0 = ex2_approx(fmaf(s[j][2 * e], sl2, -base_e));
+                            const float w1 = ex2_approx(fmaf(s[j][2 * e + 1], sl2, -base_e));
+                            l[mt][e] += w0 + w1;
+                            pf[mt][2 * j + e] = pack_bf16x2(w0, w1);
+                        }
+                    }
                 }
                 // V rows behind the last key may hold anything: they are zeroed in the fragments (fragment
                 // register 0 holds keys 2t and 2t + 1 of the 16, register 1 the same plus 8).
                 uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-                const bool tail = key0 + 15 >= kv;
+                const bool tail = key0 + 15 >= item.kv;
                 if (tail) {
                     const int k0 = key0 + 2 * t;
-                    keep0 = (k0 < kv ? 0xffffu : 0u) | (k0 + 1 < kv ? 0xffff0000u : 0u);
-                    keep1 = (k0 + 8 < kv ? 0xffffu : 0u) | (k0 + 9 < kv ? 0xffff0000u : 0u);
+                    keep0 = (k0 < item.kv ? 0xffffu : 0u) | (k0 + 1 < item.kv ? 0xffff0000u : 0u);
+                    keep1 = (k0 + 8 < item.kv ? 0xffffu : 0u) | (k0 + 9 < item.kv ? 0xffff0000u : 0u);
                 }
 #pragma unroll
                 for (int dd = 0; dd < kSteps; ++dd) {
@@ -332,130 +430,140 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                         b[2] &= keep0;
                         b[3] &= keep1;
                     }
-                    mma_16816(o[2 * dd], pf, b[0], b[1]);
-                    mma_16816(o[2 * dd + 1], pf, b[2], b[3]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        if (mt > 0 && !upper) continue;
+                        mma_16816(o[mt][2 * dd], pf[mt], b[0], b[1]);
+                        mma_16816(o[mt][2 * dd + 1], pf[mt], b[2], b[3]);
+                    }
                 }
             }
+            // The last tile's slot is kept for the merge below.
+            if (i + 1 < item.count) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty(slot));
+            }
+        }
+        if constexpr (MT > 1) {
             __syncwarp();
-            if (lane == 0) mbar_arrive(empty(slot));
+            if (lane == 0) mbar_arrive(item_empty(q_slot));
         }
 
-        // ---- the four warps' results become one --------------------------------
+        // ---- the four warps' results become one, in the slot of the last tile ----
+        const int last_slot = (it - 1) % C::kStages;
+        float* merge = reinterpret_cast<float*>(smem + last_slot * C::kStage);
+        // [warp][row][column], the columns of a row exchanged in groups of 8 so that the rows of a half warp
+        // fall on different banks.
+        auto merge_at = [&](int w, int row, int column) -> float2* {
+            return reinterpret_cast<float2*>(merge + (w * 16 + row) * D + (column ^ ((row & 3) * 8)));
+        };
+        float mine[MT][2];
 #pragma unroll
-        for (int d = 1; d < 4; d <<= 1) {
-            l_a += __shfl_xor_sync(0xffffffffu, l_a, d);
-            l_b += __shfl_xor_sync(0xffffffffu, l_b, d);
-        }
-        if (t == 0) {
-            stats[warp * 16 + g] = m_a;
-            stats[warp * 16 + g + 8] = m_b;
-            stats[64 + warp * 16 + g] = l_a;
-            stats[64 + warp * 16 + g + 8] = l_b;
-        }
-        named_barrier(1, kNarrowWarps * 32);
-        float all_a = -INFINITY, all_b = -INFINITY;
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int w = 0; w < kNarrowWarps; ++w) {
-            all_a = fmaxf(all_a, stats[w * 16 + g]);
-            all_b = fmaxf(all_b, stats[w * 16 + g + 8]);
-        }
-        float sum_a = 0.0f, sum_b = 0.0f, mine_a = 0.0f, mine_b = 0.0f;
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
-        for (int w = 0; w < kNarrowWarps; ++w) {
-            const float ma = stats[w * 16 + g], mb = stats[w * 16 + g + 8];
-            const float wa = ma == -INFINITY ? 0.0f : ex2_approx((ma - all_a) * sl2);
-            const float wb = mb == -INFINITY ? 0.0f : ex2_approx((mb - all_b) * sl2);
-            sum_a += wa * stats[64 + w * 16 + g];
-            sum_b += wb * stats[64 + w * 16 + g + 8];
-            if (w == warp) { mine_a = wa; mine_b = wb; }
-        }
-        const bool whole = s.tile == 0 && s.tile + s.count == s.last - s.first;
-        // An item that began before this CTA's range leaves its part in the CTA's first place, one that
-        // goes on behind it in the second.
-        float* part = p.partial + (2LL * blockIdx.x + (s.first < begin ? 0 : 1)) * C::kPartFloats;
-        const float inv_a = whole ? 1.0f / sum_a : 1.0f, inv_b = whole ? 1.0f / sum_b : 1.0f;
-        constexpr int kPer = kNTiles / 4;
-#pragma unroll
-        for (int quarter = 0; quarter < 4; ++quarter) {
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const float(&v)[4] = o[quarter * kPer + j];
-                float* at = merge + (warp * 16 + g) * C::kMergeStride + 8 * j + 2 * t;
-                *reinterpret_cast<float2*>(at) = make_float2(v[0] * mine_a, v[1] * mine_a);
-                *reinterpret_cast<float2*>(at + 8 * C::kMergeStride) = make_float2(v[2] * mine_b, v[3] * mine_b);
-            }
-            named_barrier(1, kNarrowWarps * 32);
-            if (warp == quarter) {
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) {
-                    float2 a = make_float2(0.0f, 0.0f), b = a;
-#pragma unroll
-                    for (int w = 0; w < kNarrowWarps; ++w) {
-                        const float* at = merge + (w * 16 + g) * C::kMergeStride + 8 * j + 2 * t;
-                        const float2 va = *reinterpret_cast<const float2*>(at);
-                        const float2 vb = *reinterpret_cast<const float2*>(at + 8 * C::kMergeStride);
-                        a.x += va.x;
-                        a.y += va.y;
-                        b.x += vb.x;
-                        b.y += vb.y;
-                    }
-                    const int column = quarter * C::kQuarter + 8 * j + 2 * t;
-                    if (!ok) continue;
-                    if (whole) {
-                        if (g < rows)
-                            *reinterpret_cast<uint32_t*>(p.o + (token0 + tok_a) * p.o_token +
-                                                         (head0 + g - tok_a * group) * p.o_head + column) =
-                                pack_bf16x2(a.x * inv_a, a.y * inv_a);
-                        if (g + 8 < rows)
-                            *reinterpret_cast<uint32_t*>(p.o + (token0 + tok_b) * p.o_token +
-                                                         (head0 + g + 8 - tok_b * group) * p.o_head + column) =
-                                pack_bf16x2(b.x * inv_b, b.y * inv_b);
-                    } else {
-                        if (g < rows) *reinterpret_cast<float2*>(part + g * D + column) = a;
-                        if (g + 8 < rows) *reinterpret_cast<float2*>(part + (g + 8) * D + column) = b;
-                    }
+                for (int d = 1; d < 4; d <<= 1) l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], d);
+                if (t == 0) {
+                    stats[(warp * MT + mt) * 16 + 8 * e + g] = m[mt][e];
+                    stats[C::kStats + (warp * MT + mt) * 16 + 8 * e + g] = l[mt][e];
                 }
             }
+        named_barrier(1, kNarrowWarps * 32);        // all warps are done with the slot's tile
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            if (mt > 0 && !upper) continue;
+            float all[2], sum[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float* at = stats + mt * 16 + 8 * e + g;
+                all[e] = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kNarrowWarps; ++w) all[e] = fmaxf(all[e], at[w * MT * 16]);
+                sum[e] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kNarrowWarps; ++w) {
+                    const float mw = at[w * MT * 16];
+                    const float weight = mw == -INFINITY ? 0.0f : ex2_approx((mw - all[e]) * sl2);
+                    sum[e] += weight * at[C::kStats + w * MT * 16];
+                    if (w == warp) mine[mt][e] = weight;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kNTiles; ++j) {
+                const float(&v)[4] = o[mt][j];
+                *merge_at(warp, g, 8 * j + 2 * t) = make_float2(v[0] * mine[mt][0], v[1] * mine[mt][0]);
+                if (rows > 16 * mt + 8)
+                    *merge_at(warp, g + 8, 8 * j + 2 * t) = make_float2(v[2] * mine[mt][1], v[3] * mine[mt][1]);
+            }
             named_barrier(1, kNarrowWarps * 32);
+            // Warp w adds up and writes columns [w * D / 4, (w + 1) * D / 4).
+            float* part = p.partial + static_cast<long long>(item.part) * C::kPartFloats;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = 16 * mt + 8 * e + g;
+                if (!ok || row >= rows) continue;
+                const int tok = row / group;
+                __nv_bfloat16* out = p.o + static_cast<long long>(item.token0 + tok) * p.o_token +
+                                     static_cast<long long>(item.head0 + row - tok * group) * p.o_head;
+                const float inv = 1.0f / sum[e];
+#pragma unroll
+                for (int j = 0; j < kNTiles / 4; ++j) {
+                    const int column = warp * (D / 4) + 8 * j + 2 * t;
+                    float2 a = make_float2(0.0f, 0.0f);
+#pragma unroll
+                    for (int w = 0; w < kNarrowWarps; ++w) {
+                        const float2 v = *merge_at(w, 8 * e + g, column);
+                        a.x += v.x;
+                        a.y += v.y;
+                    }
+                    if (item.part < 0) *reinterpret_cast<uint32_t*>(out + column) = pack_bf16x2(a.x * inv, a.y * inv);
+                    else *reinterpret_cast<float2*>(part + row * D + column) = a;
+                }
+                if (item.part >= 0 && warp == 0 && t == 0) {
+                    part[16 * MT * D + row] = all[e];
+                    part[16 * MT * D + 16 * MT + row] = sum[e];
+                }
+            }
+            if (mt + 1 < MT && upper) named_barrier(1, kNarrowWarps * 32);
         }
-        if (!whole && warp == 0 && t == 0) {
-            part[16 * D + g] = all_a;
-            part[16 * D + g + 8] = all_b;
-            part[16 * D + 16 + g] = sum_a;
-            part[16 * D + 16 + g + 8] = sum_b;
-        }
+        // The slot goes back to the copies: what was read and written here comes before them.
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(last_slot));
     }
 }
 
 // One block per border between two CTAs' ranges; the first border inside an item merges the item's
 // parts, in their order, one warp per row. It is launched while the narrow kernel still runs
 // (programmatic dependent launch) and finds its item meanwhile.
-template <int D>
-__global__ void __launch_bounds__(kNarrowRows * 32)
+template <int D, int MT>
+__global__ void __launch_bounds__(512)
 combine_narrow_kernel(const __grid_constant__ PagedParams p, int ctas)
 {
-    using C = NarrowCfg<D>;
+    using C = NarrowCfg<D, MT>;
     const FaPagedPlan& plan = p.plan;
     const long long* start = narrow_starts(plan.schedule, plan.num_seqs);
     const long long total = start[plan.num_seqs] * plan.kv_heads;
     const long long share = narrow_share(total, ctas);
     const long long border = share * (blockIdx.x + 1);
-    const int row = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int row = 16 * static_cast<int>(blockIdx.y) + threadIdx.x / 32, lane = threadIdx.x % 32;
     int count = 0;                          // parts of this block's item (0: none to merge here)
     const float* first = nullptr;           // the first ends its CTA's range; the others begin theirs
     __nv_bfloat16* out = nullptr;
     constexpr int E = D / 32;
     constexpr long long kNext = 2LL * C::kPartFloats;
     if (border < total) {
-        const NarrowSegment s = narrow_segment(plan, start, border, total);
+        const NarrowPlace s = narrow_place(plan, start, border);
         const int token0 = plan.query_start[s.b], n = plan.query_start[s.b + 1] - token0;
         const int group = plan.heads / plan.kv_heads;
-        if (s.first != border && s.first >= border - share && row < n * group) {
+        if (s.first < border && s.first >= border - share && row < n * group) {
             const long long c0 = s.first / share;
             count = static_cast<int>((s.last - 1) / share - c0) + 1;
             first = p.partial + (2 * c0 + 1) * C::kPartFloats;
             const int tok = row / group;
-            out = p.o + (token0 + tok) * p.o_token + (s.h * group + row - tok * group) * p.o_head + lane * E;
+            out = p.o + static_cast<long long>(token0 + tok) * p.o_token +
+                  static_cast<long long>(s.h * group + row - tok * group) * p.o_head + lane * E;
         }
     }
     grid_dependency_wait();
@@ -465,8 +573,8 @@ combine_narrow_kernel(const __grid_constant__ PagedParams p, int ctas)
     float top = -INFINITY, sum = 0.0f, acc[E] = {};
     for (int i0 = 0; i0 < count; i0 += 32) {
         const int mine = i0 + lane;
-        const float m = mine < count ? part(mine)[16 * D + row] : -INFINITY;
-        const float l = mine < count ? part(mine)[16 * D + 16 + row] : 0.0f;
+        const float m = mine < count ? part(mine)[16 * MT * D + row] : -INFINITY;
+        const float l = mine < count ? part(mine)[16 * MT * D + 16 * MT + row] : 0.0f;
         float high = fmaxf(m, top);
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
@@ -1259,11 +1367,14 @@ int prepare_paged_device(int device)
 {
     PagedDevice& state = g_paged_devices[device];
     std::call_once(state.once, [&]() {
-        cudaError_t err = cudaFuncSetAttribute(reinterpret_cast<const void*>(paged_narrow_kernel<64>),
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, NarrowCfg<64>::kSmemBytes);
-        if (err == cudaSuccess)
-            err = cudaFuncSetAttribute(reinterpret_cast<const void*>(paged_narrow_kernel<128>),
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, NarrowCfg<128>::kSmemBytes);
+        struct { const void* kernel; int bytes; } const narrow[] = {
+            {reinterpret_cast<const void*>(paged_narrow_kernel<64, 1>), NarrowCfg<64, 1>::kSmemBytes},
+            {reinterpret_cast<const void*>(paged_narrow_kernel<64, 2>), NarrowCfg<64, 2>::kSmemBytes},
+            {reinterpret_cast<const void*>(paged_narrow_kernel<128, 1>), NarrowCfg<128, 1>::kSmemBytes},
+            {reinterpret_cast<const void*>(paged_narrow_kernel<128, 2>), NarrowCfg<128, 2>::kSmemBytes}};
+        cudaError_t err = cudaSuccess;
+        for (int i = 0; i < 4 && err == cudaSuccess; ++i)
+            err = cudaFuncSetAttribute(narrow[i].kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, narrow[i].bytes);
         const void* const wide[] = {reinterpret_cast<const void*>(paged_wide_kernel<64>),
                                     reinterpret_cast<const void*>(paged_wide_kernel<128>)};
         for (int i = 0; i < 2 && err == cudaSuccess; ++i) {
@@ -1285,9 +1396,9 @@ int prepare_paged_device(int device)
 
 int narrow_ctas(int sms) { return kNarrowCtasPerSm * sms; }
 
-size_t narrow_workspace(int sms, int head_dim)
+size_t narrow_workspace(int sms, const FaPagedPlan& plan)
 {
-    return static_cast<size_t>(narrow_ctas(sms)) * 2 * kNarrowRows * (head_dim + 2) * sizeof(float);
+    return static_cast<size_t>(narrow_ctas(sms)) * 2 * narrow_rows(plan) * (plan.head_dim + 2) * sizeof(float);
 }
 
 size_t wide_workspace(int sms, int head_dim)
@@ -1296,16 +1407,15 @@ size_t wide_workspace(int sms, int head_dim)
 }
 
 // Which kernels a plan's requests can need: decided from the sizes that the host knows.
-bool may_be_narrow(const FaPagedPlan& plan) { return plan.heads / plan.kv_heads <= kNarrowRows; }
+bool may_be_narrow(const FaPagedPlan& plan) { return plan.heads / plan.kv_heads <= narrow_rows(plan); }
 bool may_be_wide(const FaPagedPlan& plan)
 {
-    const long long most = plan.max_new < plan.total_tokens ? plan.max_new : plan.total_tokens;
-    return most * (plan.heads / plan.kv_heads) > kNarrowRows;
+    return most_rows(plan) > narrow_rows(plan);
 }
 
 size_t workspace_bytes_of(const FaPagedPlan& plan, int sms)
 {
-    return (may_be_narrow(plan) ? narrow_workspace(sms, plan.head_dim) : 0) +
+    return (may_be_narrow(plan) ? narrow_workspace(sms, plan) : 0) +
            (may_be_wide(plan) ? wide_workspace(sms, plan.head_dim) : 0);
 }
 
@@ -1337,14 +1447,14 @@ int launch_early(void (*kernel)(Args...), dim3 grid, int threads, cudaStream_t s
     return static_cast<int>(cudaLaunchKernelEx(&config, kernel, args...));
 }
 
-template <int D>
+template <int D, int MT>
 int launch_narrow(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const PagedParams& params, int sms, cudaStream_t stream)
 {
     const int ctas = narrow_ctas(sms);
-    paged_narrow_kernel<D><<<ctas, kNarrowThreads, NarrowCfg<D>::kSmemBytes, stream>>>(tm_k, tm_v, params);
+    paged_narrow_kernel<D, MT><<<ctas, kNarrowThreads, NarrowCfg<D, MT>::kSmemBytes, stream>>>(tm_k, tm_v, params);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return static_cast<int>(err);
-    return launch_early(combine_narrow_kernel<D>, dim3(ctas - 1), kNarrowRows * 32, stream, params, ctas);
+    return launch_early(combine_narrow_kernel<D, MT>, dim3(ctas - 1, MT), 512, stream, params, ctas);
 }
 
 template <int D>
@@ -1440,8 +1550,11 @@ int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cac
     if (may_be_narrow(*plan)) {
         params.partial = reinterpret_cast<float*>(work);
         if ((status = cache_maps(kNarrowKeys)) != FA_STATUS_OK) return status;
-        status = plan->head_dim == 64 ? launch_narrow<64>(tm_k, tm_v, params, sms, s)
-                                      : launch_narrow<128>(tm_k, tm_v, params, sms, s);
+        const bool one = narrow_rows(*plan) == 16;
+        if (plan->head_dim == 64)
+            status = one ? launch_narrow<64, 1>(tm_k, tm_v, params, sms, s) : launch_narrow<64, 2>(tm_k, tm_v, params, sms, s);
+        else
+            status = one ? launch_narrow<128, 1>(tm_k, tm_v, params, sms, s) : launch_narrow<128, 2>(tm_k, tm_v, params, sms, s);
     }
     return status;
 }

@@ -2,9 +2,10 @@
 // and how a linear range of it maps back to requests.
 //
 // A request with n new tokens and a group of G query heads per K/V head has n * G query
-// rows per K/V head (row = token * G + head in group). Requests of at most kNarrowRows rows
-// go to the narrow kernel, whose unit of work is a 64-key tile; all others to the wide
-// kernel, whose unit is a 128-key tile of a block of 2 * tokens_per_tile(G) tokens.
+// rows per K/V head (row = token * G + head in group). Requests of at most narrow_rows(plan) rows
+// go to the narrow kernel, whose unit of work is a 64-key tile; all others to the wide kernel,
+// whose unit is a 128-key tile of a block of 2 * tokens_per_tile(G) tokens. Each narrow item (one
+// K/V head of a request) is preceded by kNarrowGap units without work, about what its set-up costs.
 #pragma once
 
 #include <cstdint>
@@ -13,7 +14,7 @@
 
 namespace fa_sm100 {
 
-constexpr int kNarrowRows = 16;
+constexpr int kNarrowGap = 1;
 constexpr int kNarrowKeys = 64;
 constexpr int kWideRows = 128;      // query rows of one tile (tensor-memory lanes)
 constexpr int kWideKeys = 128;
@@ -23,6 +24,19 @@ static_assert(kWideKeys == 128, "floor_sum_128 counts key tiles");
 // requests' units for one K/V head.
 __host__ __device__ inline long long* narrow_starts(long long* schedule, int) { return schedule; }
 __host__ __device__ inline long long* wide_starts(long long* schedule, int num_seqs) { return schedule + num_seqs + 1; }
+
+// Query rows per K/V head that any request of the plan can have, and the most that go to the narrow
+// kernel: 32 where no request has more (drafted tokens), else 16, which its faster variant holds.
+__host__ __device__ inline long long most_rows(const FaPagedPlan& plan)
+{
+    return static_cast<long long>(plan.max_new < plan.total_tokens ? plan.max_new : plan.total_tokens) *
+           (plan.heads / plan.kv_heads);
+}
+__host__ __device__ inline int narrow_rows(const FaPagedPlan& plan)
+{
+    const long long most = most_rows(plan);
+    return most > 16 && most <= 32 ? 32 : 16;
+}
 
 __host__ __device__ inline int tokens_per_tile(int group) { return kWideRows / group; }
 __host__ __device__ inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }

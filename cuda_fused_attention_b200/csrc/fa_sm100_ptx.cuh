@@ -83,6 +83,13 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, uint3
         : "memory");
 }
 
+// Untiled copy of `bytes` (a multiple of 16, both ends 16-byte aligned) into this CTA's shared memory.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, uint32_t bar, int c0, int c1, int c2, int c3)
 {
     asm volatile(
@@ -142,6 +149,21 @@ __device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddep
 __device__ __forceinline__ void named_barrier(int id, int threads)
 {
     asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(threads) : "memory");
+}
+
+// The same barrier, which also tells every thread whether all of them brought a true value.
+__device__ __forceinline__ bool named_barrier_and(int id, int threads, bool value)
+{
+    uint32_t all;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %3, 0;\n\t"
+        "bar.red.and.pred q, %1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t"
+        "}\n"
+        : "=r"(all) : "r"(id), "r"(threads), "r"(value ? 1u : 0u) : "memory");
+    return all != 0;
 }
 
 // ---------------------------------------------------------------------------
