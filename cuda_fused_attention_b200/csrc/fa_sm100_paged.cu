@@ -45,10 +45,10 @@ constexpr float kRebase = 16.0f;
 // requests' lengths: an item that crosses a border is merged from parts by combine_narrow_kernel. A
 // CTA's warp 4 streams the tiles by TMA through a ring that runs on across items, page by page (a page
 // that is absent reads as zeros), with each item's Q and description ahead of its first tile; warps
-// 0-3 take 16 keys of every tile each, S = Q K^T and O += P V by warp-level matrix instructions with
-// P and O in registers, a running maximum and sum per warp, and meet only at an item's end, in the ring
-// slot of its last tile. P is rounded to bf16 for the product with V (its sum is taken before);
-// everything else that is kept is 32-bit. MT is the number of 16-row tiles of queries.
+// 0-3 share out the keys of every tile (and the two 16-row tiles, if MT, their number, is 2), S = Q K^T
+// and O += P V by warp-level matrix instructions with Q, P and O in registers, a running maximum and
+// sum per warp, and meet only at an item's end, in the ring slot of its last tile. P is rounded to bf16 for the product with V (its sum is taken before);
+// everything else that is kept is 32-bit.
 constexpr int kNarrowWarps = 4;
 constexpr int kNarrowThreads = (kNarrowWarps + 1) * 32;
 constexpr int kNarrowCtasPerSm = 2;
@@ -68,19 +68,19 @@ struct NarrowCfg {
     static constexpr int kTile = kNarrowKeys * D * 2;               // bytes of a K or V tile
     static constexpr int kStage = 2 * kTile;
     static constexpr int kStages = D == 128 ? 3 : 6;                // 96 KB in flight per CTA
-    static constexpr int kQSlots = D == 128 ? (MT == 1 ? 3 : 1) : (MT == 1 ? 4 : 2);
+    static constexpr int kQSlots = D == 128 ? (MT == 1 ? 3 : 1) : (MT == 1 ? 4 : 2);    // as many as fit
     static constexpr int kQStride = 2 * D + 16;                     // bytes; the pad spreads rows over banks
     static constexpr int kQBytes = 16 * MT * kQStride;
     static constexpr int kQOff = kStages * kStage;
-    static constexpr int kStatsOff = kQOff + kQSlots * kQBytes;     // [warp][row] maxima, then sums
-    static constexpr int kStats = kNarrowWarps * 16 * MT;
+    static constexpr int kStatsOff = kQOff + kQSlots * kQBytes;     // [key group][row] maxima, then sums
+    static constexpr int kStats = kNarrowWarps * 16;
     static constexpr int kItemOff = kStatsOff + 2 * kStats * 4;
     static constexpr int kBarOff = kItemOff + kQSlots * static_cast<int>(sizeof(NarrowItem));
     static constexpr int kNumBars = 2 * kStages + 2 * kQSlots;
     static constexpr int kAbortOff = kBarOff + kNumBars * 8;
     static constexpr int kSmemBytes = kAbortOff + 16 + 1024;        // slack for 1024-byte alignment
     static constexpr int kPartFloats = 16 * MT * (D + 2);           // O [rows][D], maxima, sums
-    static_assert(kNarrowWarps * 16 * D * 4 == kStage, "a merge of 16 rows fits one ring slot");
+    static_assert(kNarrowWarps * 16 * D * 4 == kStage, "a merge fits one ring slot");
     static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
 };
 
@@ -289,15 +289,19 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     }
 
     // ======================= consumers =========================================
-    // A warp that gave up (ok false) still walks on, so that the others' barriers complete; nothing waits then.
+    // Warp (kg, mt) takes 16 * MT keys of each tile for 16 query rows. A warp that gave up (ok false) still
+    // walks on, so that the others' barriers complete; nothing waits then.
     constexpr int kSteps = D / 16;
     constexpr int kNTiles = D / 8;
+    constexpr int kGroups = kNarrowWarps / MT;      // warps that share out a tile's keys
+    constexpr int kKeys = kNarrowKeys / kGroups;    // keys of a warp, 16 * MT
     float* stats = reinterpret_cast<float*>(smem + C::kStatsOff);
+    const int mt = warp % MT, kg = warp / MT;
     const int g = lane >> 2, t = lane & 3;
     const float sl2 = p.scale_log2;
-    // ldmatrix rows of this lane within a tile (16 keys per warp).
-    const int k_row = warp * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, k_chunk = (lane >> 3) & 1;
-    const int v_row = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, v_chunk = (lane >> 4) & 1;
+    // ldmatrix rows of this lane within a tile.
+    const int k_row = kg * kKeys + (lane & 7) + ((lane >> 4) & 1) * 8, k_chunk = (lane >> 3) & 1;
+    const int v_row = kg * kKeys + (lane & 7) + ((lane >> 3) & 1) * 8, v_chunk = (lane >> 4) & 1;
     auto swizzled = [](int row, int chunk) -> uint32_t {
         return static_cast<uint32_t>((chunk >> 3) * kNarrowKeys * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
     };
@@ -311,130 +315,112 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         const NarrowItem item = items[q_slot];
         if (item.count == 0) break;
         const int rows = item.tokens * group;
+        const bool busy = 16 * mt < rows;           // this warp has rows
+        uint32_t qf[kSteps][4];
         const uint32_t q_addr = base + C::kQOff + q_slot * C::kQBytes +
-                                static_cast<uint32_t>(((lane & 7) + ((lane >> 3) & 1) * 8) * C::kQStride + (lane >> 4) * 16);
-        uint32_t qf[MT == 1 ? kSteps : 1][4];
-        if constexpr (MT == 1) {
+                                static_cast<uint32_t>((16 * mt + (lane & 7) + ((lane >> 3) & 1) * 8) * C::kQStride + (lane >> 4) * 16);
 #pragma unroll
-            for (int kk = 0; kk < kSteps; ++kk) ldmatrix_x4(q_addr + kk * 32, qf[kk]);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(item_empty(q_slot));
-        }
-        const bool upper = MT > 1 && rows > 16;         // the second 16 rows exist
+        for (int kk = 0; kk < kSteps; ++kk) ldmatrix_x4(q_addr + kk * 32, qf[kk]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(item_empty(q_slot));
         const int first_limit = plan.causal ? item.kv - item.tokens : item.kv - 1;
-        int limit[MT][2];                               // last key of rows g and g + 8 of each row tile
+        // Last keys of rows g and g + 8.
+        const int limit0 = plan.causal ? first_limit + (16 * mt + g) / group : first_limit;
+        const int limit1 = plan.causal ? first_limit + (16 * mt + 8 + g) / group : first_limit;
+        float o[kNTiles][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                limit[mt][e] = plan.causal ? first_limit + (16 * mt + 8 * e + g) / group : first_limit;
-        float o[MT][kNTiles][4];
-        float m[MT][2], l[MT][2];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            m[mt][0] = m[mt][1] = -INFINITY;
-            l[mt][0] = l[mt][1] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < kNTiles; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.0f;
-        }
+        for (int j = 0; j < kNTiles; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 
         for (int i = 0; i < item.count; ++i, ++it) {
             const int slot = it % C::kStages;
             if (ok) ok = __all_sync(0xffffffffu, wait_paged(full(slot), (it / C::kStages) & 1, abort_flag, kSiteNarrowFull));
-            const int key0 = (item.tile + i) * kNarrowKeys + warp * 16;
-            if (ok && key0 < item.kv) {
+            const int key0 = (item.tile + i) * kNarrowKeys + kg * kKeys;
+            if (ok && busy && key0 < item.kv) {
                 const uint32_t k_tile = base + slot * C::kStage, v_tile = k_tile + C::kTile;
-                float sc[MT][2][4] = {};
+                float sc[2 * MT][4] = {};
 #pragma unroll
-                for (int kk = 0; kk < kSteps; ++kk) {
-                    uint32_t b[4];
-                    ldmatrix_x4(k_tile + swizzled(k_row, 2 * kk + k_chunk), b);
-                    if constexpr (MT == 1) {
-                        mma_16816(sc[0][0], qf[kk], b[0], b[1]);
-                        mma_16816(sc[0][1], qf[kk], b[2], b[3]);
-                    } else {
+                for (int kk = 0; kk < kSteps; ++kk)
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            if (mt > 0 && !upper) continue;
-                            ldmatrix_x4(q_addr + mt * 16 * C::kQStride + kk * 32, qf[0]);
-                            mma_16816(sc[mt][0], qf[0], b[0], b[1]);
-                            mma_16816(sc[mt][1], qf[0], b[2], b[3]);
+                    for (int s = 0; s < MT; ++s) {
+                        uint32_t b[4];
+                        ldmatrix_x4(k_tile + swizzled(k_row + 16 * s, 2 * kk + k_chunk), b);
+                        mma_16816(sc[2 * s], qf[kk], b[0], b[1]);
+                        mma_16816(sc[2 * s + 1], qf[kk], b[2], b[3]);
+                    }
+                if (key0 + kKeys - 1 > first_limit) {
+#pragma unroll
+                    for (int j = 0; j < 2 * MT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int key = key0 + 8 * j + 2 * t + e;
+                            if (key > limit0) sc[j][e] = -INFINITY;
+                            if (key > limit1) sc[j][2 + e] = -INFINITY;
                         }
+                }
+                float top0 = fmaxf(sc[0][0], sc[0][1]), top1 = fmaxf(sc[0][2], sc[0][3]);
+#pragma unroll
+                for (int j = 1; j < 2 * MT; ++j) {
+                    top0 = fmaxf(top0, fmaxf(sc[j][0], sc[j][1]));
+                    top1 = fmaxf(top1, fmaxf(sc[j][2], sc[j][3]));
+                }
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) {
+                    top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, d));
+                    top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, d));
+                }
+                // The base of a row's exponents moves only when a score exceeds it by a factor 2^16 (a weight
+                // keeps its relative precision in bf16, sums are 32-bit), so O is rarely rescaled.
+                const bool move0 = (top0 - m0) * sl2 > kRebase, move1 = (top1 - m1) * sl2 > kRebase;
+                if (__any_sync(0xffffffffu, move0 || move1)) {
+                    const float keep0 = move0 ? ex2_approx((m0 - top0) * sl2) : 1.0f;
+                    const float keep1 = move1 ? ex2_approx((m1 - top1) * sl2) : 1.0f;
+                    if (move0) m0 = top0;
+                    if (move1) m1 = top1;
+                    l0 *= keep0;
+                    l1 *= keep1;
+#pragma unroll
+                    for (int j = 0; j < kNTiles; ++j) {
+                        o[j][0] *= keep0;
+                        o[j][1] *= keep0;
+                        o[j][2] *= keep1;
+                        o[j][3] *= keep1;
                     }
                 }
+                const float base0 = m0 == -INFINITY ? 0.0f : m0 * sl2, base1 = m1 == -INFINITY ? 0.0f : m1 * sl2;
                 uint32_t pf[MT][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    if (mt > 0 && !upper) continue;
-                    float(&s)[2][4] = sc[mt];
-                    if (key0 + 15 > first_limit) {
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (key0 + 8 * j + 2 * t + (e & 1) > limit[mt][e >> 1]) s[j][e] = -INFINITY;
-                    }
-                    float top[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        top[e] = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
-#pragma unroll
-                        for (int d = 1; d < 4; d <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], d));
-                    }
-                    // The base of a row's exponents moves only when a score exceeds it by a factor 2^16 (a weight
-                    // keeps its relative precision in bf16, sums are 32-bit), so O is rarely rescaled.
-                    const bool move0 = (top[0] - m[mt][0]) * sl2 > kRebase, move1 = (top[1] - m[mt][1]) * sl2 > kRebase;
-                    if (__any_sync(0xffffffffu, move0 || move1)) {
-                        const float keep0 = move0 ? ex2_approx((m[mt][0] - top[0]) * sl2) : 1.0f;
-                        const float keep1 = move1 ? ex2_approx((m[mt][1] - top[1]) * sl2) : 1.0f;
-                        if (move0) m[mt][0] = top[0];
-                        if (move1) m[mt][1] = top[1];
-                        l[mt][0] *= keep0;
-                        l[mt][1] *= keep1;
-#pragma unroll
-                        for (int j = 0; j < kNTiles; ++j) {
-                            o[mt][j][0] *= keep0;
-                            o[mt][j][1] *= keep0;
-                            o[mt][j][2] *= keep1;
-                            o[mt][j][3] *= keep1;
-                        }
-                    }
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float base_e = m[mt][e] == -INFINITY ? 0.0f : m[mt][e] * sl2;
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const float w0 = ex2_approx(fmaf(s[j][2 * e], sl2, -base_e));
-                            const float w1 = ex2_approx(fmaf(s[j][2 * e + 1], sl2, -base_e));
-                            l[mt][e] += w0 + w1;
-                            pf[mt][2 * j + e] = pack_bf16x2(w0, w1);
-                        }
-                    }
+                for (int j = 0; j < 2 * MT; ++j) {
+                    const float a0 = ex2_approx(fmaf(sc[j][0], sl2, -base0)), a1 = ex2_approx(fmaf(sc[j][1], sl2, -base0));
+                    const float b0 = ex2_approx(fmaf(sc[j][2], sl2, -base1)), b1 = ex2_approx(fmaf(sc[j][3], sl2, -base1));
+                    l0 += a0 + a1;
+                    l1 += b0 + b1;
+                    pf[j / 2][2 * (j % 2)] = pack_bf16x2(a0, a1);
+                    pf[j / 2][2 * (j % 2) + 1] = pack_bf16x2(b0, b1);
                 }
                 // V rows behind the last key may hold anything: they are zeroed in the fragments (fragment
-                // register 0 holds keys 2t and 2t + 1 of the 16, register 1 the same plus 8).
-                uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-                const bool tail = key0 + 15 >= item.kv;
-                if (tail) {
-                    const int k0 = key0 + 2 * t;
-                    keep0 = (k0 < item.kv ? 0xffffu : 0u) | (k0 + 1 < item.kv ? 0xffff0000u : 0u);
-                    keep1 = (k0 + 8 < item.kv ? 0xffffu : 0u) | (k0 + 9 < item.kv ? 0xffff0000u : 0u);
-                }
+                // register 0 holds keys 2t and 2t + 1 of 16, register 1 the same plus 8).
+                const bool tail = key0 + kKeys > item.kv;
 #pragma unroll
-                for (int dd = 0; dd < kSteps; ++dd) {
-                    uint32_t b[4];
-                    ldmatrix_x4_trans(v_tile + swizzled(v_row, 2 * dd + v_chunk), b);
+                for (int s = 0; s < MT; ++s) {
+                    uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
                     if (tail) {
-                        b[0] &= keep0;
-                        b[1] &= keep1;
-                        b[2] &= keep0;
-                        b[3] &= keep1;
+                        const int k0 = key0 + 16 * s + 2 * t;
+                        keep0 = (k0 < item.kv ? 0xffffu : 0u) | (k0 + 1 < item.kv ? 0xffff0000u : 0u);
+                        keep1 = (k0 + 8 < item.kv ? 0xffffu : 0u) | (k0 + 9 < item.kv ? 0xffff0000u : 0u);
                     }
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        if (mt > 0 && !upper) continue;
-                        mma_16816(o[mt][2 * dd], pf[mt], b[0], b[1]);
-                        mma_16816(o[mt][2 * dd + 1], pf[mt], b[2], b[3]);
+                    for (int dd = 0; dd < kSteps; ++dd) {
+                        uint32_t b[4];
+                        ldmatrix_x4_trans(v_tile + swizzled(v_row + 16 * s, 2 * dd + v_chunk), b);
+                        if (tail) {
+                            b[0] &= keep0;
+                            b[1] &= keep1;
+                            b[2] &= keep0;
+                            b[3] &= keep1;
+                        }
+                        mma_16816(o[2 * dd], pf[s], b[0], b[1]);
+                        mma_16816(o[2 * dd + 1], pf[s], b[2], b[3]);
                     }
                 }
             }
@@ -444,88 +430,81 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 if (lane == 0) mbar_arrive(empty(slot));
             }
         }
-        if constexpr (MT > 1) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(item_empty(q_slot));
-        }
 
-        // ---- the four warps' results become one, in the slot of the last tile ----
+        // ---- the key groups' results become one, in the slot of the last tile ----
         const int last_slot = (it - 1) % C::kStages;
         float* merge = reinterpret_cast<float*>(smem + last_slot * C::kStage);
-        // [warp][row][column], the columns of a row exchanged in groups of 8 so that the rows of a half warp
-        // fall on different banks.
-        auto merge_at = [&](int w, int row, int column) -> float2* {
-            return reinterpret_cast<float2*>(merge + (w * 16 + row) * D + (column ^ ((row & 3) * 8)));
+        // [key group][row][column], the columns of a row exchanged in groups of 8 so that the rows of a half
+        // warp fall on different banks.
+        auto merge_at = [&](int which, int row, int column) -> float2* {
+            return reinterpret_cast<float2*>(merge + (which * 16 * MT + row) * D + (column ^ ((row & 3) * 8)));
         };
-        float mine[MT][2];
+        float* row_stats = stats + 16 * mt + g;         // [key group][row]: maxima, then sums
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                for (int d = 1; d < 4; d <<= 1) l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], d);
-                if (t == 0) {
-                    stats[(warp * MT + mt) * 16 + 8 * e + g] = m[mt][e];
-                    stats[C::kStats + (warp * MT + mt) * 16 + 8 * e + g] = l[mt][e];
-                }
-            }
+        for (int d = 1; d < 4; d <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+        }
+        if (t == 0) {
+            row_stats[kg * 16 * MT] = m0;
+            row_stats[kg * 16 * MT + 8] = m1;
+            row_stats[C::kStats + kg * 16 * MT] = l0;
+            row_stats[C::kStats + kg * 16 * MT + 8] = l1;
+        }
         named_barrier(1, kNarrowWarps * 32);        // all warps are done with the slot's tile
+        // Weight of key group `which` of a row, whose largest maximum is `all`.
+        auto weight = [&](const float* at, int which, float all) {
+            const float mw = at[which * 16 * MT];
+            return mw == -INFINITY ? 0.0f : ex2_approx((mw - all) * sl2);
+        };
+        auto largest = [&](const float* at) {
+            float all = at[0];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            if (mt > 0 && !upper) continue;
-            float all[2], sum[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float* at = stats + mt * 16 + 8 * e + g;
-                all[e] = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kNarrowWarps; ++w) all[e] = fmaxf(all[e], at[w * MT * 16]);
-                sum[e] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kNarrowWarps; ++w) {
-                    const float mw = at[w * MT * 16];
-                    const float weight = mw == -INFINITY ? 0.0f : ex2_approx((mw - all[e]) * sl2);
-                    sum[e] += weight * at[C::kStats + w * MT * 16];
-                    if (w == warp) mine[mt][e] = weight;
-                }
-            }
+            for (int w = 1; w < kGroups; ++w) all = fmaxf(all, at[w * 16 * MT]);
+            return all;
+        };
+        if (busy) {
+            const float w0 = weight(row_stats, kg, largest(row_stats)), w1 = weight(row_stats + 8, kg, largest(row_stats + 8));
 #pragma unroll
             for (int j = 0; j < kNTiles; ++j) {
-                const float(&v)[4] = o[mt][j];
-                *merge_at(warp, g, 8 * j + 2 * t) = make_float2(v[0] * mine[mt][0], v[1] * mine[mt][0]);
+                *merge_at(kg, 16 * mt + g, 8 * j + 2 * t) = make_float2(o[j][0] * w0, o[j][1] * w0);
                 if (rows > 16 * mt + 8)
-                    *merge_at(warp, g + 8, 8 * j + 2 * t) = make_float2(v[2] * mine[mt][1], v[3] * mine[mt][1]);
+                    *merge_at(kg, 16 * mt + g + 8, 8 * j + 2 * t) = make_float2(o[j][2] * w1, o[j][3] * w1);
             }
-            named_barrier(1, kNarrowWarps * 32);
-            // Warp w adds up and writes columns [w * D / 4, (w + 1) * D / 4).
-            float* part = p.partial + static_cast<long long>(item.part) * C::kPartFloats;
+        }
+        named_barrier(1, kNarrowWarps * 32);
+        // Warp w adds up and writes columns [w * D / 4, (w + 1) * D / 4) of every row.
+        float* part = p.partial + static_cast<long long>(item.part) * C::kPartFloats;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int row = 16 * mt + 8 * e + g;
-                if (!ok || row >= rows) continue;
-                const int tok = row / group;
-                __nv_bfloat16* out = p.o + static_cast<long long>(item.token0 + tok) * p.o_token +
-                                     static_cast<long long>(item.head0 + row - tok * group) * p.o_head;
-                const float inv = 1.0f / sum[e];
+        for (int e = 0; e < 2 * MT; ++e) {
+            const int row = 8 * e + g;
+            if (!ok || row >= rows) continue;
+            const float* at = stats + row;
+            const float all = largest(at);
+            float sum = 0.0f;
 #pragma unroll
-                for (int j = 0; j < kNTiles / 4; ++j) {
-                    const int column = warp * (D / 4) + 8 * j + 2 * t;
-                    float2 a = make_float2(0.0f, 0.0f);
+            for (int w = 0; w < kGroups; ++w) sum += weight(at, w, all) * at[C::kStats + w * 16 * MT];
+            const int tok = row / group;
+            __nv_bfloat16* out = p.o + static_cast<long long>(item.token0 + tok) * p.o_token +
+                                 static_cast<long long>(item.head0 + row - tok * group) * p.o_head;
+            const float inv = 1.0f / sum;
 #pragma unroll
-                    for (int w = 0; w < kNarrowWarps; ++w) {
-                        const float2 v = *merge_at(w, 8 * e + g, column);
-                        a.x += v.x;
-                        a.y += v.y;
-                    }
-                    if (item.part < 0) *reinterpret_cast<uint32_t*>(out + column) = pack_bf16x2(a.x * inv, a.y * inv);
-                    else *reinterpret_cast<float2*>(part + row * D + column) = a;
+            for (int j = 0; j < kNTiles / 4; ++j) {
+                const int column = warp * (D / 4) + 8 * j + 2 * t;
+                float2 a = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < kGroups; ++w) {
+                    const float2 v = *merge_at(w, row, column);
+                    a.x += v.x;
+                    a.y += v.y;
                 }
-                if (item.part >= 0 && warp == 0 && t == 0) {
-                    part[16 * MT * D + row] = all[e];
-                    part[16 * MT * D + 16 * MT + row] = sum[e];
-                }
+                if (item.part < 0) *reinterpret_cast<uint32_t*>(out + column) = pack_bf16x2(a.x * inv, a.y * inv);
+                else *reinterpret_cast<float2*>(part + row * D + column) = a;
             }
-            if (mt + 1 < MT && upper) named_barrier(1, kNarrowWarps * 32);
+            if (item.part >= 0 && warp == 0 && t == 0) {
+                part[16 * MT * D + row] = all;
+                part[16 * MT * D + 16 * MT + row] = sum;
+            }
         }
         // The slot goes back to the copies: what was read and written here comes before them.
         fence_proxy_async_smem();
