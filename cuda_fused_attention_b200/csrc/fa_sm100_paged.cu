@@ -707,26 +707,26 @@ __device__ __forceinline__ long long wide_share(long long total, int ctas)
     return even > kWideMinTiles ? even : kWideMinTiles;
 }
 
+// The products of one Q tile with one K or V tile. Descriptors are those of the tiles' first elements;
+// a step along K adds to their address field (bytes / 16), which holds any shared address.
 template <int D>
-__device__ __forceinline__ void wide_issue_qk(uint32_t d_tmem, uint32_t q_saddr, uint32_t k_saddr)
+__device__ __forceinline__ void wide_issue_qk(uint32_t d_tmem, uint64_t q_desc, uint64_t k_desc)
 {
     using C = WideCfg<D>;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t off = static_cast<uint32_t>((kk >> 2) * C::kSubBytes + (kk & 3) * 32);
-        umma_ss(d_tmem, make_smem_desc(q_saddr + off, 16, 1024), make_smem_desc(k_saddr + off, 16, 1024), C::kIdescQK,
-                kk > 0 ? 1u : 0u);
+        const uint64_t off = static_cast<uint64_t>(((kk >> 2) * C::kSubBytes + (kk & 3) * 32) >> 4);
+        umma_ss(d_tmem, q_desc + off, k_desc + off, C::kIdescQK, kk > 0 ? 1u : 0u);
     }
 }
 
 template <int D, int kFirst, int kLast>
-__device__ __forceinline__ void wide_issue_pv(uint32_t d_tmem, uint32_t p_tmem, uint32_t v_saddr, bool accumulate)
+__device__ __forceinline__ void wide_issue_pv(uint32_t d_tmem, uint32_t p_tmem, uint64_t v_desc, bool accumulate)
 {
     using C = WideCfg<D>;
 #pragma unroll
     for (int kk = kFirst; kk < kLast; ++kk)
-        umma_ts(d_tmem, p_tmem + static_cast<uint32_t>(kk * 8),
-                make_smem_desc(v_saddr + static_cast<uint32_t>(kk * 16 * 128), C::kSubBytes, 1024), C::kIdescPV,
+        umma_ts(d_tmem, p_tmem + static_cast<uint32_t>(kk * 8), v_desc + static_cast<uint64_t>((kk * 16 * 128) >> 4), C::kIdescPV,
                 (accumulate || kk > 0) ? 1u : 0u);
 }
 
@@ -779,14 +779,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int group = plan.heads / plan.kv_heads;
     const int per_tile = tokens_per_tile(group);
 
-    // Takes segment number sg: every lane of a reading warp gets the values. False: gave up.
-    auto take_segment = [&](int sg, WideSegment& s) -> bool {
-        if (!__all_sync(0xffffffffu, wait_paged(bar(C::kBarSchedFull + (sg & 1)), (sg >> 1) & 1, abort_flag, kSiteWideSched)))
-            return false;
-        s = segments[sg & 1];
+    // Waits for segment number sg; false: gave up. Once its fields are read, release_segment.
+    auto await_segment = [&](int sg) -> bool {
+        return __all_sync(0xffffffffu, wait_paged(bar(C::kBarSchedFull + (sg & 1)), (sg >> 1) & 1, abort_flag, kSiteWideSched));
+    };
+    auto release_segment = [&](int sg) {
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::kBarSchedEmpty + (sg & 1)));
-        return true;
     };
 
     if (warp >= kMma) {
@@ -802,25 +801,29 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             int q_loads = 0;
             uint32_t tail_slots = 0, tail_parity = 0;      // slots whose latest load went by the tail warp; their phases
             bool ok = true;
-            WideSegment s;
             for (int sg = 0; ok; ++sg) {
-                ok = take_segment(sg, s);
-                if (!ok || s.count == 0) break;
+                ok = await_segment(sg);
+                if (!ok) break;
+                const WideSegment& seg = segments[sg & 1];
+                const int count = seg.count, first_tile = seg.tile, head = seg.h, token0 = seg.token0;
+                const int tiles = seg.tokens > per_tile ? 2 : 1;
+                const bool has_tail = seg.zero_to > seg.zero_from;
+                const int held = (seg.kv + plan.page_size - 1) >> p.page_shift;
+                const int* table = plan.block_table + static_cast<long long>(seg.b) * plan.table_stride;
+                release_segment(sg);
+                if (count == 0) break;
                 if (sg > 0 && !__all_sync(0xffffffffu, wait_paged(bar(C::kBarQEmpty), (sg - 1) & 1, abort_flag, kSiteWideQ))) {
                     ok = false;
                     break;
                 }
-                const int tiles = s.tokens > per_tile ? 2 : 1;
                 if (lane == 0) {
                     mbar_arrive_expect_tx(bar(C::kBarQFull), static_cast<uint32_t>(tiles * C::kSub * 128 * group * per_tile));
                     for (int t = 0; t < tiles; ++t)
                         for (int sub = 0; sub < C::kSub; ++sub)
                             tma_load_3d(base + t * C::kTileBytes + sub * C::kSubBytes, &tm_q, bar(C::kBarQFull), sub * 64,
-                                        s.h * group, s.token0 + t * per_tile);
+                                        head * group, token0 + t * per_tile);
                 }
                 ++q_loads;
-                const int* table = plan.block_table + static_cast<long long>(s.b) * plan.table_stride;
-                const int held = (s.kv + plan.page_size - 1) >> p.page_shift;
                 auto page_at = [&](int tile) -> int {
                     // num_pages is out of the map's range: such a box reads as zeros.
                     const int i = ((tile * kWideKeys) >> p.page_shift) + page_of_tile;
@@ -830,9 +833,9 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     atomicOr(&g_paged_error_word, FA_ERROR_BAD_PAGE);
                     return plan.num_pages;
                 };
-                int page = page_at(s.tile);
-                for (int i = 0; ok && i < s.count; ++i) {
-                    const int row = pages > 1 ? 0 : ((s.tile + i) * kWideKeys) & (plan.page_size - 1);
+                int page = page_at(first_tile);
+                for (int i = 0; ok && i < count; ++i) {
+                    const int row = pages > 1 ? 0 : ((first_tile + i) * kWideKeys) & (plan.page_size - 1);
                     for (int kv = 0; kv < 2; ++kv, ++ri) {
                         const int slot = ri % C::kStages, use = ri / C::kStages;
                         if (use > 0 && !__all_sync(0xffffffffu, wait_paged(bar(C::kBarKvEmpty + slot), (use - 1) & 1,
@@ -842,7 +845,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                         }
                         // A V tile to be zeroed in part lands on the tail warp's barrier, and that warp then
                         // completes the slot's.
-                        const bool tail = kv == 1 && i + 1 == s.count && s.zero_to > s.zero_from;
+                        const bool tail = kv == 1 && i + 1 == count && has_tail;
                         const uint32_t landed = bar((tail ? C::kBarTail : C::kBarKvFull) + slot);
                         tail_slots = tail ? tail_slots | (1u << slot) : tail_slots & ~(1u << slot);
                         if (tail) tail_parity ^= 1u << slot;
@@ -850,9 +853,9 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                         __syncwarp();
                         if (active)
                             tma_load_4d(ring + slot * C::kTileBytes + offset, kv ? &tm_v : &tm_k, landed, block * 64, row,
-                                        s.h, page);
+                                        head, page);
                     }
-                    if (ok && i + 1 < s.count) page = page_at(s.tile + i + 1);
+                    if (ok && i + 1 < count) page = page_at(first_tile + i + 1);
                 }
             }
             if (!ok && lane == 0) {
@@ -865,14 +868,16 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
         } else if (warp == kMma) {
             // ======================= MMA issuer ================================
+            // Anything but MMAs that this thread does waits until the MMAs it has queued are done, so all it
+            // needs is in registers before a segment's loop.
             const uint32_t t_s0 = tmem_base + C::kColS0, t_s1 = tmem_base + C::kColS1;
             const uint32_t t_o0 = tmem_base + C::kColO0, t_o1 = tmem_base + C::kColO1;
-            const uint32_t sq0 = base, sq1 = base + C::kTileBytes;
-            auto slot_addr = [&](int i) -> uint32_t { return ring + (i % C::kStages) * C::kTileBytes; };
+            const uint64_t q0 = make_smem_desc(base, 16, 1024), q1 = make_smem_desc(base + C::kTileBytes, 16, 1024);
+            const uint64_t k_ring = make_smem_desc(ring, 16, 1024), v_ring = make_smem_desc(ring, C::kSubBytes, 1024);
+            auto in_slot = [](uint64_t desc, int i) { return desc + static_cast<uint64_t>(i % C::kStages) * (C::kTileBytes >> 4); };
             auto empty_bar = [&](int i) -> uint32_t { return bar(C::kBarKvEmpty + i % C::kStages); };
             int ri = 0, c0 = 0, c1 = 0;
             bool ok = true;
-            WideSegment s;
             auto wait = [&](int index, uint32_t parity, uint32_t site) {
                 return wait_paged(bar(index), parity & 1u, abort_flag, site);
             };
@@ -880,63 +885,66 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 return wait_paged(bar(C::kBarKvFull + i % C::kStages), (i / C::kStages) & 1, abort_flag, site);
             };
             for (int sg = 0; ok; ++sg) {
-                ok = take_segment(sg, s);
-                if (!ok || s.count == 0) break;
+                ok = await_segment(sg);
+                if (!ok) break;
+                const int count = segments[sg & 1].count;
+                const bool two = segments[sg & 1].tokens > per_tile;
+                release_segment(sg);
+                if (count == 0) break;
                 if (lane == 0) {
-                    const bool two = s.tokens > per_tile;
                     ok = wait(C::kBarQFull, sg, kSiteWideQ) && wait_ring(ri, kSiteWideK);
                     if (ok) {
                         tc_fence_after();
-                        wide_issue_qk<D>(t_s0, sq0, slot_addr(ri));
+                        wide_issue_qk<D>(t_s0, q0, in_slot(k_ring, ri));
                         umma_commit(bar(C::kBarSFull + 0));
                         if (two) {
-                            wide_issue_qk<D>(t_s1, sq1, slot_addr(ri));
+                            wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ri));
                             umma_commit(bar(C::kBarSFull + 1));
                         }
                         umma_commit(empty_bar(ri));
-                        if (s.count == 1) umma_commit(bar(C::kBarQEmpty));
+                        if (count == 1) umma_commit(bar(C::kBarQEmpty));
                     }
-                    for (int j = 0; ok && j < s.count; ++j) {
-                        const int vi = ri + 2 * j + 1, ki = vi + 1;
-                        const bool more = j + 1 < s.count;
+                    for (int j = 0; ok && j < count; ++j) {
+                        const int vi = ri + 1, ki = ri + 2;
+                        const bool more = j + 1 < count;
                         if (!wait_ring(vi, kSiteWideV)) { ok = false; break; }
-                        if (!wait(C::kBarPHalf + 0, c0 + j, kSiteWideP)) { ok = false; break; }
+                        if (!wait(C::kBarPHalf + 0, c0, kSiteWideP)) { ok = false; break; }
                         tc_fence_after();
-                        wide_issue_pv<D, 0, 4>(t_o0, t_s0, slot_addr(vi), j > 0);
+                        wide_issue_pv<D, 0, 4>(t_o0, t_s0, in_slot(v_ring, vi), j > 0);
                         umma_commit(bar(C::kBarPvHalf + 0));
-                        if (!wait(C::kBarPFull + 0, c0 + j, kSiteWideP)) { ok = false; break; }
+                        if (!wait(C::kBarPFull + 0, c0, kSiteWideP)) { ok = false; break; }
                         tc_fence_after();
-                        wide_issue_pv<D, 4, 8>(t_o0, t_s0, slot_addr(vi), true);
+                        wide_issue_pv<D, 4, 8>(t_o0, t_s0, in_slot(v_ring, vi), true);
                         if (!more) umma_commit(bar(C::kBarOFull + 0));
                         if (more) {
                             if (!wait_ring(ki, kSiteWideK)) { ok = false; break; }
                             tc_fence_after();
-                            wide_issue_qk<D>(t_s0, sq0, slot_addr(ki));
+                            wide_issue_qk<D>(t_s0, q0, in_slot(k_ring, ki));
                             umma_commit(bar(C::kBarSFull + 0));
                         }
                         if (two) {
-                            if (!wait(C::kBarPHalf + 1, c1 + j, kSiteWideP)) { ok = false; break; }
+                            if (!wait(C::kBarPHalf + 1, c1, kSiteWideP)) { ok = false; break; }
                             tc_fence_after();
-                            wide_issue_pv<D, 0, 4>(t_o1, t_s1, slot_addr(vi), j > 0);
+                            wide_issue_pv<D, 0, 4>(t_o1, t_s1, in_slot(v_ring, vi), j > 0);
                             umma_commit(bar(C::kBarPvHalf + 1));
-                            if (!wait(C::kBarPFull + 1, c1 + j, kSiteWideP)) { ok = false; break; }
+                            if (!wait(C::kBarPFull + 1, c1, kSiteWideP)) { ok = false; break; }
                             tc_fence_after();
-                            wide_issue_pv<D, 4, 8>(t_o1, t_s1, slot_addr(vi), true);
+                            wide_issue_pv<D, 4, 8>(t_o1, t_s1, in_slot(v_ring, vi), true);
                             if (!more) umma_commit(bar(C::kBarOFull + 1));
+                            ++c1;
                         }
                         umma_commit(empty_bar(vi));
                         if (more) {
                             if (two) {
-                                wide_issue_qk<D>(t_s1, sq1, slot_addr(ki));
+                                wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ki));
                                 umma_commit(bar(C::kBarSFull + 1));
                             }
                             umma_commit(empty_bar(ki));
-                            if (j + 2 == s.count) umma_commit(bar(C::kBarQEmpty));
+                            if (j + 2 == count) umma_commit(bar(C::kBarQEmpty));
                         }
+                        ++c0;
+                        ri += 2;
                     }
-                    ri += 2 * s.count;
-                    c0 += s.count;
-                    if (two) c1 += s.count;
                 }
                 ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
             }
@@ -950,23 +958,24 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             // ======================= zeroes behind the last key ================
             int ri = 0;
             uint32_t parity = 0;
-            WideSegment s;
-            for (int sg = 0; take_segment(sg, s) && s.count > 0; ++sg) {
-                if (s.zero_to > s.zero_from) {
-                    const int vi = ri + 2 * s.count - 1, slot = vi % C::kStages;
-                    if (!__all_sync(0xffffffffu, wait_paged(bar(C::kBarTail + slot), parity >> slot & 1u, abort_flag, kSiteWideTail)))
-                        break;
-                    parity ^= 1u << slot;
-                    const int bytes = (s.zero_to - s.zero_from) * 128;
-                    for (int sub = 0; sub < C::kSub; ++sub) {
-                        uint8_t* at = smem + C::kRingOff + slot * C::kTileBytes + sub * C::kSubBytes + s.zero_from * 128;
-                        for (int i = lane * 16; i < bytes; i += 512) *reinterpret_cast<uint4*>(at + i) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(C::kBarKvFull + slot));
+            for (int sg = 0; await_segment(sg); ++sg) {
+                const int count = segments[sg & 1].count, from = segments[sg & 1].zero_from, to = segments[sg & 1].zero_to;
+                release_segment(sg);
+                if (count == 0) break;
+                ri += 2 * count;
+                if (from >= to) continue;
+                const int slot = (ri - 1) % C::kStages;
+                if (!__all_sync(0xffffffffu, wait_paged(bar(C::kBarTail + slot), parity >> slot & 1u, abort_flag, kSiteWideTail)))
+                    break;
+                parity ^= 1u << slot;
+                const int bytes = (to - from) * 128;
+                for (int sub = 0; sub < C::kSub; ++sub) {
+                    uint8_t* at = smem + C::kRingOff + slot * C::kTileBytes + sub * C::kSubBytes + from * 128;
+                    for (int i = lane * 16; i < bytes; i += 512) *reinterpret_cast<uint4*>(at + i) = make_uint4(0, 0, 0, 0);
                 }
-                ri += 2 * s.count;
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(C::kBarKvFull + slot));
             }
         } else if (lane == 0) {
             // ======================= the walk along the line ===================
@@ -1060,14 +1069,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         bool ok = true;
         for (int sg = 0; ok; ++sg) {
             // The slot stays this segment's until the epilogue has read it.
-            ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarSchedFull + (sg & 1)), (sg >> 1) & 1, abort_flag, kSiteWideSched));
+            ok = await_segment(sg);
             if (!ok) break;
             const WideSegment& seg = segments[sg & 1];
             const int count = seg.count;
             if (count == 0) break;
             if (t == 1 && seg.tokens <= per_tile) {     // this block has one tile
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(C::kBarSchedEmpty + (sg & 1)));
+                release_segment(sg);
                 continue;
             }
             const int tile = seg.tile;
@@ -1160,8 +1168,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             const bool real = in_tile && tok < seg.tokens;
             __nv_bfloat16* out = p.o + static_cast<long long>(seg.token0 + tok) * p.o_token +
                                  static_cast<long long>(seg.h * group + r % group) * p.o_head;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(C::kBarSchedEmpty + (sg & 1)));
+            release_segment(sg);
             if (part < 0) {
                 const float inv = 1.0f / row_sum;
 #pragma unroll
