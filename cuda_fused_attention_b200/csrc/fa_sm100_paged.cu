@@ -8,6 +8,7 @@
 #include <cmath>
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "fa_sm100_internal.h"
 #include "fa_sm100_paged.cuh"
@@ -707,27 +708,35 @@ __device__ __forceinline__ long long wide_share(long long total, int ctas)
     return even > kWideMinTiles ? even : kWideMinTiles;
 }
 
-// The products of one Q tile with one K or V tile. Descriptors are those of the tiles' first elements;
-// a step along K adds to their address field (bytes / 16), which holds any shared address.
+// A matrix descriptor (fa_sm100_ptx.cuh) as its low word -- address and leading offset, which a step along
+// K adds to -- and its high word, the same for all tiles: only one register changes between MMAs.
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lbo_bytes) { return (saddr >> 4) | (lbo_bytes >> 4) << 16; }
+__device__ __forceinline__ uint64_t desc_of(uint32_t low)
+{
+    constexpr uint32_t kHigh = (1024u >> 4) | 1u << 14 | 2u << 29;     // 8-row groups 1024 bytes apart, version 1, 128-byte swizzle
+    return static_cast<uint64_t>(kHigh) << 32 | low;
+}
+
+// The products of one Q tile with one K or V tile, from the low words of the tiles' descriptors.
 template <int D>
-__device__ __forceinline__ void wide_issue_qk(uint32_t d_tmem, uint64_t q_desc, uint64_t k_desc)
+__device__ __forceinline__ void wide_issue_qk(uint32_t d_tmem, uint32_t q_low, uint32_t k_low)
 {
     using C = WideCfg<D>;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
-        const uint64_t off = static_cast<uint64_t>(((kk >> 2) * C::kSubBytes + (kk & 3) * 32) >> 4);
-        umma_ss(d_tmem, q_desc + off, k_desc + off, C::kIdescQK, kk > 0 ? 1u : 0u);
+        const uint32_t off = static_cast<uint32_t>(((kk >> 2) * C::kSubBytes + (kk & 3) * 32) >> 4);
+        umma_ss(d_tmem, desc_of(q_low + off), desc_of(k_low + off), C::kIdescQK, kk > 0 ? 1u : 0u);
     }
 }
 
 template <int D, int kFirst, int kLast>
-__device__ __forceinline__ void wide_issue_pv(uint32_t d_tmem, uint32_t p_tmem, uint64_t v_desc, bool accumulate)
+__device__ __forceinline__ void wide_issue_pv(uint32_t d_tmem, uint32_t p_tmem, uint32_t v_low, bool accumulate)
 {
     using C = WideCfg<D>;
 #pragma unroll
     for (int kk = kFirst; kk < kLast; ++kk)
-        umma_ts(d_tmem, p_tmem + static_cast<uint32_t>(kk * 8), v_desc + static_cast<uint64_t>((kk * 16 * 128) >> 4), C::kIdescPV,
-                (accumulate || kk > 0) ? 1u : 0u);
+        umma_ts(d_tmem, p_tmem + static_cast<uint32_t>(kk * 8), desc_of(v_low + static_cast<uint32_t>((kk * 16 * 128) >> 4)),
+                C::kIdescPV, (accumulate || kk > 0) ? 1u : 0u);
 }
 
 template <int D>
@@ -872,17 +881,67 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             // needs is in registers before a segment's loop.
             const uint32_t t_s0 = tmem_base + C::kColS0, t_s1 = tmem_base + C::kColS1;
             const uint32_t t_o0 = tmem_base + C::kColO0, t_o1 = tmem_base + C::kColO1;
-            const uint64_t q0 = make_smem_desc(base, 16, 1024), q1 = make_smem_desc(base + C::kTileBytes, 16, 1024);
-            const uint64_t k_ring = make_smem_desc(ring, 16, 1024), v_ring = make_smem_desc(ring, C::kSubBytes, 1024);
-            auto in_slot = [](uint64_t desc, int i) { return desc + static_cast<uint64_t>(i % C::kStages) * (C::kTileBytes >> 4); };
+            const uint32_t q0 = desc_low(base, 16), q1 = desc_low(base + C::kTileBytes, 16);
+            const uint32_t k_ring = desc_low(ring, 16), v_ring = desc_low(ring, C::kSubBytes);
+            auto in_slot = [](uint32_t low, int i) { return low + static_cast<uint32_t>(i % C::kStages) * (C::kTileBytes >> 4); };
             auto empty_bar = [&](int i) -> uint32_t { return bar(C::kBarKvEmpty + i % C::kStages); };
-            int ri = 0, c0 = 0, c1 = 0;
+            int ri = 0;                         // ring index of the segment's first K tile
+            uint32_t par0 = 0, par1 = 0;        // parity of each Q tile's per-key-tile barriers
             bool ok = true;
-            auto wait = [&](int index, uint32_t parity, uint32_t site) {
-                return wait_paged(bar(index), parity & 1u, abort_flag, site);
-            };
+            auto wait = [&](int index, uint32_t parity, uint32_t site) { return wait_paged(bar(index), parity, abort_flag, site); };
             auto wait_ring = [&](int i, uint32_t site) {
                 return wait_paged(bar(C::kBarKvFull + i % C::kStages), (i / C::kStages) & 1, abort_flag, site);
+            };
+            // A segment's products; two Q tiles or one (separate code: the issuing thread's own instructions count).
+            auto issue_segment = [&](auto both, int count) -> bool {
+                constexpr bool two = decltype(both)::value;
+                wide_issue_qk<D>(t_s0, q0, in_slot(k_ring, ri));
+                umma_commit(bar(C::kBarSFull + 0));
+                if constexpr (two) {
+                    wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ri));
+                    umma_commit(bar(C::kBarSFull + 1));
+                }
+                umma_commit(empty_bar(ri));
+                for (int j = 0; j < count; ++j) {
+                    const int vi = ri + 2 * j + 1, ki = vi + 1;
+                    const bool more = j + 1 < count;
+                    if (!wait_ring(vi, kSiteWideV)) return false;
+                    if (!wait(C::kBarPHalf + 0, par0, kSiteWideP)) return false;
+                    tc_fence_after();
+                    wide_issue_pv<D, 0, 4>(t_o0, t_s0, in_slot(v_ring, vi), j > 0);
+                    umma_commit(bar(C::kBarPvHalf + 0));
+                    if (!wait(C::kBarPFull + 0, par0, kSiteWideP)) return false;
+                    tc_fence_after();
+                    wide_issue_pv<D, 4, 8>(t_o0, t_s0, in_slot(v_ring, vi), true);
+                    par0 ^= 1u;
+                    if (!more) umma_commit(bar(C::kBarOFull + 0));
+                    if (more) {
+                        if (!wait_ring(ki, kSiteWideK)) return false;
+                        tc_fence_after();
+                        wide_issue_qk<D>(t_s0, q0, in_slot(k_ring, ki));
+                        umma_commit(bar(C::kBarSFull + 0));
+                    }
+                    if constexpr (two) {
+                        if (!wait(C::kBarPHalf + 1, par1, kSiteWideP)) return false;
+                        tc_fence_after();
+                        wide_issue_pv<D, 0, 4>(t_o1, t_s1, in_slot(v_ring, vi), j > 0);
+                        umma_commit(bar(C::kBarPvHalf + 1));
+                        if (!wait(C::kBarPFull + 1, par1, kSiteWideP)) return false;
+                        tc_fence_after();
+                        wide_issue_pv<D, 4, 8>(t_o1, t_s1, in_slot(v_ring, vi), true);
+                        par1 ^= 1u;
+                        umma_commit(empty_bar(vi));
+                        if (!more) umma_commit(bar(C::kBarOFull + 1));
+                        if (more) {
+                            wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ki));
+                            umma_commit(bar(C::kBarSFull + 1));
+                        }
+                    } else {
+                        umma_commit(empty_bar(vi));
+                    }
+                    if (more) umma_commit(empty_bar(ki));
+                }
+                return true;
             };
             for (int sg = 0; ok; ++sg) {
                 ok = await_segment(sg);
@@ -892,58 +951,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 release_segment(sg);
                 if (count == 0) break;
                 if (lane == 0) {
-                    ok = wait(C::kBarQFull, sg, kSiteWideQ) && wait_ring(ri, kSiteWideK);
+                    ok = wait(C::kBarQFull, sg & 1, kSiteWideQ) && wait_ring(ri, kSiteWideK);
                     if (ok) {
                         tc_fence_after();
-                        wide_issue_qk<D>(t_s0, q0, in_slot(k_ring, ri));
-                        umma_commit(bar(C::kBarSFull + 0));
-                        if (two) {
-                            wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ri));
-                            umma_commit(bar(C::kBarSFull + 1));
-                        }
-                        umma_commit(empty_bar(ri));
-                        if (count == 1) umma_commit(bar(C::kBarQEmpty));
-                    }
-                    for (int j = 0; ok && j < count; ++j) {
-                        const int vi = ri + 1, ki = ri + 2;
-                        const bool more = j + 1 < count;
-                        if (!wait_ring(vi, kSiteWideV)) { ok = false; break; }
-                        if (!wait(C::kBarPHalf + 0, c0, kSiteWideP)) { ok = false; break; }
-                        tc_fence_after();
-                        wide_issue_pv<D, 0, 4>(t_o0, t_s0, in_slot(v_ring, vi), j > 0);
-                        umma_commit(bar(C::kBarPvHalf + 0));
-                        if (!wait(C::kBarPFull + 0, c0, kSiteWideP)) { ok = false; break; }
-                        tc_fence_after();
-                        wide_issue_pv<D, 4, 8>(t_o0, t_s0, in_slot(v_ring, vi), true);
-                        if (!more) umma_commit(bar(C::kBarOFull + 0));
-                        if (more) {
-                            if (!wait_ring(ki, kSiteWideK)) { ok = false; break; }
-                            tc_fence_after();
-                            wide_issue_qk<D>(t_s0, q0, in_slot(k_ring, ki));
-                            umma_commit(bar(C::kBarSFull + 0));
-                        }
-                        if (two) {
-                            if (!wait(C::kBarPHalf + 1, c1, kSiteWideP)) { ok = false; break; }
-                            tc_fence_after();
-                            wide_issue_pv<D, 0, 4>(t_o1, t_s1, in_slot(v_ring, vi), j > 0);
-                            umma_commit(bar(C::kBarPvHalf + 1));
-                            if (!wait(C::kBarPFull + 1, c1, kSiteWideP)) { ok = false; break; }
-                            tc_fence_after();
-                            wide_issue_pv<D, 4, 8>(t_o1, t_s1, in_slot(v_ring, vi), true);
-                            if (!more) umma_commit(bar(C::kBarOFull + 1));
-                            ++c1;
-                        }
-                        umma_commit(empty_bar(vi));
-                        if (more) {
-                            if (two) {
-                                wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ki));
-                                umma_commit(bar(C::kBarSFull + 1));
-                            }
-                            umma_commit(empty_bar(ki));
-                            if (j + 2 == count) umma_commit(bar(C::kBarQEmpty));
-                        }
-                        ++c0;
-                        ri += 2;
+                        ok = two ? issue_segment(std::true_type{}, count) : issue_segment(std::false_type{}, count);
+                        // Q is free once the segment's last S is done, a little earlier than this.
+                        if (ok) umma_commit(bar(C::kBarQEmpty));
+                        ri += 2 * count;
                     }
                 }
                 ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
