@@ -611,7 +611,7 @@ combine_narrow_kernel(const __grid_constant__ PagedParams p, int ctas)
 // those of the dense kernel (fa_sm100.cu). P is rounded to bf16 for the product with V.
 constexpr int kWideThreads = 384;
 constexpr int kWideMinTiles = 2;        // tiles a CTA takes at least
-constexpr uint32_t kWideRegsLaunch = 168, kWideRegsSoftmax = 216, kWideRegsOther = 72;
+constexpr uint32_t kWideRegsLaunch = 168, kWideRegsSoftmax = 200, kWideRegsOther = 104;
 static_assert(2 * 128 * kWideRegsSoftmax + 128 * kWideRegsOther <= kWideThreads * kWideRegsLaunch,
               "the warpgroup register split must fit in the registers the CTA launches with");
 
