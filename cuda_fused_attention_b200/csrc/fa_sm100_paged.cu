@@ -599,8 +599,9 @@ combine_narrow_kernel(const __grid_constant__ PagedParams p, int ctas)
 // tiles (256 rows) that ping-pong between two softmax warpgroups, as in the dense kernel. The
 // arithmetic is 4 D operations per (row, key) against 4 D bytes per key and block, so the tensor
 // pipe and the exponentials bound it, not memory. The work of all requests, K/V heads and blocks
-// is one line of 128-key tiles (request, head, block, key) of which each of the grid's CTAs (one
-// per SM, persistent) takes an equal stretch; blocks that cross a border are merged from parts by
+// is one line of 128-key tiles (request, head, block, key; each block preceded by kWideGap idle units
+// that stand for its set-up and epilogue) of which each of the grid's CTAs (one per SM, persistent)
+// takes an equal stretch; blocks that cross a border are merged from parts by
 // combine_wide_kernel. Within a CTA the K/V ring runs on across blocks, the first products of a
 // block overlap the epilogue of the one before.
 //
@@ -610,7 +611,7 @@ combine_narrow_kernel(const __grid_constant__ PagedParams p, int ctas)
 // Tensor memory, barriers per key tile, register split and the lazily moved exponent base are
 // those of the dense kernel (fa_sm100.cu). P is rounded to bf16 for the product with V.
 constexpr int kWideThreads = 384;
-constexpr int kWideMinTiles = 2;        // tiles a CTA takes at least
+constexpr int kWideMinTiles = 4;        // units a CTA takes at least
 constexpr uint32_t kWideRegsLaunch = 168, kWideRegsSoftmax = 200, kWideRegsOther = 104;
 static_assert(2 * 128 * kWideRegsSoftmax + 128 * kWideRegsOther <= kWideThreads * kWideRegsLaunch,
               "the warpgroup register split must fit in the registers the CTA launches with");
@@ -642,7 +643,10 @@ struct WideCfg {
     static constexpr int kNumBars = kBarSchedEmpty + 2;
     static constexpr int kMiscOff = kBarOff + kNumBars * 8;     // tensor memory base, abort flag
     static constexpr int kSegOff = (kMiscOff + 8 + 15) / 16 * 16;
-    static constexpr int kSmemBytes = kSegOff + 2 * 64 + 1024;
+    // Epilogue staging per softmax warp: 32 rows of 32 columns, 16 bytes apart so that rows fall on different banks.
+    static constexpr int kStageStride = 80;
+    static constexpr int kStageOff = kSegOff + 2 * 64;
+    static constexpr int kSmemBytes = kStageOff + 8 * 32 * kStageStride + 1024;
     static constexpr uint32_t kColS0 = 0, kColS1 = 128, kColO0 = 256, kColO1 = 256 + D;
     static constexpr uint32_t kIdescQK = make_idesc_bf16(kWideRows, kWideKeys, false);
     static constexpr uint32_t kIdescPV = make_idesc_bf16(kWideRows, D, true);
@@ -681,16 +685,17 @@ __device__ inline WideSegment wide_segment(const FaPagedPlan& plan, const long l
     int lo = 0, hi = (n - 1) / span;        // last block whose tiles begin at or before x
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (head_first + wide_tiles_through(mid, span, cached, n, causal) <= x) lo = mid;
+        if (head_first + wide_units_through(mid, span, cached, n, causal) <= x) lo = mid;
         else hi = mid - 1;
     }
-    s.first = head_first + wide_tiles_through(lo, span, cached, n, causal);
+    s.first = head_first + wide_units_through(lo, span, cached, n, causal) + kWideGap;
     s.last = s.first + wide_tiles_of(lo, span, cached, n, causal);
+    if (x < s.first) x = s.first;
     s.token0 = plan.query_start[s.b] + lo * span;
     s.tokens = min(span, n - lo * span);
     s.pos0 = cached + lo * span;
     s.tile = static_cast<int>(x - s.first);
-    s.count = static_cast<int>((s.last < end ? s.last : end) - x);
+    s.count = static_cast<int>((s.last < end ? s.last : end) - x);     // 0 or less: only idle units are left before end
     s.part = -1;
     s.reserved = 0;
     // Behind the last key: rows of the last page (pages behind it are zero-filled by the copy).
@@ -902,6 +907,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     umma_commit(bar(C::kBarSFull + 1));
                 }
                 umma_commit(empty_bar(ri));
+                if (count == 1) umma_commit(bar(C::kBarQEmpty));
                 for (int j = 0; j < count; ++j) {
                     const int vi = ri + 2 * j + 1, ki = vi + 1;
                     const bool more = j + 1 < count;
@@ -940,6 +946,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                         umma_commit(empty_bar(vi));
                     }
                     if (more) umma_commit(empty_bar(ki));
+                    if (j + 2 == count) umma_commit(bar(C::kBarQEmpty));    // the segment's last S is on its way
                 }
                 return true;
             };
@@ -955,8 +962,6 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     if (ok) {
                         tc_fence_after();
                         ok = two ? issue_segment(std::true_type{}, count) : issue_segment(std::false_type{}, count);
-                        // Q is free once the segment's last S is done, a little earlier than this.
-                        if (ok) umma_commit(bar(C::kBarQEmpty));
                         ri += 2 * count;
                     }
                 }
@@ -998,15 +1003,20 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 if (sg > 1 && !wait_paged(bar(C::kBarSchedEmpty + (sg & 1)), ((sg >> 1) - 1) & 1, abort_flag, kSiteWideSched))
                     break;
                 WideSegment s;
-                if (x < end) {
+                s.count = 0;
+                while (x < end && s.count <= 0) {
                     s = wide_segment(plan, start, x, end);
+                    if (s.count <= 0) {
+                        s.count = 0;
+                        x = s.last;
+                    }
+                }
+                if (s.count > 0) {
                     // A block that began before this CTA's range leaves its part in the CTA's first place, one
                     // that goes on behind it in the second.
                     if (s.first < begin) s.part = 2 * static_cast<int>(blockIdx.x);
                     else if (s.last > end) s.part = 2 * static_cast<int>(blockIdx.x) + 1;
-                    x += s.count;
-                } else {
-                    s.count = 0;
+                    x = s.first + s.tile + s.count;
                 }
                 segments[sg & 1] = s;
                 mbar_arrive(bar(C::kBarSchedFull + (sg & 1)));
@@ -1024,7 +1034,6 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const uint32_t t_s = lane_base + (t == 0 ? C::kColS0 : C::kColS1);
         const uint32_t t_o = lane_base + (t == 0 ? C::kColO0 : C::kColO1);
         const int tok = t * per_tile + r / group;       // token of this row within its block
-        const bool in_tile = r < per_tile * group;
         const float sl2 = p.scale_log2;
         const uint64_t c2 = f2_pack(sl2, sl2);
         uint32_t phase = 0;                        // parity of this tile's per-key-tile barriers
@@ -1179,27 +1188,47 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             o_phase ^= 1u;
             tc_fence_after();
             const int part = seg.part;
-            const bool real = in_tile && tok < seg.tokens;
-            __nv_bfloat16* out = p.o + static_cast<long long>(seg.token0 + tok) * p.o_token +
-                                 static_cast<long long>(seg.h * group + r % group) * p.o_head;
+            // A row of 32 columns is 64 bytes: staged in shared memory, four lanes write one row, so that a warp's
+            // store touches 8 rows and not 32. This lane writes rows 8 i + lane / 4 of the warp's 32.
+            __nv_bfloat16* out[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = quarter * 32 + 8 * i + lane / 4;
+                const int row_tok = t * per_tile + row / group;
+                const bool real = row < per_tile * group && row_tok < seg.tokens;
+                out[i] = real ? p.o + static_cast<long long>(seg.token0 + row_tok) * p.o_token +
+                                    static_cast<long long>(seg.h * group + row % group) * p.o_head + (lane % 4) * 8
+                              : nullptr;
+            }
             release_segment(sg);
             if (part < 0) {
                 const float inv = 1.0f / row_sum;
+                const uint32_t stage = base + C::kStageOff + static_cast<uint32_t>(warp * 32 * C::kStageStride);
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t o[32];
                     tmem_ld32(t_o + static_cast<uint32_t>(c * 32), o);
                     tmem_wait_ld();
                     reg_fence32(o);
-                    if (real) {
+                    __syncwarp();
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            uint32_t w[4];
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t w[4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                w[i] = pack_bf16x2(__uint_as_float(o[8 * q + 2 * i]) * inv, __uint_as_float(o[8 * q + 2 * i + 1]) * inv);
-                            *reinterpret_cast<uint4*>(out + c * 32 + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            w[i] = pack_bf16x2(__uint_as_float(o[8 * q + 2 * i]) * inv, __uint_as_float(o[8 * q + 2 * i + 1]) * inv);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                                     :: "r"(stage + lane * C::kStageStride + q * 16), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                                     : "memory");
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint4 w;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                                     : "r"(stage + (8 * i + lane / 4) * C::kStageStride + (lane % 4) * 16) : "memory");
+                        if (out[i] != nullptr) *reinterpret_cast<uint4*>(out[i] + c * 32) = w;
                     }
                 }
             } else {
@@ -1251,7 +1280,7 @@ combine_wide_kernel(const __grid_constant__ PagedParams p, int ctas)
     bool merges = false;
     if (border < total) {
         s = wide_segment(plan, start, border, total);
-        merges = s.first != border && s.first >= border - share && r < per_tile * group && tok < s.tokens;
+        merges = s.first < border && s.first >= border - share && r < per_tile * group && tok < s.tokens;
     }
     grid_dependency_wait();
     if (!merges) return;

@@ -5,7 +5,8 @@
 // rows per K/V head (row = token * G + head in group). Requests of at most narrow_rows(plan) rows
 // go to the narrow kernel, whose unit of work is a 64-key tile; all others to the wide kernel,
 // whose unit is a 128-key tile of a block of 2 * tokens_per_tile(G) tokens. Each narrow item (one
-// K/V head of a request) is preceded by kNarrowGap units without work, about what its set-up costs.
+// K/V head of a request) and each block is preceded by kNarrowGap or kWideGap units without work,
+// about what its set-up and epilogue cost.
 #pragma once
 
 #include <cstdint>
@@ -15,6 +16,7 @@
 namespace fa_sm100 {
 
 constexpr int kNarrowGap = 1;
+constexpr int kWideGap = 2;
 constexpr int kNarrowKeys = 64;
 constexpr int kWideRows = 128;      // query rows of one tile (tensor-memory lanes)
 constexpr int kWideKeys = 128;
@@ -61,15 +63,15 @@ __host__ __device__ inline long long wide_tiles_of(long long u, long long span, 
     return ceil_div(cached + (causal ? end : n), kWideKeys);
 }
 
-// Key tiles of the request's first `blocks` token blocks.
-__host__ __device__ inline long long wide_tiles_through(long long blocks, long long span, long long cached, long long n,
+// Units (key tiles and gaps) of the request's first `blocks` token blocks.
+__host__ __device__ inline long long wide_units_through(long long blocks, long long span, long long cached, long long n,
                                                         bool causal)
 {
     if (blocks <= 0) return 0;
-    if (!causal) return blocks * ceil_div(cached + n, kWideKeys);
+    if (!causal) return blocks * (kWideGap + ceil_div(cached + n, kWideKeys));
     const long long whole = n / span < blocks ? n / span : blocks;      // blocks that end at (u + 1) * span
     const long long sum = floor_sum_128(whole, span, cached + span + kWideKeys - 1);
-    return sum + (blocks > whole ? ceil_div(cached + n, kWideKeys) : 0);
+    return sum + blocks * kWideGap + (blocks > whole ? ceil_div(cached + n, kWideKeys) : 0);
 }
 
 // Last b in [0, num_seqs) with start[b] <= y, for start[0] = 0 <= y < start[num_seqs].

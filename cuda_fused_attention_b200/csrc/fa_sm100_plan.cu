@@ -111,7 +111,7 @@ plan_kernel(const PlanParams p)
         if (!fits && first_cta && b < plan.num_seqs) record_plan_error(FA_ERROR_BAD_LENGTH);
         if (valid && fits && n > 0) {
             if (n * group <= narrow_rows(plan)) narrow_units = kNarrowGap + ceil_div(cached + n, kNarrowKeys);
-            else wide_units = wide_tiles_through(ceil_div(n, span), span, cached, n, plan.causal != 0);
+            else wide_units = wide_units_through(ceil_div(n, span), span, cached, n, plan.causal != 0);
         }
         s_start[tid] = static_cast<int>(tokens_before < total ? tokens_before : total);
         s_page[tid] = static_cast<int>(pages_before - carry.pages < INT_MAX ? pages_before - carry.pages : INT_MAX);
