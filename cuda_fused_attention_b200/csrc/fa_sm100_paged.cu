@@ -43,7 +43,7 @@ constexpr float kRebase = 16.0f;
 // D = 128 against 32 * 4 * 128 operations. The work of all requests and K/V heads is one line of
 // 64-key tiles (request, then head, then key; each item preceded by kNarrowGap idle units that stand
 // for its set-up), and each of the grid's CTAs (two per SM) takes an equal stretch of it, whatever the
-// requests' lengths: an item that crosses a border is merged from parts by combine_narrow_kernel. A
+// requests' lengths: an item that crosses a border is merged from parts (paged_combine_kernel). A
 // CTA's warp 4 streams the tiles by TMA through a ring that runs on across items, page by page (a page
 // that is absent reads as zeros), with each item's Q and description ahead of its first tile; warps
 // 0-3 share out the keys of every tile (and the two 16-row tiles, if MT, their number, is 2), S = Q K^T
@@ -171,7 +171,10 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const long long share = narrow_share(total, gridDim.x);
     const long long begin = share * blockIdx.x;
     grid_dependents_launch();
-    if (begin >= total) return;
+    if (begin >= total) {
+        grid_dependency_wait();
+        return;
+    }
     const long long end = begin + share < total ? begin + share : total;
 
     extern __shared__ uint8_t smem_raw[];
@@ -286,6 +289,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             for (int i = sg > C::kQSlots ? sg - C::kQSlots : 0; i < sg; ++i)
                 drain_paged(item_full(i % C::kQSlots), (i / C::kQSlots) & 1);
         }
+        grid_dependency_wait();     // the wide kernel, if it was launched before this one, is done when this one is
         return;
     }
 
@@ -514,83 +518,6 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     }
 }
 
-// One block per border between two CTAs' ranges; the first border inside an item merges the item's
-// parts, in their order, one warp per row. It is launched while the narrow kernel still runs
-// (programmatic dependent launch) and finds its item meanwhile.
-template <int D, int MT>
-__global__ void __launch_bounds__(512)
-combine_narrow_kernel(const __grid_constant__ PagedParams p, int ctas)
-{
-    using C = NarrowCfg<D, MT>;
-    const FaPagedPlan& plan = p.plan;
-    const long long* start = narrow_starts(plan.schedule, plan.num_seqs);
-    const long long total = start[plan.num_seqs] * plan.kv_heads;
-    const long long share = narrow_share(total, ctas);
-    const long long border = share * (blockIdx.x + 1);
-    const int row = 16 * static_cast<int>(blockIdx.y) + threadIdx.x / 32, lane = threadIdx.x % 32;
-    int count = 0;                          // parts of this block's item (0: none to merge here)
-    const float* first = nullptr;           // the first ends its CTA's range; the others begin theirs
-    __nv_bfloat16* out = nullptr;
-    constexpr int E = D / 32;
-    constexpr long long kNext = 2LL * C::kPartFloats;
-    if (border < total) {
-        const NarrowPlace s = narrow_place(plan, start, border);
-        const int token0 = plan.query_start[s.b], n = plan.query_start[s.b + 1] - token0;
-        const int group = plan.heads / plan.kv_heads;
-        if (s.first < border && s.first >= border - share && row < n * group) {
-            const long long c0 = s.first / share;
-            count = static_cast<int>((s.last - 1) / share - c0) + 1;
-            first = p.partial + (2 * c0 + 1) * C::kPartFloats;
-            const int tok = row / group;
-            out = p.o + static_cast<long long>(token0 + tok) * p.o_token +
-                  static_cast<long long>(s.h * group + row - tok * group) * p.o_head + lane * E;
-        }
-    }
-    grid_dependency_wait();
-    if (count == 0) return;
-    auto part = [&](int i) { return i == 0 ? first : first + i * kNext - C::kPartFloats; };
-    // 32 parts at a time: a lane reads one part's maximum and sum, then all lanes add up its columns.
-    float top = -INFINITY, sum = 0.0f, acc[E] = {};
-    for (int i0 = 0; i0 < count; i0 += 32) {
-        const int mine = i0 + lane;
-        const float m = mine < count ? part(mine)[16 * MT * D + row] : -INFINITY;
-        const float l = mine < count ? part(mine)[16 * MT * D + 16 * MT + row] : 0.0f;
-        float high = fmaxf(m, top);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
-        const float keep = top == -INFINITY ? 0.0f : ex2_approx((top - high) * p.scale_log2);
-        const float w = m == -INFINITY ? 0.0f : ex2_approx((m - high) * p.scale_log2);
-        float wl = w * l;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) wl += __shfl_xor_sync(0xffffffffu, wl, d);
-        sum = sum * keep + wl;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] *= keep;
-        top = high;
-        const int here = min(32, count - i0);
-#pragma unroll 8
-        for (int i = 0; i < here; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float* at = part(i0 + i) + row * D + lane * E;
-            if constexpr (E == 4) {
-                const float4 v = *reinterpret_cast<const float4*>(at);
-                acc[0] += wi * v.x;
-                acc[1] += wi * v.y;
-                acc[2] += wi * v.z;
-                acc[3] += wi * v.w;
-            } else {
-                const float2 v = *reinterpret_cast<const float2*>(at);
-                acc[0] += wi * v.x;
-                acc[1] += wi * v.y;
-            }
-        }
-    }
-    const float inv = 1.0f / sum;
-#pragma unroll
-    for (int e = 0; e < E; e += 2)
-        *reinterpret_cast<uint32_t*>(out + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
-}
-
 // =============================================================================
 // Wide kernel: requests of more than 16 query rows per K/V head (chunks of tokens)
 // =============================================================================
@@ -601,8 +528,7 @@ combine_narrow_kernel(const __grid_constant__ PagedParams p, int ctas)
 // pipe and the exponentials bound it, not memory. The work of all requests, K/V heads and blocks
 // is one line of 128-key tiles (request, head, block, key; each block preceded by kWideGap idle units
 // that stand for its set-up and epilogue) of which each of the grid's CTAs (one per SM, persistent)
-// takes an equal stretch; blocks that cross a border are merged from parts by
-// combine_wide_kernel. Within a CTA the K/V ring runs on across blocks, the first products of a
+// takes an equal stretch; blocks that cross a border are merged from parts. Within a CTA the K/V ring runs on across blocks, the first products of a
 // block overlap the epilogue of the one before.
 //
 // Warps: 0-3 and 4-7 softmax, O correction and epilogue of Q tile 0 and 1 (one thread per row);
@@ -1260,21 +1186,103 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
 }
 
-// One block row per border between two CTAs' ranges; the first border inside a block of tokens merges
-// its parts, in their order. A thread is a query row and takes 32 columns of one Q tile. Launched while
-// the wide kernel still runs, as combine_narrow_kernel.
+// =============================================================================
+// Merging of parts
+// =============================================================================
+// An item (narrow) or block (wide) that crosses borders between CTAs' ranges left a part in each; the
+// first border inside it merges them, in their order, so that a result does not depend on which CTA
+// was done first. A row's parts O_i, with maxima m_i and sums l_i, give
+//     sum_i w_i O_i / sum_i w_i l_i,   w_i = 2^((m_i - max_i m_i) log2(e) / sqrt(D)).
+// The kernel is launched while those before it still run (programmatic dependent launch) and finds its
+// parts' places meanwhile.
+constexpr int kCombineThreads = 512;
+
+// One row per warp; a lane has D / 32 columns.
+template <int D, int MT>
+__device__ __forceinline__ void combine_narrow(const PagedParams& p, int ctas, int border_index, int row_tile)
+{
+    using C = NarrowCfg<D, MT>;
+    const FaPagedPlan& plan = p.plan;
+    const long long* start = narrow_starts(plan.schedule, plan.num_seqs);
+    const long long total = start[plan.num_seqs] * plan.kv_heads;
+    const long long share = narrow_share(total, ctas);
+    const long long border = share * (border_index + 1);
+    const int row = 16 * row_tile + threadIdx.x / 32, lane = threadIdx.x % 32;
+    int count = 0;                          // parts of this border's item (0: none to merge here)
+    const float* first = nullptr;           // the first ends its CTA's range; the others begin theirs
+    __nv_bfloat16* out = nullptr;
+    constexpr int E = D / 32;
+    constexpr long long kNext = 2LL * C::kPartFloats;
+    if (border < total) {
+        const NarrowPlace s = narrow_place(plan, start, border);
+        const int token0 = plan.query_start[s.b], n = plan.query_start[s.b + 1] - token0;
+        const int group = plan.heads / plan.kv_heads;
+        if (s.first < border && s.first >= border - share && row < n * group) {
+            const long long c0 = s.first / share;
+            count = static_cast<int>((s.last - 1) / share - c0) + 1;
+            first = p.partial + (2 * c0 + 1) * C::kPartFloats;
+            const int tok = row / group;
+            out = p.o + static_cast<long long>(token0 + tok) * p.o_token +
+                  static_cast<long long>(s.h * group + row - tok * group) * p.o_head + lane * E;
+        }
+    }
+    grid_dependency_wait();
+    if (count == 0) return;
+    auto part = [&](int i) { return i == 0 ? first : first + i * kNext - C::kPartFloats; };
+    // 32 parts at a time: a lane reads one part's maximum and sum, then all lanes add up its columns.
+    float top = -INFINITY, sum = 0.0f, acc[E] = {};
+    for (int i0 = 0; i0 < count; i0 += 32) {
+        const int mine = i0 + lane;
+        const float m = mine < count ? part(mine)[16 * MT * D + row] : -INFINITY;
+        const float l = mine < count ? part(mine)[16 * MT * D + 16 * MT + row] : 0.0f;
+        float high = fmaxf(m, top);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+        const float keep = top == -INFINITY ? 0.0f : ex2_approx((top - high) * p.scale_log2);
+        const float w = m == -INFINITY ? 0.0f : ex2_approx((m - high) * p.scale_log2);
+        float wl = w * l;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) wl += __shfl_xor_sync(0xffffffffu, wl, d);
+        sum = sum * keep + wl;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= keep;
+        top = high;
+        const int here = min(32, count - i0);
+#pragma unroll 8
+        for (int i = 0; i < here; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const float* at = part(i0 + i) + row * D + lane * E;
+            if constexpr (E == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(at);
+                acc[0] += wi * v.x;
+                acc[1] += wi * v.y;
+                acc[2] += wi * v.z;
+                acc[3] += wi * v.w;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(at);
+                acc[0] += wi * v.x;
+                acc[1] += wi * v.y;
+            }
+        }
+    }
+    const float inv = 1.0f / sum;
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+        *reinterpret_cast<uint32_t*>(out + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+}
+
+// A thread is a query row and takes 32 columns (group c) of Q tile t.
 template <int D>
-__global__ void __launch_bounds__(kWideRows)
-combine_wide_kernel(const __grid_constant__ PagedParams p, int ctas)
+__device__ __forceinline__ void combine_wide(const PagedParams& p, int ctas, int border_index, int t, int c)
 {
     using C = WideCfg<D>;
     const FaPagedPlan& plan = p.plan;
     const long long* start = wide_starts(plan.schedule, plan.num_seqs);
     const long long total = start[plan.num_seqs] * plan.kv_heads;
     const long long share = wide_share(total, ctas);
-    const long long border = share * (blockIdx.x + 1);
+    const long long border = share * (border_index + 1);
     const int group = plan.heads / plan.kv_heads, per_tile = tokens_per_tile(group);
-    const int t = blockIdx.y / (D / 32), c = blockIdx.y % (D / 32), r = threadIdx.x;
+    const int r = threadIdx.x % kWideRows;
     const int tok = t * per_tile + r / group;
     WideSegment s;
     bool merges = false;
@@ -1315,6 +1323,22 @@ combine_wide_kernel(const __grid_constant__ PagedParams p, int ctas)
         *reinterpret_cast<uint4*>(out + q * 4) =
             make_uint4(pack_bf16x2(acc[q].x * inv, acc[q].y * inv), pack_bf16x2(acc[q].z * inv, acc[q].w * inv),
                        pack_bf16x2(acc[q + 1].x * inv, acc[q + 1].y * inv), pack_bf16x2(acc[q + 1].z * inv, acc[q + 1].w * inv));
+}
+
+// Blocks [0, narrow_blocks) serve the narrow kernel's borders, the others the wide kernel's.
+template <int D, int MT>
+__global__ void __launch_bounds__(kCombineThreads)
+paged_combine_kernel(const __grid_constant__ PagedParams p, int narrow_ctas, int wide_ctas)
+{
+    const int narrow_blocks = narrow_ctas > 0 ? (narrow_ctas - 1) * MT : 0;
+    const int block = static_cast<int>(blockIdx.x);
+    if (block < narrow_blocks) {
+        combine_narrow<D, MT>(p, narrow_ctas, block / MT, block % MT);
+    } else {
+        constexpr int kPieces = 2 * (D / 32), kPerBlock = kCombineThreads / kWideRows;
+        const int piece = (block - narrow_blocks) * kPerBlock + static_cast<int>(threadIdx.x) / kWideRows;
+        combine_wide<D>(p, wide_ctas, piece / kPieces, piece % kPieces / (D / 32), piece % (D / 32));
+    }
 }
 
 }  // namespace fa_sm100
@@ -1459,41 +1483,46 @@ int cache_map(CUtensorMap* map, const void* ptr, const FaPagedPlan& plan, const 
     return fa_sm100_internal::encode_map(map, ptr, 4, dims, bytes, box);
 }
 
-// Launches a kernel that may start before the one in front of it in the stream is done; it waits for
-// that one itself (grid_dependency_wait).
+// Launches a kernel; `early`: it may start before the one in front of it in the stream is done, and waits
+// for that one itself (grid_dependency_wait).
 template <typename... Args>
-int launch_early(void (*kernel)(Args...), dim3 grid, int threads, cudaStream_t stream, Args... args)
+int launch(void (*kernel)(Args...), int grid, int threads, int shared_bytes, bool early, cudaStream_t stream, const Args&... args)
 {
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = grid;
+    config.gridDim = dim3(static_cast<unsigned>(grid));
     config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.dynamicSmemBytes = static_cast<size_t>(shared_bytes);
     config.stream = stream;
     config.attrs = &attribute;
-    config.numAttrs = 1;
+    config.numAttrs = early ? 1 : 0;
     return static_cast<int>(cudaLaunchKernelEx(&config, kernel, args...));
 }
 
-template <int D, int MT>
-int launch_narrow(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const PagedParams& params, int sms, cudaStream_t stream)
-{
-    const int ctas = narrow_ctas(sms);
-    paged_narrow_kernel<D, MT><<<ctas, kNarrowThreads, NarrowCfg<D, MT>::kSmemBytes, stream>>>(tm_k, tm_v, params);
-    cudaError_t err = cudaGetLastError();
-    if (err != cudaSuccess) return static_cast<int>(err);
-    return launch_early(combine_narrow_kernel<D, MT>, dim3(ctas - 1, MT), 512, stream, params, ctas);
-}
+struct PagedMaps {
+    CUtensorMap q;                          // wide
+    CUtensorMap wide_k, wide_v;
+    CUtensorMap narrow_k, narrow_v;
+};
 
-template <int D>
-int launch_wide(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const PagedParams& params,
-                int sms, cudaStream_t stream)
+// The wide kernel, the narrow one (it needs nothing of the wide one, so it fills the SMs that fall idle), then
+// the merging of both kernels' parts.
+template <int D, int MT>
+int launch_attention(const PagedMaps& maps, const PagedParams& params, bool wide, bool narrow, int sms, cudaStream_t stream)
 {
-    paged_wide_kernel<D><<<sms, kWideThreads, WideCfg<D>::kSmemBytes, stream>>>(tm_q, tm_k, tm_v, params);
-    cudaError_t err = cudaGetLastError();
-    if (err != cudaSuccess) return static_cast<int>(err);
-    return launch_early(combine_wide_kernel<D>, dim3(sms - 1, 2 * (D / 32)), kWideRows, stream, params, sms);
+    int status = FA_STATUS_OK;
+    if (wide)
+        status = launch(paged_wide_kernel<D>, sms, kWideThreads, WideCfg<D>::kSmemBytes, false, stream, maps.q, maps.wide_k,
+                        maps.wide_v, params);
+    const int ctas = narrow ? narrow_ctas(sms) : 0;
+    if (narrow && status == FA_STATUS_OK)
+        status = launch(paged_narrow_kernel<D, MT>, ctas, kNarrowThreads, NarrowCfg<D, MT>::kSmemBytes, wide, stream,
+                        maps.narrow_k, maps.narrow_v, params);
+    if (status != FA_STATUS_OK) return status;
+    const int blocks = (narrow ? (ctas - 1) * MT : 0) + (wide ? (sms - 1) * 2 * (D / 32) * kWideRows / kCombineThreads : 0);
+    return launch(paged_combine_kernel<D, MT>, blocks, kCombineThreads, 0, true, stream, params, ctas, wide ? sms : 0);
 }
 
 }  // namespace
@@ -1551,41 +1580,37 @@ int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cac
     params.page_shift = __builtin_ctz(static_cast<unsigned>(plan->page_size));
     params.scale_log2 = fa_default_scale(plan->head_dim) * 1.4426950408889634f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    CUtensorMap tm_k, tm_v;
-    int map_rows = 0;           // rows of a box of the two maps; they serve both kernels where pages are that short
-    auto cache_maps = [&](int rows) -> int {
-        rows = plan->page_size < rows ? plan->page_size : rows;
-        if (rows == map_rows) return FA_STATUS_OK;
-        map_rows = rows;
-        const int made = cache_map(&tm_k, k_cache, *plan, strides + 4, rows);
-        return made != FA_STATUS_OK ? made : cache_map(&tm_v, v_cache, *plan, strides + 7, rows);
-    };
+    const bool wide = may_be_wide(*plan), narrow = may_be_narrow(*plan);
+    PagedMaps maps;
     char* work = static_cast<char*>(workspace);
-    if (may_be_wide(*plan)) {
+    if (wide) {
         params.wide_partial = reinterpret_cast<float*>(work);
         work += wide_workspace(sms, plan->head_dim);
-        CUtensorMap tm_q;
         const int group = plan->heads / plan->kv_heads;
         const cuuint64_t dims[3] = {static_cast<cuuint64_t>(plan->head_dim), static_cast<cuuint64_t>(plan->heads),
                                     static_cast<cuuint64_t>(plan->total_tokens)};
         const cuuint64_t bytes[2] = {static_cast<cuuint64_t>(params.q_head) * 2u, static_cast<cuuint64_t>(params.q_token) * 2u};
         const cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(tokens_per_tile(group))};
-        if ((status = fa_sm100_internal::encode_map(&tm_q, q, 3, dims, bytes, box)) != FA_STATUS_OK) return status;
-        if ((status = cache_maps(kWideKeys)) != FA_STATUS_OK) return status;
-        status = plan->head_dim == 64 ? launch_wide<64>(tm_q, tm_k, tm_v, params, sms, s)
-                                      : launch_wide<128>(tm_q, tm_k, tm_v, params, sms, s);
-        if (status != FA_STATUS_OK) return status;
+        if ((status = fa_sm100_internal::encode_map(&maps.q, q, 3, dims, bytes, box)) != FA_STATUS_OK) return status;
+        if ((status = cache_map(&maps.wide_k, k_cache, *plan, strides + 4, kWideKeys)) != FA_STATUS_OK) return status;
+        if ((status = cache_map(&maps.wide_v, v_cache, *plan, strides + 7, kWideKeys)) != FA_STATUS_OK) return status;
     }
-    if (may_be_narrow(*plan)) {
+    if (narrow) {
         params.partial = reinterpret_cast<float*>(work);
-        if ((status = cache_maps(kNarrowKeys)) != FA_STATUS_OK) return status;
-        const bool one = narrow_rows(*plan) == 16;
-        if (plan->head_dim == 64)
-            status = one ? launch_narrow<64, 1>(tm_k, tm_v, params, sms, s) : launch_narrow<64, 2>(tm_k, tm_v, params, sms, s);
-        else
-            status = one ? launch_narrow<128, 1>(tm_k, tm_v, params, sms, s) : launch_narrow<128, 2>(tm_k, tm_v, params, sms, s);
+        if (wide && plan->page_size <= kNarrowKeys) {       // the same boxes
+            maps.narrow_k = maps.wide_k;
+            maps.narrow_v = maps.wide_v;
+        } else {
+            if ((status = cache_map(&maps.narrow_k, k_cache, *plan, strides + 4, kNarrowKeys)) != FA_STATUS_OK) return status;
+            if ((status = cache_map(&maps.narrow_v, v_cache, *plan, strides + 7, kNarrowKeys)) != FA_STATUS_OK) return status;
+        }
     }
-    return status;
+    const bool one = narrow_rows(*plan) == 16;
+    if (plan->head_dim == 64)
+        return one ? launch_attention<64, 1>(maps, params, wide, narrow, sms, s)
+                   : launch_attention<64, 2>(maps, params, wide, narrow, sms, s);
+    return one ? launch_attention<128, 1>(maps, params, wide, narrow, sms, s)
+               : launch_attention<128, 2>(maps, params, wide, narrow, sms, s);
 }
 
 }  // extern "C"

@@ -292,6 +292,46 @@ rotary_kernel(const __grid_constant__ RotaryParams p)
     const int tokens = min(group, p.tokens - token0);
     const int pairs = p.rotary_dim / 2;
 
+    // An item is a unit of a row. Neighbouring threads take the units of a row, then the rows that are
+    // neighbours in memory: the next head of a packed token, the next token of a [heads, tokens] tensor.
+    const int rotating = p.rotary_dim / 16;
+    const int rows = p.rows[0] + (kAppend ? p.rows[1] + p.rows[2] : 0);
+    const int total = (kAppend ? tokens : group) * rows << p.unit_shift;
+    const int unit = threadIdx.x & ((1 << p.unit_shift) - 1);       // the same for all of a thread's items
+    const bool turns = unit < rotating;
+    // The unit's two 8-element pieces: the two halves of its pairs, or 16 neighbours.
+    const int lo = turns && !kInterleaved ? 8 * unit : 16 * unit;
+    const int hi = turns && !kInterleaved ? pairs + 8 * unit : 16 * unit + 8;
+    // Token, head and tensor of an item; false: there is none.
+    auto locate = [&](int index, int& tok, int& head, int& which) -> bool {
+        const int item = index >> p.unit_shift;
+        which = 0;
+        if (kAppend) {
+            tok = item / rows;
+            head = item - tok * rows;
+            if (head >= p.rows[0]) { head -= p.rows[0]; which = 1; }
+            if (which == 1 && head >= p.rows[1]) { head -= p.rows[1]; which = 2; }
+            return index < total;
+        }
+        tok = item & (group - 1);
+        head = item >> p.group_shift;
+        return index < total && tok < tokens;
+    };
+    uint4 x0[kRotaryBatch], x1[kRotaryBatch];
+    auto load = [&](int first) {
+#pragma unroll
+        for (int k = 0; k < kRotaryBatch; ++k) {
+            int tok, head, which;
+            if (!locate(first + k * kRotaryThreads, tok, head, which)) continue;
+            const __nv_bfloat16* src = p.src[which] + batch * p.src_batch + (token0 + tok) * p.src_token[which] +
+                                       head * p.src_head[which];
+            x0[k] = *reinterpret_cast<const uint4*>(src + (which == 2 ? 16 * unit : lo));
+            x1[k] = *reinterpret_cast<const uint4*>(src + (which == 2 ? 16 * unit + 8 : hi));
+        }
+    };
+
+    // The first rows are on their way while the angles are computed.
+    load(threadIdx.x);
     if (kAppend && threadIdx.x < tokens) {
         long long slot = p.slots[token0 + threadIdx.x];
         if (slot >= p.num_slots) {
@@ -306,62 +346,24 @@ rotary_kernel(const __grid_constant__ RotaryParams p)
 #pragma unroll
         for (int a = 0; a < kMaxAxes - 1; ++a) axis += pair >= p.section_end[a] ? 1 : 0;
         const int position = p.positions[axis * p.position_axis + batch * p.position_batch + token0 + tok];
-        const double turns = static_cast<double>(position) * static_cast<double>(p.inv_freq[pair]) * 0.15915494309189533577;
+        const double around = static_cast<double>(position) * static_cast<double>(p.inv_freq[pair]) * 0.15915494309189533577;
         float sine, cosine;
-        sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sine, &cosine);
+        sincospif(2.0f * static_cast<float>(around - rint(around)), &sine, &cosine);
         turn[tok][pair] = make_float2(cosine, p.sign * sine);
     }
     __syncthreads();
 
-    // Neighbouring threads take the units of a row, then the rows that are neighbours in memory: the next
-    // head of a packed token, the next token of a [heads, tokens] tensor.
-    const int rotating = p.rotary_dim / 16;
-    const int rows = p.rows[0] + (kAppend ? p.rows[1] + p.rows[2] : 0);
-    const int total = (kAppend ? tokens : group) * rows << p.unit_shift;
-    const int unit = threadIdx.x & ((1 << p.unit_shift) - 1);       // the same for all of a thread's items
-    const bool turns = unit < rotating;
-    // The unit's two 8-element pieces: the two halves of its pairs, or 16 neighbours.
-    const int lo = turns && !kInterleaved ? 8 * unit : 16 * unit;
-    const int hi = turns && !kInterleaved ? pairs + 8 * unit : 16 * unit + 8;
     for (int first = threadIdx.x; first < total; first += kRotaryBatch * kRotaryThreads) {
-        uint4 x0[kRotaryBatch], x1[kRotaryBatch];
-        __nv_bfloat16* dst[kRotaryBatch];
-        int tok[kRotaryBatch];                  // -1: nothing here; + 256: copied, not turned (V)
+        if (first != threadIdx.x) load(first);
 #pragma unroll
         for (int k = 0; k < kRotaryBatch; ++k) {
-            const int item = (first + k * kRotaryThreads) >> p.unit_shift;
-            tok[k] = -1;
-            if (first + k * kRotaryThreads >= total) continue;
-            int t, head, which = 0;
-            if (kAppend) {
-                t = item / rows;
-                head = item - t * rows;
-                if (slots[t] < 0) continue;
-                if (head >= p.rows[0]) { head -= p.rows[0]; which = 1; }
-                if (which == 1 && head >= p.rows[1]) { head -= p.rows[1]; which = 2; }
-            } else {
-                t = item & (group - 1);
-                head = item >> p.group_shift;
-                if (t >= tokens) continue;
-            }
-            const long long token = token0 + t;
-            const __nv_bfloat16* src = p.src[which] + batch * p.src_batch + token * p.src_token[which] + head * p.src_head[which];
-            __nv_bfloat16* to = p.dst[which] + head * p.dst_head[which];
-            if (kAppend && which > 0)
-                to += (slots[t] >> p.page_shift) * p.dst_page[which] + (slots[t] & ((1LL << p.page_shift) - 1)) * p.dst_token[which];
-            else
-                to += batch * p.dst_batch + token * p.dst_token[which];
-            dst[k] = to;
-            tok[k] = t + (which == 2 ? 256 : 0);
-            x0[k] = *reinterpret_cast<const uint4*>(src + (which == 2 ? 16 * unit : lo));
-            x1[k] = *reinterpret_cast<const uint4*>(src + (which == 2 ? 16 * unit + 8 : hi));
-        }
-#pragma unroll
-        for (int k = 0; k < kRotaryBatch; ++k) {
-            if (tok[k] < 0) continue;
-            const bool copied = kAppend && tok[k] >= 256;
+            int tok, head, which;
+            if (!locate(first + k * kRotaryThreads, tok, head, which)) continue;
+            const long long slot = kAppend ? slots[tok] : 0;
+            if (slot < 0) continue;
+            const bool copied = kAppend && which == 2;
             if (turns && !copied) {
-                const float4* cs = reinterpret_cast<const float4*>(&turn[tok[k]][8 * unit]);
+                const float4* cs = reinterpret_cast<const float4*>(&turn[tok][8 * unit]);
                 float a[8], b[8], u[8], w[8];
                 unpack8(x0[k], a);
                 unpack8(x1[k], b);
@@ -386,8 +388,13 @@ rotary_kernel(const __grid_constant__ RotaryParams p)
                 x0[k] = pack8(u);
                 x1[k] = pack8(w);
             }
-            *reinterpret_cast<uint4*>(dst[k] + (copied ? 16 * unit : lo)) = x0[k];
-            *reinterpret_cast<uint4*>(dst[k] + (copied ? 16 * unit + 8 : hi)) = x1[k];
+            __nv_bfloat16* dst = p.dst[which] + head * p.dst_head[which];
+            if (kAppend && which > 0)
+                dst += (slot >> p.page_shift) * p.dst_page[which] + (slot & ((1LL << p.page_shift) - 1)) * p.dst_token[which];
+            else
+                dst += batch * p.dst_batch + (token0 + tok) * p.dst_token[which];
+            *reinterpret_cast<uint4*>(dst + (copied ? 16 * unit : lo)) = x0[k];
+            *reinterpret_cast<uint4*>(dst + (copied ? 16 * unit + 8 : hi)) = x1[k];
         }
     }
 }
