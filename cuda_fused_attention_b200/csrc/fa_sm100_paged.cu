@@ -28,8 +28,19 @@ struct PagedParams {
     long long k_page, k_head, k_row, v_page, v_head, v_row;
     int page_shift;
     float scale_log2;
-    float* wide_partial;        // the same of the wide kernel's blocks
-    float* partial;             // parts of items that cross a border between CTAs' ranges
+    // Parts of items that cross a border between CTAs' ranges, two places per CTA, and per CTA what is to be
+    // merged from the second place on; for the narrow and for the wide kernel.
+    float* partial;
+    struct Merge* merges;
+    float* wide_partial;
+    struct Merge* wide_merges;
+};
+
+// The item whose first part lies in a CTA's second place: it has `parts` parts, the others in the first
+// places of the CTAs that follow. 0: there is none.
+struct Merge {
+    int parts;
+    int token0, tokens, head0;      // packed row of the first token, tokens, first query head
 };
 
 // A row keeps its exponent base until a score exceeds it by this much in the exp2 domain.
@@ -172,7 +183,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const long long begin = share * blockIdx.x;
     grid_dependents_launch();
     if (begin >= total) {
-        grid_dependency_wait();
+        if (threadIdx.x == 0) p.merges[blockIdx.x] = Merge{};
         return;
     }
     const long long end = begin + share < total ? begin + share : total;
@@ -212,6 +223,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         const uint32_t offset = static_cast<uint32_t>(is_v * C::kTile + block * kNarrowKeys * 128 + page_of_tile * rows * 128);
         const void* map = is_v ? static_cast<const void*>(&tm_v) : static_cast<const void*>(&tm_k);
         int it = 0, sg = 0;
+        Merge merge{};
         bool ok = true;
         for (long long x = begin; ok;) {
             NarrowItem item{};
@@ -236,6 +248,9 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 // goes on behind it in the second.
                 item.part = s.first < begin ? 2 * static_cast<int>(blockIdx.x)
                                             : s.last > end ? 2 * static_cast<int>(blockIdx.x) + 1 : -1;
+                if (s.first >= begin && s.last > end)
+                    merge = {static_cast<int>((s.last - 1) / share) - static_cast<int>(blockIdx.x) + 1, item.token0, item.tokens,
+                             item.head0};
                 x = stop;
             }
             const int q_slot = sg % C::kQSlots;
@@ -289,7 +304,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             for (int i = sg > C::kQSlots ? sg - C::kQSlots : 0; i < sg; ++i)
                 drain_paged(item_full(i % C::kQSlots), (i / C::kQSlots) & 1);
         }
-        grid_dependency_wait();     // the wide kernel, if it was launched before this one, is done when this one is
+        if (lane == 0) p.merges[blockIdx.x] = merge;
         return;
     }
 
@@ -592,7 +607,7 @@ struct WideSegment {
     int part;               // place of its part, -1: the whole block, written directly
     int zero_from, zero_to; // rows of the last V tile that must read as zero ([0, 0): none)
     int reserved;
-    long long first, last;  // the block's tiles on the line (combine)
+    long long first, last;  // the block's tiles on the line
 };
 static_assert(sizeof(WideSegment) == 64, "segment slots");
 
@@ -682,7 +697,10 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const long long share = wide_share(total, gridDim.x);
     const long long begin = share * blockIdx.x;
     grid_dependents_launch();
-    if (begin >= total) return;
+    if (begin >= total) {
+        if (threadIdx.x == 0) p.wide_merges[blockIdx.x] = Merge{};
+        return;
+    }
     const long long end = begin + share < total ? begin + share : total;
 
     extern __shared__ uint8_t smem_raw[];
@@ -925,6 +943,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         } else if (lane == 0) {
             // ======================= the walk along the line ===================
             long long x = begin;
+            Merge merge{};
             for (int sg = 0;; ++sg) {
                 if (sg > 1 && !wait_paged(bar(C::kBarSchedEmpty + (sg & 1)), ((sg >> 1) - 1) & 1, abort_flag, kSiteWideSched))
                     break;
@@ -942,12 +961,16 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     // that goes on behind it in the second.
                     if (s.first < begin) s.part = 2 * static_cast<int>(blockIdx.x);
                     else if (s.last > end) s.part = 2 * static_cast<int>(blockIdx.x) + 1;
+                    if (s.first >= begin && s.last > end)
+                        merge = {static_cast<int>((s.last - 1) / share) - static_cast<int>(blockIdx.x) + 1, s.token0, s.tokens,
+                                 s.h * group};
                     x = s.first + s.tile + s.count;
                 }
                 segments[sg & 1] = s;
                 mbar_arrive(bar(C::kBarSchedFull + (sg & 1)));
                 if (s.count == 0) break;
             }
+            p.wide_merges[blockIdx.x] = merge;
         }
         __syncwarp();
     } else {
@@ -1189,52 +1212,32 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 // =============================================================================
 // Merging of parts
 // =============================================================================
-// An item (narrow) or block (wide) that crosses borders between CTAs' ranges left a part in each; the
-// first border inside it merges them, in their order, so that a result does not depend on which CTA
-// was done first. A row's parts O_i, with maxima m_i and sums l_i, give
+// An item (narrow) or block (wide) that crossed borders between CTAs' ranges left a part in each; they
+// are merged in their order, so that a result does not depend on which CTA was done first. A row's
+// parts O_i, with maxima m_i and sums l_i, give
 //     sum_i w_i O_i / sum_i w_i l_i,   w_i = 2^((m_i - max_i m_i) log2(e) / sqrt(D)).
-// The kernel is launched while those before it still run (programmatic dependent launch) and finds its
-// parts' places meanwhile.
-constexpr int kCombineThreads = 512;
+// What to merge was written down by the CTA with the first part. A few round trips to memory bound
+// this, so its blocks are small and launched while the kernel before still runs (programmatic
+// dependent launch).
+constexpr int kCombineThreads = 128;
 
 // One row per warp; a lane has D / 32 columns.
 template <int D, int MT>
-__device__ __forceinline__ void combine_narrow(const PagedParams& p, int ctas, int border_index, int row_tile)
+__device__ __forceinline__ void combine_narrow(const PagedParams& p, int cta, int row)
 {
     using C = NarrowCfg<D, MT>;
-    const FaPagedPlan& plan = p.plan;
-    const long long* start = narrow_starts(plan.schedule, plan.num_seqs);
-    const long long total = start[plan.num_seqs] * plan.kv_heads;
-    const long long share = narrow_share(total, ctas);
-    const long long border = share * (border_index + 1);
-    const int row = 16 * row_tile + threadIdx.x / 32, lane = threadIdx.x % 32;
-    int count = 0;                          // parts of this border's item (0: none to merge here)
-    const float* first = nullptr;           // the first ends its CTA's range; the others begin theirs
-    __nv_bfloat16* out = nullptr;
     constexpr int E = D / 32;
-    constexpr long long kNext = 2LL * C::kPartFloats;
-    if (border < total) {
-        const NarrowPlace s = narrow_place(plan, start, border);
-        const int token0 = plan.query_start[s.b], n = plan.query_start[s.b + 1] - token0;
-        const int group = plan.heads / plan.kv_heads;
-        if (s.first < border && s.first >= border - share && row < n * group) {
-            const long long c0 = s.first / share;
-            count = static_cast<int>((s.last - 1) / share - c0) + 1;
-            first = p.partial + (2 * c0 + 1) * C::kPartFloats;
-            const int tok = row / group;
-            out = p.o + static_cast<long long>(token0 + tok) * p.o_token +
-                  static_cast<long long>(s.h * group + row - tok * group) * p.o_head + lane * E;
-        }
-    }
-    grid_dependency_wait();
-    if (count == 0) return;
-    auto part = [&](int i) { return i == 0 ? first : first + i * kNext - C::kPartFloats; };
+    const Merge merge = p.merges[cta];
+    const int group = p.plan.heads / p.plan.kv_heads, lane = threadIdx.x % 32;
+    if (row >= merge.tokens * group || merge.parts == 0) return;
+    const float* first = p.partial + (2LL * cta + 1) * C::kPartFloats;
+    auto part = [&](int i) { return i == 0 ? first : first + (2LL * i - 1) * C::kPartFloats; };
     // 32 parts at a time: a lane reads one part's maximum and sum, then all lanes add up its columns.
     float top = -INFINITY, sum = 0.0f, acc[E] = {};
-    for (int i0 = 0; i0 < count; i0 += 32) {
+    for (int i0 = 0; i0 < merge.parts; i0 += 32) {
         const int mine = i0 + lane;
-        const float m = mine < count ? part(mine)[16 * MT * D + row] : -INFINITY;
-        const float l = mine < count ? part(mine)[16 * MT * D + 16 * MT + row] : 0.0f;
+        const float m = mine < merge.parts ? part(mine)[16 * MT * D + row] : -INFINITY;
+        const float l = mine < merge.parts ? part(mine)[16 * MT * D + 16 * MT + row] : 0.0f;
         float high = fmaxf(m, top);
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
@@ -1247,7 +1250,7 @@ __device__ __forceinline__ void combine_narrow(const PagedParams& p, int ctas, i
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] *= keep;
         top = high;
-        const int here = min(32, count - i0);
+        const int here = min(32, merge.parts - i0);
 #pragma unroll 8
         for (int i = 0; i < here; ++i) {
             const float wi = __shfl_sync(0xffffffffu, w, i);
@@ -1266,6 +1269,9 @@ __device__ __forceinline__ void combine_narrow(const PagedParams& p, int ctas, i
         }
     }
     const float inv = 1.0f / sum;
+    const int tok = row / group;
+    __nv_bfloat16* out = p.o + static_cast<long long>(merge.token0 + tok) * p.o_token +
+                         static_cast<long long>(merge.head0 + row - tok * group) * p.o_head + lane * E;
 #pragma unroll
     for (int e = 0; e < E; e += 2)
         *reinterpret_cast<uint32_t*>(out + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
@@ -1273,35 +1279,22 @@ __device__ __forceinline__ void combine_narrow(const PagedParams& p, int ctas, i
 
 // A thread is a query row and takes 32 columns (group c) of Q tile t.
 template <int D>
-__device__ __forceinline__ void combine_wide(const PagedParams& p, int ctas, int border_index, int t, int c)
+__device__ __forceinline__ void combine_wide(const PagedParams& p, int cta, int t, int c)
 {
     using C = WideCfg<D>;
-    const FaPagedPlan& plan = p.plan;
-    const long long* start = wide_starts(plan.schedule, plan.num_seqs);
-    const long long total = start[plan.num_seqs] * plan.kv_heads;
-    const long long share = wide_share(total, ctas);
-    const long long border = share * (border_index + 1);
-    const int group = plan.heads / plan.kv_heads, per_tile = tokens_per_tile(group);
-    const int r = threadIdx.x % kWideRows;
-    const int tok = t * per_tile + r / group;
-    WideSegment s;
-    bool merges = false;
-    if (border < total) {
-        s = wide_segment(plan, start, border, total);
-        merges = s.first < border && s.first >= border - share && r < per_tile * group && tok < s.tokens;
-    }
-    grid_dependency_wait();
-    if (!merges) return;
-    const long long c0 = s.first / share, c1 = (s.last - 1) / share;
-    auto part = [&](long long cta) {
-        return p.wide_partial + ((2 * cta + (cta == c0 ? 1 : 0)) * 2 + t) * C::kPartTileFloats;
-    };
+    const Merge merge = p.wide_merges[cta];
+    const int group = p.plan.heads / p.plan.kv_heads, per_tile = tokens_per_tile(group);
+    const int r = threadIdx.x, tok = t * per_tile + r / group;
+    if (merge.parts == 0 || r >= per_tile * group || tok >= merge.tokens) return;
+    const float* first = p.wide_partial + ((2LL * cta + 1) * 2 + t) * C::kPartTileFloats;
+    auto part = [&](int i) { return i == 0 ? first : first + (2LL * i - 1) * 2 * C::kPartTileFloats; };
     float top = -INFINITY;
-    for (long long cta = c0; cta <= c1; ++cta) top = fmaxf(top, part(cta)[D * kWideRows + r]);
+#pragma unroll 4
+    for (int i = 0; i < merge.parts; ++i) top = fmaxf(top, part(i)[D * kWideRows + r]);
     float4 acc[8] = {};
     float sum = 0.0f;
-    for (long long cta = c0; cta <= c1; ++cta) {
-        const float* at = part(cta);
+    for (int i = 0; i < merge.parts; ++i) {
+        const float* at = part(i);
         const float m = at[D * kWideRows + r];
         const float w = m == -INFINITY ? 0.0f : ex2_approx((m - top) * p.scale_log2);
         sum += w * at[D * kWideRows + kWideRows + r];
@@ -1316,8 +1309,8 @@ __device__ __forceinline__ void combine_wide(const PagedParams& p, int ctas, int
         }
     }
     const float inv = 1.0f / sum;
-    __nv_bfloat16* out = p.o + static_cast<long long>(s.token0 + tok) * p.o_token +
-                         static_cast<long long>(s.h * group + r % group) * p.o_head + c * 32;
+    __nv_bfloat16* out = p.o + static_cast<long long>(merge.token0 + tok) * p.o_token +
+                         static_cast<long long>(merge.head0 + r % group) * p.o_head + c * 32;
 #pragma unroll
     for (int q = 0; q < 8; q += 2)
         *reinterpret_cast<uint4*>(out + q * 4) =
@@ -1325,20 +1318,20 @@ __device__ __forceinline__ void combine_wide(const PagedParams& p, int ctas, int
                        pack_bf16x2(acc[q + 1].x * inv, acc[q + 1].y * inv), pack_bf16x2(acc[q + 1].z * inv, acc[q + 1].w * inv));
 }
 
-// Blocks [0, narrow_blocks) serve the narrow kernel's borders, the others the wide kernel's.
+// Blocks of the wide kernel's CTAs (one per Q tile and 32 columns), then those of the narrow kernel's (one
+// per four rows). The last CTA's item ends with its range.
 template <int D, int MT>
 __global__ void __launch_bounds__(kCombineThreads)
-paged_combine_kernel(const __grid_constant__ PagedParams p, int narrow_ctas, int wide_ctas)
+paged_combine_kernel(const __grid_constant__ PagedParams p, int wide_blocks)
 {
-    const int narrow_blocks = narrow_ctas > 0 ? (narrow_ctas - 1) * MT : 0;
+    constexpr int kPieces = 2 * (D / 32), kRowBlocks = 16 * MT / (kCombineThreads / 32);
     const int block = static_cast<int>(blockIdx.x);
-    if (block < narrow_blocks) {
-        combine_narrow<D, MT>(p, narrow_ctas, block / MT, block % MT);
-    } else {
-        constexpr int kPieces = 2 * (D / 32), kPerBlock = kCombineThreads / kWideRows;
-        const int piece = (block - narrow_blocks) * kPerBlock + static_cast<int>(threadIdx.x) / kWideRows;
-        combine_wide<D>(p, wide_ctas, piece / kPieces, piece % kPieces / (D / 32), piece % (D / 32));
-    }
+    grid_dependency_wait();
+    if (block < wide_blocks)
+        combine_wide<D>(p, block / kPieces, block % kPieces / (D / 32), block % (D / 32));
+    else
+        combine_narrow<D, MT>(p, (block - wide_blocks) / kRowBlocks,
+                              (block - wide_blocks) % kRowBlocks * (kCombineThreads / 32) + static_cast<int>(threadIdx.x) / 32);
 }
 
 }  // namespace fa_sm100
@@ -1449,15 +1442,18 @@ int prepare_paged_device(int device)
 
 int narrow_ctas(int sms) { return kNarrowCtasPerSm * sms; }
 
-size_t narrow_workspace(int sms, const FaPagedPlan& plan)
+// Workspace: the parts, then the merges, of each kernel.
+size_t narrow_parts(int sms, const FaPagedPlan& plan)
 {
     return static_cast<size_t>(narrow_ctas(sms)) * 2 * narrow_rows(plan) * (plan.head_dim + 2) * sizeof(float);
 }
+size_t narrow_workspace(int sms, const FaPagedPlan& plan) { return narrow_parts(sms, plan) + narrow_ctas(sms) * sizeof(Merge); }
 
-size_t wide_workspace(int sms, int head_dim)
+size_t wide_parts(int sms, int head_dim)
 {
     return static_cast<size_t>(sms) * 2 * 2 * kWideRows * (head_dim + 2) * sizeof(float);
 }
+size_t wide_workspace(int sms, int head_dim) { return wide_parts(sms, head_dim) + sms * sizeof(Merge); }
 
 // Which kernels a plan's requests can need: decided from the sizes that the host knows.
 bool may_be_narrow(const FaPagedPlan& plan) { return plan.heads / plan.kv_heads <= narrow_rows(plan); }
@@ -1507,8 +1503,7 @@ struct PagedMaps {
     CUtensorMap narrow_k, narrow_v;
 };
 
-// The wide kernel, the narrow one (it needs nothing of the wide one, so it fills the SMs that fall idle), then
-// the merging of both kernels' parts.
+// The wide kernel, the narrow one, then the merging of both kernels' parts.
 template <int D, int MT>
 int launch_attention(const PagedMaps& maps, const PagedParams& params, bool wide, bool narrow, int sms, cudaStream_t stream)
 {
@@ -1518,11 +1513,12 @@ int launch_attention(const PagedMaps& maps, const PagedParams& params, bool wide
                         maps.wide_v, params);
     const int ctas = narrow ? narrow_ctas(sms) : 0;
     if (narrow && status == FA_STATUS_OK)
-        status = launch(paged_narrow_kernel<D, MT>, ctas, kNarrowThreads, NarrowCfg<D, MT>::kSmemBytes, wide, stream,
+        status = launch(paged_narrow_kernel<D, MT>, ctas, kNarrowThreads, NarrowCfg<D, MT>::kSmemBytes, false, stream,
                         maps.narrow_k, maps.narrow_v, params);
     if (status != FA_STATUS_OK) return status;
-    const int blocks = (narrow ? (ctas - 1) * MT : 0) + (wide ? (sms - 1) * 2 * (D / 32) * kWideRows / kCombineThreads : 0);
-    return launch(paged_combine_kernel<D, MT>, blocks, kCombineThreads, 0, true, stream, params, ctas, wide ? sms : 0);
+    const int wide_blocks = wide ? sms * 2 * (D / 32) : 0;
+    const int narrow_blocks = ctas * (16 * MT / (kCombineThreads / 32));
+    return launch(paged_combine_kernel<D, MT>, wide_blocks + narrow_blocks, kCombineThreads, 0, true, stream, params, wide_blocks);
 }
 
 }  // namespace
@@ -1585,6 +1581,7 @@ int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cac
     char* work = static_cast<char*>(workspace);
     if (wide) {
         params.wide_partial = reinterpret_cast<float*>(work);
+        params.wide_merges = reinterpret_cast<Merge*>(work + wide_parts(sms, plan->head_dim));
         work += wide_workspace(sms, plan->head_dim);
         const int group = plan->heads / plan->kv_heads;
         const cuuint64_t dims[3] = {static_cast<cuuint64_t>(plan->head_dim), static_cast<cuuint64_t>(plan->heads),
@@ -1597,6 +1594,7 @@ int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cac
     }
     if (narrow) {
         params.partial = reinterpret_cast<float*>(work);
+        params.merges = reinterpret_cast<Merge*>(work + narrow_parts(sms, *plan));
         if (wide && plan->page_size <= kNarrowKeys) {       // the same boxes
             maps.narrow_k = maps.wide_k;
             maps.narrow_v = maps.wide_v;

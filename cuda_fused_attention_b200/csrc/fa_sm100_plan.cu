@@ -226,16 +226,18 @@ plan_kernel(const PlanParams p)
 // =============================================================================
 // Rotary positions, and the append of K and V
 // =============================================================================
-// A CTA serves a few neighbouring tokens: it first computes their angles' sines and cosines, once
-// for all heads, into shared memory, then streams the tokens' rows in units of eight pairs (two
-// 16-byte accesses), each element read once and written once; memory bounds it. An angle is a
-// position times a frequency; far positions need more than 24 bits of it, so the product is taken
-// in turns (1 / 2 pi) in 64 bits, its whole turns dropped there, and only the rest goes to
-// sincospif.
+// Every element is read once and written once, in units of eight pairs (two 16-byte accesses); memory
+// bounds it once there is enough of it. An angle is a position times a frequency; far positions need
+// more than 24 bits of it, so the product is taken in turns (1 / 2 pi) in 64 bits, its whole turns
+// dropped there, and only the rest goes to sincospif. That costs more than a unit's rotation, so
+// angles are shared by the heads, in one of two ways:
+//   rotary_kernel      a CTA serves a few neighbouring tokens; their angles go through shared memory
+//   rotary_long_kernel a thread keeps the angles of one token's unit in registers and walks over
+//                      heads; neighbouring threads take neighbouring tokens, so that each head of a
+//                      [heads, tokens] tensor is read in long runs
 constexpr int kRotaryThreads = 256;
 constexpr int kMaxAxes = 4;
-constexpr int kMaxTokensPerCta = 8;     // tokens that share a CTA
-constexpr int kRotaryBatch = 4;         // units a thread has in flight
+constexpr int kMaxTokensPerCta = 4;     // tokens that share a CTA of rotary_kernel
 
 struct RotaryParams {
     const __nv_bfloat16* src[3];        // q, k, v (x alone: q)
@@ -246,7 +248,8 @@ struct RotaryParams {
     int rows[3];                        // heads of each
     int batch, tokens;
     int unit_shift;                     // log2 of the 16-element units per row
-    int group_shift;
+    int group_shift;                    // rotary_kernel: log2 of the tokens per CTA
+    int head_split;                     // rotary_long_kernel: threads that share a token's heads
     int rotary_dim;
     const int* positions;
     long long position_axis, position_batch;
@@ -279,11 +282,53 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8])
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// (cos, sin) of a token's pair.
+__device__ __forceinline__ float2 rotary_angle(const RotaryParams& p, int batch, int token, int pair)
+{
+    int axis = 0;
+#pragma unroll
+    for (int a = 0; a < kMaxAxes - 1; ++a) axis += pair >= p.section_end[a] ? 1 : 0;
+    const int position = p.positions[axis * p.position_axis + batch * p.position_batch + token];
+    const double around = static_cast<double>(position) * static_cast<double>(p.inv_freq[pair]) * 0.15915494309189533577;
+    float sine, cosine;
+    sincospif(2.0f * static_cast<float>(around - rint(around)), &sine, &cosine);
+    return make_float2(cosine, p.sign * sine);
+}
+
+// A unit's eight pairs turned: x0 and x1 are its two pieces, turn(i) the (cos, sin) of its pairs 2i and 2i + 1.
+template <bool kInterleaved, typename Turn>
+__device__ __forceinline__ void rotate_unit(uint4& x0, uint4& x1, Turn&& turn)
+{
+    float a[8], b[8], u[8], w[8];
+    unpack8(x0, a);
+    unpack8(x1, b);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float4 two = turn(i / 2);
+        if (kInterleaved) {
+            float(&v)[8] = i < 4 ? a : b;
+            float(&out)[8] = i < 4 ? u : w;
+            const int q = 2 * (i & 3);
+            out[q] = v[q] * two.x - v[q + 1] * two.y;
+            out[q + 1] = v[q + 1] * two.x + v[q] * two.y;
+            out[q + 2] = v[q + 2] * two.z - v[q + 3] * two.w;
+            out[q + 3] = v[q + 3] * two.z + v[q + 2] * two.w;
+        } else {
+            u[i] = a[i] * two.x - b[i] * two.y;
+            w[i] = b[i] * two.x + a[i] * two.y;
+            u[i + 1] = a[i + 1] * two.z - b[i + 1] * two.w;
+            w[i + 1] = b[i + 1] * two.z + a[i + 1] * two.w;
+        }
+    }
+    x0 = pack8(u);
+    x1 = pack8(w);
+}
+
 template <bool kAppend, bool kInterleaved>
-__global__ void __launch_bounds__(kRotaryThreads)
+__global__ void __launch_bounds__(kRotaryThreads, 6)
 rotary_kernel(const __grid_constant__ RotaryParams p)
 {
-    __shared__ float2 turn[kMaxTokensPerCta][64];       // (cos, sin) of each token's pairs
+    __shared__ __align__(16) float2 turn[kMaxTokensPerCta][64];
     __shared__ long long slots[kMaxTokensPerCta];
     const int group = 1 << p.group_shift;
     const int blocks_per_batch = (p.tokens + group - 1) >> p.group_shift;
@@ -294,16 +339,15 @@ rotary_kernel(const __grid_constant__ RotaryParams p)
 
     // An item is a unit of a row. Neighbouring threads take the units of a row, then the rows that are
     // neighbours in memory: the next head of a packed token, the next token of a [heads, tokens] tensor.
-    const int rotating = p.rotary_dim / 16;
     const int rows = p.rows[0] + (kAppend ? p.rows[1] + p.rows[2] : 0);
     const int total = (kAppend ? tokens : group) * rows << p.unit_shift;
     const int unit = threadIdx.x & ((1 << p.unit_shift) - 1);       // the same for all of a thread's items
-    const bool turns = unit < rotating;
+    const bool turns = unit < p.rotary_dim / 16;
     // The unit's two 8-element pieces: the two halves of its pairs, or 16 neighbours.
     const int lo = turns && !kInterleaved ? 8 * unit : 16 * unit;
     const int hi = turns && !kInterleaved ? pairs + 8 * unit : 16 * unit + 8;
-    // Token, head and tensor of an item; false: there is none.
-    auto locate = [&](int index, int& tok, int& head, int& which) -> bool {
+    int tok, head, which;           // of the item at hand
+    auto locate = [&](int index) -> bool {
         const int item = index >> p.unit_shift;
         which = 0;
         if (kAppend) {
@@ -317,21 +361,16 @@ rotary_kernel(const __grid_constant__ RotaryParams p)
         head = item >> p.group_shift;
         return index < total && tok < tokens;
     };
-    uint4 x0[kRotaryBatch], x1[kRotaryBatch];
-    auto load = [&](int first) {
-#pragma unroll
-        for (int k = 0; k < kRotaryBatch; ++k) {
-            int tok, head, which;
-            if (!locate(first + k * kRotaryThreads, tok, head, which)) continue;
-            const __nv_bfloat16* src = p.src[which] + batch * p.src_batch + (token0 + tok) * p.src_token[which] +
-                                       head * p.src_head[which];
-            x0[k] = *reinterpret_cast<const uint4*>(src + (which == 2 ? 16 * unit : lo));
-            x1[k] = *reinterpret_cast<const uint4*>(src + (which == 2 ? 16 * unit + 8 : hi));
-        }
+    uint4 x0, x1;
+    auto load = [&]() {
+        const __nv_bfloat16* src = p.src[which] + batch * p.src_batch + (token0 + tok) * p.src_token[which] +
+                                   head * p.src_head[which];
+        x0 = *reinterpret_cast<const uint4*>(src + (which == 2 ? 16 * unit : lo));
+        x1 = *reinterpret_cast<const uint4*>(src + (which == 2 ? 16 * unit + 8 : hi));
     };
 
     // The first rows are on their way while the angles are computed.
-    load(threadIdx.x);
+    if (locate(threadIdx.x)) load();
     if (kAppend && threadIdx.x < tokens) {
         long long slot = p.slots[token0 + threadIdx.x];
         if (slot >= p.num_slots) {
@@ -340,62 +379,60 @@ rotary_kernel(const __grid_constant__ RotaryParams p)
         }
         slots[threadIdx.x] = slot;
     }
-    for (int i = threadIdx.x; i < tokens * pairs; i += kRotaryThreads) {
-        const int tok = i / pairs, pair = i - tok * pairs;
-        int axis = 0;
-#pragma unroll
-        for (int a = 0; a < kMaxAxes - 1; ++a) axis += pair >= p.section_end[a] ? 1 : 0;
-        const int position = p.positions[axis * p.position_axis + batch * p.position_batch + token0 + tok];
-        const double around = static_cast<double>(position) * static_cast<double>(p.inv_freq[pair]) * 0.15915494309189533577;
-        float sine, cosine;
-        sincospif(2.0f * static_cast<float>(around - rint(around)), &sine, &cosine);
-        turn[tok][pair] = make_float2(cosine, p.sign * sine);
-    }
+    for (int i = threadIdx.x; i < tokens * pairs; i += kRotaryThreads)
+        turn[i / pairs][i % pairs] = rotary_angle(p, batch, token0 + i / pairs, i % pairs);
     __syncthreads();
 
-    for (int first = threadIdx.x; first < total; first += kRotaryBatch * kRotaryThreads) {
-        if (first != threadIdx.x) load(first);
-#pragma unroll
-        for (int k = 0; k < kRotaryBatch; ++k) {
-            int tok, head, which;
-            if (!locate(first + k * kRotaryThreads, tok, head, which)) continue;
-            const long long slot = kAppend ? slots[tok] : 0;
-            if (slot < 0) continue;
-            const bool copied = kAppend && which == 2;
-            if (turns && !copied) {
-                const float4* cs = reinterpret_cast<const float4*>(&turn[tok][8 * unit]);
-                float a[8], b[8], u[8], w[8];
-                unpack8(x0[k], a);
-                unpack8(x1[k], b);
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const float4 two = cs[i / 2];       // cos, sin of pairs i and i + 1
-                    if (kInterleaved) {
-                        float(&v)[8] = i < 4 ? a : b;
-                        float(&out)[8] = i < 4 ? u : w;
-                        const int q = 2 * (i & 3);
-                        out[q] = v[q] * two.x - v[q + 1] * two.y;
-                        out[q + 1] = v[q + 1] * two.x + v[q] * two.y;
-                        out[q + 2] = v[q + 2] * two.z - v[q + 3] * two.w;
-                        out[q + 3] = v[q + 3] * two.z + v[q + 2] * two.w;
-                    } else {
-                        u[i] = a[i] * two.x - b[i] * two.y;
-                        w[i] = b[i] * two.x + a[i] * two.y;
-                        u[i + 1] = a[i + 1] * two.z - b[i + 1] * two.w;
-                        w[i + 1] = b[i + 1] * two.z + a[i + 1] * two.w;
-                    }
-                }
-                x0[k] = pack8(u);
-                x1[k] = pack8(w);
-            }
-            __nv_bfloat16* dst = p.dst[which] + head * p.dst_head[which];
-            if (kAppend && which > 0)
-                dst += (slot >> p.page_shift) * p.dst_page[which] + (slot & ((1LL << p.page_shift) - 1)) * p.dst_token[which];
-            else
-                dst += batch * p.dst_batch + (token0 + tok) * p.dst_token[which];
-            *reinterpret_cast<uint4*>(dst + (copied ? 16 * unit : lo)) = x0[k];
-            *reinterpret_cast<uint4*>(dst + (copied ? 16 * unit + 8 : hi)) = x1[k];
+    for (int index = threadIdx.x; index < total; index += kRotaryThreads) {
+        if (!locate(index)) continue;
+        const long long slot = kAppend ? slots[tok] : 0;
+        if (slot < 0) continue;
+        if (index != threadIdx.x) load();
+        const bool copied = kAppend && which == 2;
+        if (turns && !copied) {
+            const float4* cs = reinterpret_cast<const float4*>(&turn[tok][8 * unit]);
+            rotate_unit<kInterleaved>(x0, x1, [&](int i) { return cs[i]; });
         }
+        __nv_bfloat16* dst = p.dst[which] + head * p.dst_head[which];
+        if (kAppend && which > 0)
+            dst += (slot >> p.page_shift) * p.dst_page[which] + (slot & ((1LL << p.page_shift) - 1)) * p.dst_token[which];
+        else
+            dst += batch * p.dst_batch + (token0 + tok) * p.dst_token[which];
+        *reinterpret_cast<uint4*>(dst + (copied ? 16 * unit : lo)) = x0;
+        *reinterpret_cast<uint4*>(dst + (copied ? 16 * unit + 8 : hi)) = x1;
+    }
+}
+
+template <bool kInterleaved>
+__global__ void __launch_bounds__(kRotaryThreads)
+rotary_long_kernel(const __grid_constant__ RotaryParams p)
+{
+    const long long index = static_cast<long long>(blockIdx.x) * kRotaryThreads + threadIdx.x;
+    const int unit = static_cast<int>(index) & ((1 << p.unit_shift) - 1);
+    const long long all = static_cast<long long>(p.tokens) * p.batch, rest = index >> p.unit_shift;
+    const int part = static_cast<int>(rest / all);
+    if (part >= p.head_split) return;
+    const long long flat = rest - part * all;
+    const int batch = static_cast<int>(flat / p.tokens), token = static_cast<int>(flat - static_cast<long long>(batch) * p.tokens);
+    const int pairs = p.rotary_dim / 2;
+    const bool turns = unit < p.rotary_dim / 16;
+    const int lo = turns && !kInterleaved ? 8 * unit : 16 * unit;
+    const int hi = turns && !kInterleaved ? pairs + 8 * unit : 16 * unit + 8;
+    float4 cs[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (!turns) break;
+        const float2 even = rotary_angle(p, batch, token, 8 * unit + 2 * i), odd = rotary_angle(p, batch, token, 8 * unit + 2 * i + 1);
+        cs[i] = make_float4(even.x, even.y, odd.x, odd.y);
+    }
+    const __nv_bfloat16* src = p.src[0] + batch * p.src_batch + token * p.src_token[0];
+    __nv_bfloat16* dst = p.dst[0] + batch * p.dst_batch + token * p.dst_token[0];
+    for (int head = part; head < p.rows[0]; head += p.head_split) {
+        uint4 x0 = *reinterpret_cast<const uint4*>(src + head * p.src_head[0] + lo);
+        uint4 x1 = *reinterpret_cast<const uint4*>(src + head * p.src_head[0] + hi);
+        if (turns) rotate_unit<kInterleaved>(x0, x1, [&](int i) { return cs[i]; });
+        *reinterpret_cast<uint4*>(dst + head * p.dst_head[0] + lo) = x0;
+        *reinterpret_cast<uint4*>(dst + head * p.dst_head[0] + hi) = x1;
     }
 }
 
@@ -430,6 +467,9 @@ int fill_sections(RotaryParams& params, const int* sections, int axes, int rotar
     return end == rotary_dim / 2 ? FA_STATUS_OK : FA_STATUS_INVALID_ARGUMENT;
 }
 
+// Units of one head per SM from which rotary_embed takes the long kernel.
+constexpr long long kLongUnits = 512;
+
 template <bool kAppend>
 int launch_rotary(RotaryParams& params, bool interleaved, cudaStream_t stream)
 {
@@ -439,14 +479,24 @@ int launch_rotary(RotaryParams& params, bool interleaved, cudaStream_t stream)
     const long long tokens = static_cast<long long>(params.tokens) * params.batch;
     const int rows = params.rows[0] + (kAppend ? params.rows[1] + params.rows[2] : 0);
     if (tokens == 0 || rows == 0) return FA_STATUS_OK;
+    if (tokens > INT_MAX || (static_cast<long long>(rows) << 7) > INT_MAX) return FA_STATUS_INVALID_ARGUMENT;
+    const long long units = tokens << params.unit_shift;        // of one head
+    if (!kAppend && units >= kLongUnits * static_cast<long long>(sms)) {
+        // Heads are shared out until the threads fill the GPU once (2048 per SM).
+        const long long split = (2048LL * sms + units - 1) / units;
+        params.head_split = static_cast<int>(split < rows ? split : rows);
+        const long long blocks = ceil_div(units * params.head_split, kRotaryThreads);
+        if (blocks > INT_MAX) return FA_STATUS_INVALID_ARGUMENT;
+        if (interleaved) rotary_long_kernel<true><<<static_cast<unsigned>(blocks), kRotaryThreads, 0, stream>>>(params);
+        else rotary_long_kernel<false><<<static_cast<unsigned>(blocks), kRotaryThreads, 0, stream>>>(params);
+        return static_cast<int>(cudaGetLastError());
+    }
     // Tokens share a CTA (and its set-up) once the CTAs would fill the GPU without it, four per SM.
     params.group_shift = 0;
     while ((2 << params.group_shift) <= kMaxTokensPerCta && (tokens >> (params.group_shift + 1)) >= 4LL * sms)
         ++params.group_shift;
-    const long long per_batch = ceil_div(params.tokens, 1LL << params.group_shift);
-    const long long blocks = per_batch * params.batch;
-    if (blocks > INT_MAX || per_batch << params.group_shift > INT_MAX || (static_cast<long long>(rows) << 7) > INT_MAX)
-        return FA_STATUS_INVALID_ARGUMENT;
+    const long long blocks = ceil_div(params.tokens, 1LL << params.group_shift) * params.batch;
+    if (blocks > INT_MAX) return FA_STATUS_INVALID_ARGUMENT;
     if (interleaved) rotary_kernel<kAppend, true><<<static_cast<unsigned>(blocks), kRotaryThreads, 0, stream>>>(params);
     else rotary_kernel<kAppend, false><<<static_cast<unsigned>(blocks), kRotaryThreads, 0, stream>>>(params);
     return static_cast<int>(cudaGetLastError());
