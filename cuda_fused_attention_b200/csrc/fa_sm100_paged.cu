@@ -54,7 +54,7 @@ constexpr float kRebase = 16.0f;
 // D = 128 against 32 * 4 * 128 operations. The work of all requests and K/V heads is one line of
 // 64-key tiles (request, then head, then key; each item preceded by kNarrowGap idle units that stand
 // for its set-up), and each of the grid's CTAs (two per SM) takes an equal stretch of it, whatever the
-// requests' lengths: an item that crosses a border is merged from parts (paged_combine_kernel). A
+// requests' lengths: an item that crosses a border is merged from parts (paged_combine_narrow_kernel). A
 // CTA's warp 4 streams the tiles by TMA through a ring that runs on across items, page by page (a page
 // that is absent reads as zeros), with each item's Q and description ahead of its first tile; warps
 // 0-3 share out the keys of every tile (and the two 16-row tiles, if MT, their number, is 2), S = Q K^T
@@ -184,6 +184,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     grid_dependents_launch();
     if (begin >= total) {
         if (threadIdx.x == 0) p.merges[blockIdx.x] = Merge{};
+        grid_dependency_wait();
         return;
     }
     const long long end = begin + share < total ? begin + share : total;
@@ -305,6 +306,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 drain_paged(item_full(i % C::kQSlots), (i / C::kQSlots) & 1);
         }
         if (lane == 0) p.merges[blockIdx.x] = merge;
+        grid_dependency_wait();     // what was launched before this kernel is done when this one is
         return;
     }
 
@@ -611,10 +613,11 @@ struct WideSegment {
 };
 static_assert(sizeof(WideSegment) == 64, "segment slots");
 
+// For one warp, all lanes with the same arguments.
 __device__ inline WideSegment wide_segment(const FaPagedPlan& plan, const long long* start, long long x, long long end)
 {
     WideSegment s;
-    s.b = find_request(start, plan.num_seqs, x / plan.kv_heads);
+    s.b = find_request_warp(start, plan.num_seqs, x / plan.kv_heads);
     const long long tiles = start[s.b + 1] - start[s.b], base = start[s.b] * plan.kv_heads;
     s.h = static_cast<int>((x - base) / tiles);
     const long long head_first = base + s.h * tiles;
@@ -940,12 +943,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(C::kBarKvFull + slot));
             }
-        } else if (lane == 0) {
+        } else {
             // ======================= the walk along the line ===================
             long long x = begin;
             Merge merge{};
             for (int sg = 0;; ++sg) {
-                if (sg > 1 && !wait_paged(bar(C::kBarSchedEmpty + (sg & 1)), ((sg >> 1) - 1) & 1, abort_flag, kSiteWideSched))
+                if (sg > 1 && !__all_sync(0xffffffffu, wait_paged(bar(C::kBarSchedEmpty + (sg & 1)), ((sg >> 1) - 1) & 1,
+                                                                  abort_flag, kSiteWideSched)))
                     break;
                 WideSegment s;
                 s.count = 0;
@@ -966,11 +970,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                                  s.h * group};
                     x = s.first + s.tile + s.count;
                 }
-                segments[sg & 1] = s;
-                mbar_arrive(bar(C::kBarSchedFull + (sg & 1)));
+                if (lane == 0) {
+                    segments[sg & 1] = s;
+                    mbar_arrive(bar(C::kBarSchedFull + (sg & 1)));
+                }
                 if (s.count == 0) break;
             }
-            p.wide_merges[blockIdx.x] = merge;
+            if (lane == 0) p.wide_merges[blockIdx.x] = merge;
         }
         __syncwarp();
     } else {
@@ -1069,8 +1075,8 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 reg_fence32(sc[1]);
                 reg_fence32(sc[2]);
                 reg_fence32(sc[3]);
-                if (j >= mask_from) {
-                    const int key0 = (tile + j) * kWideKeys;
+                const int key0 = (tile + j) * kWideKeys;
+                if (j >= mask_from && __any_sync(0xffffffffu, limit < key0 + kWideKeys - 1)) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -1318,20 +1324,27 @@ __device__ __forceinline__ void combine_wide(const PagedParams& p, int cta, int 
                        pack_bf16x2(acc[q + 1].x * inv, acc[q + 1].y * inv), pack_bf16x2(acc[q + 1].z * inv, acc[q + 1].w * inv));
 }
 
-// Blocks of the wide kernel's CTAs (one per Q tile and 32 columns), then those of the narrow kernel's (one
-// per four rows). The last CTA's item ends with its range.
+// A block per CTA of the wide kernel, Q tile and 32 columns.
+template <int D>
+__global__ void __launch_bounds__(kCombineThreads)
+paged_combine_wide_kernel(const __grid_constant__ PagedParams p)
+{
+    constexpr int kPieces = 2 * (D / 32);
+    const int block = static_cast<int>(blockIdx.x);
+    grid_dependents_launch();
+    grid_dependency_wait();
+    combine_wide<D>(p, block / kPieces, block % kPieces / (D / 32), block % (D / 32));
+}
+
+// A block per CTA of the narrow kernel and four rows.
 template <int D, int MT>
 __global__ void __launch_bounds__(kCombineThreads)
-paged_combine_kernel(const __grid_constant__ PagedParams p, int wide_blocks)
+paged_combine_narrow_kernel(const __grid_constant__ PagedParams p)
 {
-    constexpr int kPieces = 2 * (D / 32), kRowBlocks = 16 * MT / (kCombineThreads / 32);
+    constexpr int kWarps = kCombineThreads / 32, kRowBlocks = 16 * MT / kWarps;
     const int block = static_cast<int>(blockIdx.x);
     grid_dependency_wait();
-    if (block < wide_blocks)
-        combine_wide<D>(p, block / kPieces, block % kPieces / (D / 32), block % (D / 32));
-    else
-        combine_narrow<D, MT>(p, (block - wide_blocks) / kRowBlocks,
-                              (block - wide_blocks) % kRowBlocks * (kCombineThreads / 32) + static_cast<int>(threadIdx.x) / 32);
+    combine_narrow<D, MT>(p, block / kRowBlocks, block % kRowBlocks * kWarps + static_cast<int>(threadIdx.x) / 32);
 }
 
 }  // namespace fa_sm100
@@ -1503,22 +1516,25 @@ struct PagedMaps {
     CUtensorMap narrow_k, narrow_v;
 };
 
-// The wide kernel, the narrow one, then the merging of both kernels' parts.
+// The wide kernel and the merging of its parts, then the narrow kernel and the merging of its own. The narrow
+// kernel needs nothing of the wide one: it fills the SMs that fall idle and runs beside the merging.
 template <int D, int MT>
 int launch_attention(const PagedMaps& maps, const PagedParams& params, bool wide, bool narrow, int sms, cudaStream_t stream)
 {
     int status = FA_STATUS_OK;
-    if (wide)
+    if (wide) {
         status = launch(paged_wide_kernel<D>, sms, kWideThreads, WideCfg<D>::kSmemBytes, false, stream, maps.q, maps.wide_k,
                         maps.wide_v, params);
-    const int ctas = narrow ? narrow_ctas(sms) : 0;
-    if (narrow && status == FA_STATUS_OK)
-        status = launch(paged_narrow_kernel<D, MT>, ctas, kNarrowThreads, NarrowCfg<D, MT>::kSmemBytes, false, stream,
-                        maps.narrow_k, maps.narrow_v, params);
+        if (status == FA_STATUS_OK)
+            status = launch(paged_combine_wide_kernel<D>, sms * 2 * (D / 32), kCombineThreads, 0, true, stream, params);
+    }
+    if (!narrow || status != FA_STATUS_OK) return status;
+    const int ctas = narrow_ctas(sms);
+    status = launch(paged_narrow_kernel<D, MT>, ctas, kNarrowThreads, NarrowCfg<D, MT>::kSmemBytes, wide, stream, maps.narrow_k,
+                    maps.narrow_v, params);
     if (status != FA_STATUS_OK) return status;
-    const int wide_blocks = wide ? sms * 2 * (D / 32) : 0;
-    const int narrow_blocks = ctas * (16 * MT / (kCombineThreads / 32));
-    return launch(paged_combine_kernel<D, MT>, wide_blocks + narrow_blocks, kCombineThreads, 0, true, stream, params, wide_blocks);
+    return launch(paged_combine_narrow_kernel<D, MT>, ctas * (16 * MT / (kCombineThreads / 32)), kCombineThreads, 0, true, stream,
+                  params);
 }
 
 }  // namespace

@@ -74,18 +74,6 @@ __host__ __device__ inline long long wide_units_through(long long blocks, long l
     return sum + blocks * kWideGap + (blocks > whole ? ceil_div(cached + n, kWideKeys) : 0);
 }
 
-// Last b in [0, num_seqs) with start[b] <= y, for start[0] = 0 <= y < start[num_seqs].
-__device__ inline int find_request(const long long* start, int num_seqs, long long y)
-{
-    int lo = 0, hi = num_seqs - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (start[mid] <= y) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
-}
-
 }  // namespace fa_sm100
 
 namespace fa_sm100_internal {
