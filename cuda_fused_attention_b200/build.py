@@ -12,6 +12,10 @@ NVIDIA driver at run time.
 The same sources compiled with FA_SM100_DEBUG_DUMP give lib/libfa_sm100_debug.so,
 whose kernel also dumps its intermediate tiles for layout checks
 (fa_sm100_debug_read); only tests load it.
+
+lib/_paged.so is the CPython binding of the paged-cache operators for torch tensors
+(csrc/paged_binding.cpp). It is the one part that is compiled against torch's headers
+and needs torch at run time; the two libraries above do not.
 """
 import os
 import shutil
@@ -24,6 +28,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libfa_sm100.so")
 DEBUG_LIB_PATH = os.path.join(LIB_DIR, "libfa_sm100_debug.so")
+BINDING_PATH = os.path.join(LIB_DIR, "_paged.so")
 SOURCES = ["fa_sm100.cu", "fa_sm100_host.cu", "fa_sm100_api.cu", "fa_sm100_static.cu",
            "fa_sm100_plan.cu", "fa_sm100_paged.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -43,10 +48,21 @@ def compile_command(output=LIB_PATH, extra=()):
             *extra, *srcs, "-o", output]
 
 
+def binding_command(output=BINDING_PATH):
+    import sysconfig
+    from torch.utils import cpp_extension
+    includes = [os.path.join(ROOT, "include"), *cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"]]
+    return ["g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden",
+            *(flag for path in includes for flag in ("-I", path)), os.path.join(CSRC, "paged_binding.cpp"),
+            *(flag for path in cpp_extension.library_paths("cuda") for flag in ("-L", path)),
+            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-ldl", "-o", output]
+
+
 def needs_build():
-    if not os.path.exists(LIB_PATH) or not os.path.exists(DEBUG_LIB_PATH):
+    outputs = (LIB_PATH, DEBUG_LIB_PATH, BINDING_PATH)
+    if not all(os.path.exists(path) for path in outputs):
         return True
-    lib_time = min(os.path.getmtime(LIB_PATH), os.path.getmtime(DEBUG_LIB_PATH))
+    lib_time = min(os.path.getmtime(path) for path in outputs)
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
     deps += [os.path.join(ROOT, "include", f) for f in os.listdir(os.path.join(ROOT, "include"))]
     return any(os.path.getmtime(d) > lib_time for d in deps)
@@ -59,7 +75,7 @@ def build(force=False, verbose=True, ptxas_verbose=False):
     os.makedirs(LIB_DIR, exist_ok=True)
     extra = ["-Xptxas", "-v"] if ptxas_verbose else []
     cmds = [compile_command(extra=extra),
-            compile_command(output=DEBUG_LIB_PATH, extra=["-DFA_SM100_DEBUG_DUMP"])]
+            compile_command(output=DEBUG_LIB_PATH, extra=["-DFA_SM100_DEBUG_DUMP"]), binding_command()]
     procs = []
     for cmd in cmds:
         if verbose:
@@ -73,7 +89,7 @@ def build(force=False, verbose=True, ptxas_verbose=False):
             sys.stderr.write(err)
         failed = failed or proc.returncode
     if failed:
-        raise RuntimeError(f"nvcc failed with exit code {failed}")
+        raise RuntimeError(f"the compiler failed with exit code {failed}")
     return LIB_PATH
 
 

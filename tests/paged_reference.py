@@ -2,12 +2,21 @@
 
 Tolerances count roundings: one to bf16 is off by at most 2^-8 of the value (half a step).
 """
+import ctypes
 import math
 
 import numpy as np
 import torch
 
 BF16_HALF_STEP = 2.0 ** -8
+
+
+class FaPagedPlan(ctypes.Structure):
+    """Layout of FaPagedPlan (include/fa_sm100_paged.h)."""
+    _fields_ = [(name, ctypes.c_int) for name in (
+        "num_seqs", "total_tokens", "max_new", "num_pages", "table_width", "table_stride", "heads", "kv_heads",
+        "head_dim", "page_size", "causal", "reserved")] + [(name, ctypes.c_void_p) for name in (
+            "query_start", "kv_lens", "positions", "slots", "block_table", "free_cursor", "schedule")]
 
 
 class Requests:

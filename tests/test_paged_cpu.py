@@ -1,12 +1,12 @@
 """Refusals of the paged-cache operators, made on the host before any CUDA call."""
 import ctypes
-import struct
 
 import pytest
 import torch
 
 import cuda_fused_attention_b200 as fa
 from cuda_fused_attention_b200 import _lib
+from paged_reference import FaPagedPlan
 
 
 @pytest.fixture(scope="module")
@@ -20,14 +20,6 @@ def _i32(*shape):
 
 def _bf16(*shape):
     return torch.zeros(shape, dtype=torch.bfloat16)
-
-
-class FaPagedPlan(ctypes.Structure):
-    """Layout of FaPagedPlan (include/fa_sm100_paged.h)."""
-    _fields_ = [(name, ctypes.c_int) for name in (
-        "num_seqs", "total_tokens", "max_new", "num_pages", "table_width", "table_stride", "heads", "kv_heads",
-        "head_dim", "page_size", "causal", "reserved")] + [(name, ctypes.c_void_p) for name in (
-            "query_start", "kv_lens", "positions", "slots", "block_table", "free_cursor", "schedule")]
 
 
 def _plan(**changes):
@@ -128,7 +120,8 @@ def test_python_refusals():
             (dict(block_table=_i32(4, 2).t()), ValueError), (dict(block_table=_i32(1, 4).expand(2, 4)), ValueError),
             (dict(free_pages=_i32(3).float()), TypeError), (dict(free_cursor=_i32(2)), ValueError),
             (dict(total_tokens=-1), ValueError), (dict(num_pages=-1), ValueError), (dict(max_new=-1), ValueError),
-            (dict(num_pages=2 ** 28), ValueError), (dict(total_tokens=2 ** 31), ValueError),
+            (dict(num_pages=2 ** 28), ValueError), (dict(total_tokens=2 ** 31), ValueError), (dict(num_pages=1.5), TypeError),
+            (dict(shape=(8, 2, 64)), TypeError),
             ({}, TypeError)]:        # CPU tensors: no silent CPU path
         with pytest.raises(error):
             fa.paged_plan(**{**good, **change})
@@ -145,7 +138,8 @@ def test_python_refusals():
             (dict(inv_freq=torch.ones(32).half()), TypeError), (dict(inv_freq=torch.ones(0)), ValueError),
             (dict(sections=(16, 15)), ValueError), (dict(sections=(16, 17)), ValueError),
             (dict(sections=(-1, 33)), ValueError), (dict(sections=()), ValueError),
-            (dict(sections=(8, 8, 8, 4, 4)), ValueError), ({}, TypeError)]:
+            (dict(sections=(8, 8, 8, 4, 4)), ValueError), (dict(sections=3), TypeError), (dict(x=3), TypeError),
+            ({}, TypeError)]:
         with pytest.raises(error):
             fa.rotary_embed(**{**good, **change})
 
@@ -161,8 +155,9 @@ def test_python_refusals():
         with pytest.raises(error):
             fa.rotary_append(**{**good, **change})
 
-    plan = fa.paged.PagedPlan(2, 5, shape, _i32(1))
-    plan.num_pages = 3
+    plan = fa.PagedPlan(shape, 2, 5)
+    struct = _plan(total_tokens=5, num_pages=3, heads=8, kv_heads=2, head_dim=64, page_size=16)
+    plan._filled((_i32(40), bytes(struct), 0, 0), _i32(2, 4), 3, True)
     good = dict(q=_bf16(5, 8, 64), k_cache=_bf16(3, 2, 16, 64), v_cache=_bf16(3, 2, 16, 64), plan=plan)
     for change, error in [
             (dict(q=_bf16(4, 8, 64)), ValueError), (dict(q=torch.zeros(5, 8, 64)), TypeError),
@@ -170,22 +165,6 @@ def test_python_refusals():
             (dict(v_cache=_bf16(3, 2, 16, 72)[..., 4:68]), ValueError), ({}, TypeError)]:
         with pytest.raises(error):
             fa.paged_attention(**{**good, **change})
-
-
-def test_plan_views_are_the_struct_s_pointers():
-    """The packed struct has the C layout, and the views are where its pointers say."""
-    plan = fa.paged.PagedPlan(3, 7, fa.PagedShape(8, 2, 64, 16), _i32(1))
-    table = _i32(3, 9)[:, :5]
-    plan._fill(table, 5, 9, 11, 6, 1)
-    c = FaPagedPlan.from_buffer_copy(plan.c)
-    assert len(plan.c) == ctypes.sizeof(FaPagedPlan) == struct.calcsize("12i7P")
-    assert [getattr(c, n) for n, _ in FaPagedPlan._fields_[:12]] == [3, 7, 6, 11, 5, 9, 8, 2, 64, 16, 1, 0]
-    for name, size in (("query_start", 4), ("kv_lens", 3), ("positions", 7), ("slots", 7), ("free_cursor", 1)):
-        view = getattr(plan, name)
-        assert view.data_ptr() == getattr(c, name) and view.shape == (size,) and view.dtype == torch.int32
-    assert c.block_table == table.data_ptr() and c.schedule == plan._buffer.data_ptr()
-    assert plan.free_cursor.data_ptr() + 4 == plan._buffer.data_ptr() + 4 * plan._buffer.numel()
-    assert c.query_start == c.schedule + _lib.load().fa_sm100_paged_schedule_bytes(3)
 
 
 def test_status_strings(lib):

@@ -1,11 +1,14 @@
 """Paged-cache operators on a B200 against plain 64-bit forms: plan, rotary positions, append, attention,
 and a run of them together."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import cuda_fused_attention_b200 as fa
-from paged_reference import Requests, attention, attention_bound, normal, rotary
+from cuda_fused_attention_b200 import _lib
+from paged_reference import FaPagedPlan, Requests, attention, attention_bound, normal, rotary
 
 pytestmark = pytest.mark.gpu
 
@@ -75,6 +78,24 @@ def test_plan_schedule(cuda_device, group, causal):
     units = np.array([_units(c, n, group, causal) for c, n in zip(cached, new)])
     want = np.concatenate([np.zeros((1, 2), np.int64), np.cumsum(units, 0)]).T.tolist()
     assert got == want
+
+
+def test_plan_views_are_the_struct_s_pointers(cuda_device):
+    """The struct that the C calls get has the C layout, and the views are where its pointers say."""
+    r = Requests([5, 40, 0], [1, 3, 7], 16, cuda_device)
+    plan = r.plan(fa.PagedShape(8, 2, 64, 16), max_new=9)
+    c = FaPagedPlan.from_buffer_copy(plan._struct)
+    assert len(plan._struct) == ctypes.sizeof(FaPagedPlan)
+    width = r.block_table.shape[1]
+    assert [getattr(c, n) for n, _ in FaPagedPlan._fields_[:12]] == [3, 11, 9, r.num_pages, width, width, 8, 2, 64, 16, 1, 0]
+    for name, size in (("query_start", 4), ("kv_lens", 3), ("positions", 11), ("slots", 11), ("free_cursor", 1)):
+        view = getattr(plan, name)
+        assert view.data_ptr() == getattr(c, name) and view.shape == (size,) and view.dtype == torch.int32
+    assert c.block_table == r.block_table.data_ptr() and c.schedule == plan._buffer.data_ptr()
+    assert plan.free_cursor.data_ptr() + 4 == plan._buffer.data_ptr() + 4 * plan._buffer.numel()
+    assert c.query_start == c.schedule + _lib.load().fa_sm100_paged_schedule_bytes(3)
+    with pytest.raises(ValueError):
+        r.plan(fa.PagedShape(8, 2, 128, 16), plan=plan)
 
 
 def test_plan_steps_through_the_free_list(cuda_device):
