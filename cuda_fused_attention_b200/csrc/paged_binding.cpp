@@ -326,7 +326,11 @@ PyObject* split(PyObject* const* args, Py_ssize_t count)
     PyObject* views = PyTuple_New(5);
     if (views == nullptr) return nullptr;
     for (int i = 0; i < 5; ++i) {
-        PyTuple_SET_ITEM(views, i, THPVariable_Wrap(buffer.narrow(0, from, sizes[i])));
+        // A tensor on the same storage (int32 views need no autograd record, which is most of narrow's cost).
+        at::Tensor view = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), buffer.dtype());
+        view.unsafeGetTensorImpl()->set_storage_offset(buffer.storage_offset() + from);
+        view.unsafeGetTensorImpl()->set_sizes_contiguous({sizes[i]});
+        PyTuple_SET_ITEM(views, i, THPVariable_Wrap(view));
         from += sizes[i];
     }
     return views;
