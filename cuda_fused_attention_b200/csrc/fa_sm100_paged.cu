@@ -129,39 +129,71 @@ __device__ __forceinline__ void drain_paged(uint32_t bar, uint32_t parity)
 
 enum PagedSite : uint32_t { kSiteNarrowFull = 32, kSiteNarrowEmpty = 33, kSiteNarrowItem = 34, kSiteNarrowItemFree = 35 };
 
-// Where x falls on the narrow line: the item's request and head, and its tiles' place [first, last).
-struct NarrowPlace {
-    int b, h;
-    long long first, last;
+// A request as the attention kernels see it: the units of one K/V head on the line, and its tokens and keys.
+struct Request {
+    int b;
+    long long start, units;
+    int token0, tokens, kv;
 };
 
-// For one warp, all lanes with the same arguments. 32 borders are read at a time, so a thousand
-// requests take two round trips to memory.
-__device__ __forceinline__ int find_request_warp(const long long* start, int num_seqs, long long y)
-{
-    const int lane = threadIdx.x % 32;
-    int lo = 0, count = num_seqs;           // the last b in [lo, lo + count) with start[b] <= y
-    while (count > 1) {
-        const int step = (count + 31) / 32;
-        const int at = lo + lane * step;
-        const bool below = lane * step < count && start[at] <= y;
-        const int last = 31 - __clz(static_cast<int>(__ballot_sync(0xffffffffu, below)));
-        lo += last * step;
-        count = min(step, count - last * step);
+// Finds requests by their place on the line, for one warp (all lanes with the same arguments). Up to 32 requests
+// are held in the lanes, loaded together when the kernel starts; with more, 32 borders are read at a time, so a
+// thousand requests take two round trips to memory.
+class RequestFinder {
+public:
+    __device__ __forceinline__ RequestFinder(const FaPagedPlan& plan, const long long* start)
+        : plan_(plan), start_(start), lane_(threadIdx.x % 32), held_(plan.num_seqs <= 32)
+    {
+        if (held_ && lane_ < plan.num_seqs) {
+            my_start_ = start[lane_];
+            my_end_ = start[lane_ + 1];
+            my_token0_ = plan.query_start[lane_];
+            my_tokens_ = plan.query_start[lane_ + 1] - my_token0_;
+            my_kv_ = plan.kv_lens[lane_];
+        }
     }
-    return lo;
-}
+    // The request whose units [start, start + units) hold y.
+    __device__ __forceinline__ Request find(long long y) const
+    {
+        Request r;
+        if (held_) {
+            r.b = last_of(lane_ < plan_.num_seqs && my_start_ <= y);
+            r.start = __shfl_sync(0xffffffffu, my_start_, r.b);
+            r.units = __shfl_sync(0xffffffffu, my_end_, r.b) - r.start;
+            r.token0 = __shfl_sync(0xffffffffu, my_token0_, r.b);
+            r.tokens = __shfl_sync(0xffffffffu, my_tokens_, r.b);
+            r.kv = __shfl_sync(0xffffffffu, my_kv_, r.b);
+            return r;
+        }
+        int lo = 0, count = plan_.num_seqs;         // the last request in [lo, lo + count) that begins at or before y
+        while (count > 1) {
+            const int step = (count + 31) / 32;
+            const int at = last_of(lane_ * step < count && start_[lo + lane_ * step] <= y);
+            lo += at * step;
+            count = min(step, count - at * step);
+        }
+        r.b = lo;
+        r.start = start_[lo];
+        r.units = start_[lo + 1] - r.start;
+        r.token0 = plan_.query_start[lo];
+        r.tokens = plan_.query_start[lo + 1] - r.token0;
+        r.kv = plan_.kv_lens[lo];
+        return r;
+    }
+    // The last lane for which the condition holds (it does for lane 0).
+    static __device__ __forceinline__ int last_of(bool condition)
+    {
+        return 31 - __clz(static_cast<int>(__ballot_sync(0xffffffffu, condition)));
+    }
 
-__device__ __forceinline__ NarrowPlace narrow_place(const FaPagedPlan& plan, const long long* start, long long x)
-{
-    NarrowPlace s;
-    s.b = find_request_warp(start, plan.num_seqs, x / plan.kv_heads);
-    const long long units = start[s.b + 1] - start[s.b], base = start[s.b] * plan.kv_heads;
-    s.h = static_cast<int>((x - base) / units);
-    s.first = base + s.h * units + kNarrowGap;
-    s.last = s.first - kNarrowGap + units;
-    return s;
-}
+private:
+    const FaPagedPlan& plan_;
+    const long long* start_;
+    const int lane_;
+    const bool held_;
+    long long my_start_ = 0, my_end_ = 0;
+    int my_token0_ = 0, my_tokens_ = 0, my_kv_ = 0;
+};
 
 // Units per CTA when `total` are shared out over `ctas`.
 __device__ __forceinline__ long long narrow_share(long long total, int ctas)
@@ -179,15 +211,9 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const FaPagedPlan& plan = p.plan;
     const long long* start = narrow_starts(plan.schedule, plan.num_seqs);
     const long long total = start[plan.num_seqs] * plan.kv_heads;
-    const long long share = narrow_share(total, gridDim.x);
-    const long long begin = share * blockIdx.x;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int group = plan.heads / plan.kv_heads;
     grid_dependents_launch();
-    if (begin >= total) {
-        if (threadIdx.x == 0) p.merges[blockIdx.x] = Merge{};
-        grid_dependency_wait();
-        return;
-    }
-    const long long end = begin + share < total ? begin + share : total;
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
@@ -200,8 +226,6 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     auto empty = [&](int s) -> uint32_t { return bar(C::kStages + s); };
     auto item_full = [&](int s) -> uint32_t { return bar(2 * C::kStages + s); };
     auto item_empty = [&](int s) -> uint32_t { return bar(2 * C::kStages + C::kQSlots + s); };
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int group = plan.heads / plan.kv_heads;
     if (warp == 0) {
         for (int i = lane; i < C::kNumBars; i += 32) {
             const bool released = (i >= C::kStages && i < 2 * C::kStages) || i >= 2 * C::kStages + C::kQSlots;
@@ -210,6 +234,15 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         if (lane == 0) *abort_flag = 0u;
         fence_mbarrier_init();
     }
+    const RequestFinder finder(plan, start);        // used by the producer
+    const long long share = narrow_share(total, gridDim.x);
+    const long long begin = share * blockIdx.x;
+    if (begin >= total) {
+        if (threadIdx.x == 0) p.merges[blockIdx.x] = Merge{};
+        grid_dependency_wait();
+        return;
+    }
+    const long long end = begin + share < total ? begin + share : total;
     __syncthreads();
 
     if (warp == kNarrowWarps) {
@@ -230,27 +263,30 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             NarrowItem item{};
             int b = 0, h = 0;
             if (x < end) {
-                const NarrowPlace s = narrow_place(plan, start, x);
-                if (x < s.first) x = s.first;
-                const long long stop = s.last < end ? s.last : end;
+                const Request r = finder.find(x / plan.kv_heads);
+                b = r.b;
+                h = static_cast<int>((x - r.start * plan.kv_heads) / r.units);
+                // The item's tiles lie at [first, last) of the line, behind its gap.
+                const long long first = r.start * plan.kv_heads + h * r.units + kNarrowGap;
+                const long long last = first - kNarrowGap + r.units;
+                if (x < first) x = first;
+                const long long stop = last < end ? last : end;
                 if (x >= stop) {                // only idle units are left of this range
-                    x = s.last;
+                    x = last;
                     continue;
                 }
-                b = s.b;
-                h = s.h;
-                item.token0 = plan.query_start[b];
-                item.tokens = plan.query_start[b + 1] - item.token0;
+                item.token0 = r.token0;
+                item.tokens = r.tokens;
                 item.head0 = h * group;
-                item.kv = plan.kv_lens[b];
-                item.tile = static_cast<int>(x - s.first);
+                item.kv = r.kv;
+                item.tile = static_cast<int>(x - first);
                 item.count = static_cast<int>(stop - x);
                 // An item that began before this CTA's range leaves its part in the CTA's first place, one that
                 // goes on behind it in the second.
-                item.part = s.first < begin ? 2 * static_cast<int>(blockIdx.x)
-                                            : s.last > end ? 2 * static_cast<int>(blockIdx.x) + 1 : -1;
-                if (s.first >= begin && s.last > end)
-                    merge = {static_cast<int>((s.last - 1) / share) - static_cast<int>(blockIdx.x) + 1, item.token0, item.tokens,
+                item.part = first < begin ? 2 * static_cast<int>(blockIdx.x)
+                                          : last > end ? 2 * static_cast<int>(blockIdx.x) + 1 : -1;
+                if (first >= begin && last > end)
+                    merge = {static_cast<int>((last - 1) / share) - static_cast<int>(blockIdx.x) + 1, item.token0, item.tokens,
                              item.head0};
                 x = stop;
             }
@@ -614,28 +650,32 @@ struct WideSegment {
 static_assert(sizeof(WideSegment) == 64, "segment slots");
 
 // For one warp, all lanes with the same arguments.
-__device__ inline WideSegment wide_segment(const FaPagedPlan& plan, const long long* start, long long x, long long end)
+__device__ inline WideSegment wide_segment(const FaPagedPlan& plan, const RequestFinder& finder, long long x, long long end)
 {
     WideSegment s;
-    s.b = find_request_warp(start, plan.num_seqs, x / plan.kv_heads);
-    const long long tiles = start[s.b + 1] - start[s.b], base = start[s.b] * plan.kv_heads;
-    s.h = static_cast<int>((x - base) / tiles);
-    const long long head_first = base + s.h * tiles;
-    const int n = plan.query_start[s.b + 1] - plan.query_start[s.b];
-    s.kv = plan.kv_lens[s.b];
+    const Request r = finder.find(x / plan.kv_heads);
+    s.b = r.b;
+    s.h = static_cast<int>((x - r.start * plan.kv_heads) / r.units);
+    const long long head_first = r.start * plan.kv_heads + s.h * r.units;
+    const int n = r.tokens;
+    s.kv = r.kv;
     const int cached = s.kv - n;
     const int span = 2 * tokens_per_tile(plan.heads / plan.kv_heads);
     const bool causal = plan.causal != 0;
-    int lo = 0, hi = (n - 1) / span;        // last block whose tiles begin at or before x
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (head_first + wide_units_through(mid, span, cached, n, causal) <= x) lo = mid;
-        else hi = mid - 1;
+    const int lane = threadIdx.x % 32;
+    int lo = 0, blocks = (n - 1) / span + 1;    // the last block in [lo, lo + blocks) whose units begin at or before x
+    while (blocks > 1) {
+        const int step = (blocks + 31) / 32;
+        const bool below = lane * step < blocks &&
+                           head_first + wide_units_through(lo + lane * step, span, cached, n, causal) <= x;
+        const int at = RequestFinder::last_of(below);
+        lo += at * step;
+        blocks = min(step, blocks - at * step);
     }
     s.first = head_first + wide_units_through(lo, span, cached, n, causal) + kWideGap;
     s.last = s.first + wide_tiles_of(lo, span, cached, n, causal);
     if (x < s.first) x = s.first;
-    s.token0 = plan.query_start[s.b] + lo * span;
+    s.token0 = r.token0 + lo * span;
     s.tokens = min(span, n - lo * span);
     s.pos0 = cached + lo * span;
     s.tile = static_cast<int>(x - s.first);
@@ -945,6 +985,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
         } else {
             // ======================= the walk along the line ===================
+            const RequestFinder finder(plan, start);
             long long x = begin;
             Merge merge{};
             for (int sg = 0;; ++sg) {
@@ -954,7 +995,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 WideSegment s;
                 s.count = 0;
                 while (x < end && s.count <= 0) {
-                    s = wide_segment(plan, start, x, end);
+                    s = wide_segment(plan, finder, x, end);
                     if (s.count <= 0) {
                         s.count = 0;
                         x = s.last;
