@@ -8,7 +8,6 @@
 #include <cmath>
 #include <cstdint>
 #include <mutex>
-#include <type_traits>
 
 #include "fa_sm100_internal.h"
 #include "fa_sm100_paged.cuh"
@@ -585,12 +584,12 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 // block overlap the epilogue of the one before.
 //
 // Warps: 0-3 and 4-7 softmax, O correction and epilogue of Q tile 0 and 1 (one thread per row);
-// 8 MMA issuer; 9 TMA producer; 10 zeroes what V's last page holds behind the last key (a weight
-// of zero does not silence a NaN); 11 walks the line and hands out the segments.
-// Tensor memory, barriers per key tile, register split and the lazily moved exponent base are
-// those of the dense kernel (fa_sm100.cu). P is rounded to bf16 for the product with V.
+// 8 MMA issuer; 9 and 10 TMA producers of Q and K and of V; 11 walks the line, hands out the segments,
+// and zeroes what V's last page holds behind the last key (a weight of zero does not silence a NaN).
+// Tensor memory, barriers per key tile and the lazily moved exponent base are those of the dense
+// kernel (fa_sm100.cu); a block of at most 128 rows has its S double-buffered. P is rounded to bf16 for the product with V.
 constexpr int kWideThreads = 384;
-constexpr int kWideMinTiles = 4;        // units a CTA takes at least
+constexpr int kWideMinUnits = 8;        // units a CTA takes at least, more than a tile's
 constexpr uint32_t kWideRegsLaunch = 168, kWideRegsSoftmax = 200, kWideRegsOther = 104;
 static_assert(2 * 128 * kWideRegsSoftmax + 128 * kWideRegsOther <= kWideThreads * kWideRegsLaunch,
               "the warpgroup register split must fit in the registers the CTA launches with");
@@ -610,10 +609,13 @@ struct WideCfg {
     static constexpr int kBarOff = kRingOff + kStages * kTileBytes;
     static constexpr int kBarQFull = 0, kBarQEmpty = 1;
     static constexpr int kBarKvFull = 2, kBarKvEmpty = 2 + kStages;
-    static constexpr int kBarSFull = 2 + 2 * kStages;           // per Q tile from here
-    static constexpr int kBarPHalf = kBarSFull + 2;
-    static constexpr int kBarPFull = kBarPHalf + 2;
-    static constexpr int kBarPvHalf = kBarPFull + 2;
+    // Three sets of S, P-half and P barriers: Q tile 0's (in a block of one Q tile, its even key tiles'), Q tile
+    // 1's, and that of the odd key tiles of a block of one Q tile. Q tile 1's are its own because a warpgroup that
+    // sits a block out must not have to follow their phases.
+    static constexpr int kBarSFull = 2 + 2 * kStages;
+    static constexpr int kBarPHalf = kBarSFull + 3;
+    static constexpr int kBarPFull = kBarPHalf + 3;
+    static constexpr int kBarPvHalf = kBarPFull + 3;            // per Q tile
     static constexpr int kBarOFull = kBarPvHalf + 2;
     static constexpr int kBarTail = kBarOFull + 2;              // per ring slot: a V tile to be zeroed in part has landed
     static constexpr int kBarDrain = kBarTail + kStages;
@@ -645,12 +647,15 @@ struct WideSegment {
     int part;               // place of its part, -1: the whole block, written directly
     int zero_from, zero_to; // rows of the last V tile that must read as zero ([0, 0): none)
     int reserved;
-    long long first, last;  // the block's tiles on the line
+    long long last;         // end of the block's units on the line
+    int parts;              // CTAs that share the block
+    int reserved2;
 };
 static_assert(sizeof(WideSegment) == 64, "segment slots");
 
 // For one warp, all lanes with the same arguments.
-__device__ inline WideSegment wide_segment(const FaPagedPlan& plan, const RequestFinder& finder, long long x, long long end)
+__device__ inline WideSegment wide_segment(const FaPagedPlan& plan, const RequestFinder& finder, long long x, long long end,
+                                           long long share)
 {
     WideSegment s;
     const Request r = finder.find(x / plan.kv_heads);
@@ -672,16 +677,22 @@ __device__ inline WideSegment wide_segment(const FaPagedPlan& plan, const Reques
         lo += at * step;
         blocks = min(step, blocks - at * step);
     }
-    s.first = head_first + wide_units_through(lo, span, cached, n, causal) + kWideGap;
-    s.last = s.first + wide_tiles_of(lo, span, cached, n, causal);
-    if (x < s.first) x = s.first;
+    // The block's tiles lie at first, first + weight, ... of the line; a CTA takes those that begin in its range.
+    const long long first = head_first + wide_units_through(lo, span, cached, n, causal) + kWideGap;
+    const int weight = wide_weight(lo, span, n);
+    const int tiles = static_cast<int>(wide_tiles_of(lo, span, cached, n, causal));
+    s.last = first + static_cast<long long>(weight) * tiles;
     s.token0 = r.token0 + lo * span;
     s.tokens = min(span, n - lo * span);
     s.pos0 = cached + lo * span;
-    s.tile = static_cast<int>(x - s.first);
-    s.count = static_cast<int>((s.last < end ? s.last : end) - x);     // 0 or less: only idle units are left before end
-    s.part = -1;
-    s.reserved = 0;
+    s.tile = x <= first ? 0 : static_cast<int>(ceil_div(x - first, weight));
+    const int stop = end >= s.last ? tiles : end <= first ? 0 : static_cast<int>(ceil_div(end - first, weight));
+    s.count = stop - s.tile;        // 0 or less: no tile of the block begins in the rest of the range
+    // A block whose first tile is another CTA's leaves its part in the CTA's first place, one whose last tile is
+    // another's in the second.
+    s.part = s.tile > 0 ? 0 : stop < tiles ? 1 : -1;
+    s.parts = static_cast<int>((first + static_cast<long long>(weight) * (tiles - 1)) / share - first / share) + 1;
+    s.reserved = s.reserved2 = 0;
     // Behind the last key: rows of the last page (pages behind it are zero-filled by the copy).
     const int v0 = (s.tile + s.count - 1) * kWideKeys;
     const int held = (s.kv + plan.page_size - 1) / plan.page_size * plan.page_size;
@@ -694,7 +705,7 @@ __device__ inline WideSegment wide_segment(const FaPagedPlan& plan, const Reques
 __device__ __forceinline__ long long wide_share(long long total, int ctas)
 {
     const long long even = (total + ctas - 1) / ctas;
-    return even > kWideMinTiles ? even : kWideMinTiles;
+    return even > kWideMinUnits ? even : kWideMinUnits;
 }
 
 // A matrix descriptor (fa_sm100_ptx.cuh) as its low word -- address and leading offset, which a step along
@@ -756,7 +767,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     WideSegment* segments = reinterpret_cast<WideSegment*>(smem + C::kSegOff);
     auto bar = [&](int index) -> uint32_t { return base + C::kBarOff + static_cast<uint32_t>(index) * 8u; };
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    constexpr int kMma = 8, kLoad = 9, kTail = 10;
+    constexpr int kMma = 8, kLoadK = 9, kLoadV = 10;
     constexpr int kReaders = 11;            // warps that read a segment slot
 
     if (warp == 0) {
@@ -791,16 +802,20 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 
     if (warp >= kMma) {
         regs_decrease<kWideRegsOther>();
-        if (warp == kLoad) {
-            // ======================= TMA producer ==============================
+        if (warp == kLoadK || warp == kLoadV) {
+            // ======================= TMA producers =============================
+            // One warp copies Q and K, one V: pages of 16 tokens make 32 boxes of a key tile, more than one warp
+            // can issue in the time of a tile. Ring slots alternate between K and V.
+            const int is_v = warp == kLoadV ? 1 : 0;
+            const void* map = is_v ? static_cast<const void*>(&tm_v) : static_cast<const void*>(&tm_k);
             const int rows = plan.page_size < kWideKeys ? plan.page_size : kWideKeys;
             const int pages = kWideKeys / rows;
             const bool active = lane < pages * C::kSub;
             const int page_of_tile = lane / C::kSub, block = lane % C::kSub;
             const uint32_t offset = static_cast<uint32_t>(block * C::kSubBytes + page_of_tile * rows * 128);
-            int ri = 0;                 // ring index of the next K or V tile
+            int ri = is_v;              // ring index of the next tile
             int q_loads = 0;
-            uint32_t tail_slots = 0, tail_parity = 0;      // slots whose latest load went by the tail warp; their phases
+            uint32_t tail_slots = 0, tail_parity = 0;      // slots whose latest load went by the tail barrier; their phases
             bool ok = true;
             for (int sg = 0; ok; ++sg) {
                 ok = await_segment(sg);
@@ -813,18 +828,20 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 const int* table = plan.block_table + static_cast<long long>(seg.b) * plan.table_stride;
                 release_segment(sg);
                 if (count == 0) break;
-                if (sg > 0 && !__all_sync(0xffffffffu, wait_paged(bar(C::kBarQEmpty), (sg - 1) & 1, abort_flag, kSiteWideQ))) {
-                    ok = false;
-                    break;
+                if (!is_v) {
+                    if (sg > 0 && !__all_sync(0xffffffffu, wait_paged(bar(C::kBarQEmpty), (sg - 1) & 1, abort_flag, kSiteWideQ))) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(bar(C::kBarQFull), static_cast<uint32_t>(tiles * C::kSub * 128 * group * per_tile));
+                        for (int t = 0; t < tiles; ++t)
+                            for (int sub = 0; sub < C::kSub; ++sub)
+                                tma_load_3d(base + t * C::kTileBytes + sub * C::kSubBytes, &tm_q, bar(C::kBarQFull), sub * 64,
+                                            head * group, token0 + t * per_tile);
+                    }
+                    ++q_loads;
                 }
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(bar(C::kBarQFull), static_cast<uint32_t>(tiles * C::kSub * 128 * group * per_tile));
-                    for (int t = 0; t < tiles; ++t)
-                        for (int sub = 0; sub < C::kSub; ++sub)
-                            tma_load_3d(base + t * C::kTileBytes + sub * C::kSubBytes, &tm_q, bar(C::kBarQFull), sub * 64,
-                                        head * group, token0 + t * per_tile);
-                }
-                ++q_loads;
                 auto page_at = [&](int tile) -> int {
                     // num_pages is out of the map's range: such a box reads as zeros.
                     const int i = ((tile * kWideKeys) >> p.page_shift) + page_of_tile;
@@ -835,33 +852,29 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     return plan.num_pages;
                 };
                 int page = page_at(first_tile);
-                for (int i = 0; ok && i < count; ++i) {
+                for (int i = 0; i < count; ++i, ri += 2) {
                     const int row = pages > 1 ? 0 : ((first_tile + i) * kWideKeys) & (plan.page_size - 1);
-                    for (int kv = 0; kv < 2; ++kv, ++ri) {
-                        const int slot = ri % C::kStages, use = ri / C::kStages;
-                        if (use > 0 && !__all_sync(0xffffffffu, wait_paged(bar(C::kBarKvEmpty + slot), (use - 1) & 1,
-                                                                           abort_flag, kSiteWideEmpty))) {
-                            ok = false;
-                            break;
-                        }
-                        // A V tile to be zeroed in part lands on the tail warp's barrier, and that warp then
-                        // completes the slot's.
-                        const bool tail = kv == 1 && i + 1 == count && has_tail;
-                        const uint32_t landed = bar((tail ? C::kBarTail : C::kBarKvFull) + slot);
-                        tail_slots = tail ? tail_slots | (1u << slot) : tail_slots & ~(1u << slot);
-                        if (tail) tail_parity ^= 1u << slot;
-                        if (lane == 0) mbar_arrive_expect_tx(landed, C::kTileBytes);
-                        __syncwarp();
-                        if (active)
-                            tma_load_4d(ring + slot * C::kTileBytes + offset, kv ? &tm_v : &tm_k, landed, block * 64, row,
-                                        head, page);
+                    const int slot = ri % C::kStages, use = ri / C::kStages;
+                    if (use > 0 && !__all_sync(0xffffffffu, wait_paged(bar(C::kBarKvEmpty + slot), (use - 1) & 1, abort_flag,
+                                                                       kSiteWideEmpty))) {
+                        ok = false;
+                        break;
                     }
-                    if (ok && i + 1 < count) page = page_at(first_tile + i + 1);
+                    // A V tile to be zeroed in part lands on the tail barrier; warp 11 then completes the slot's.
+                    const bool tail = is_v && i + 1 == count && has_tail;
+                    const uint32_t landed = bar((tail ? C::kBarTail : C::kBarKvFull) + slot);
+                    tail_slots = tail ? tail_slots | (1u << slot) : tail_slots & ~(1u << slot);
+                    if (tail) tail_parity ^= 1u << slot;
+                    if (lane == 0) mbar_arrive_expect_tx(landed, C::kTileBytes);
+                    __syncwarp();
+                    if (active)
+                        tma_load_4d(ring + slot * C::kTileBytes + offset, map, landed, block * 64, row, head, page);
+                    if (i + 1 < count) page = page_at(first_tile + i + 1);
                 }
             }
             if (!ok && lane == 0) {
                 if (q_loads > 0) drain_paged(bar(C::kBarQFull), (q_loads - 1) & 1);
-                for (int i = ri > C::kStages ? ri - C::kStages : 0; i < ri; ++i) {
+                for (int i = ri > C::kStages ? ri - C::kStages : is_v; i < ri; i += 2) {
                     const int slot = i % C::kStages;
                     if (tail_slots >> slot & 1u) drain_paged(bar(C::kBarTail + slot), (tail_parity >> slot & 1u) ^ 1u);
                     else drain_paged(bar(C::kBarKvFull + slot), (i / C::kStages) & 1);
@@ -878,21 +891,54 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             auto in_slot = [](uint32_t low, int i) { return low + static_cast<uint32_t>(i % C::kStages) * (C::kTileBytes >> 4); };
             auto empty_bar = [&](int i) -> uint32_t { return bar(C::kBarKvEmpty + i % C::kStages); };
             int ri = 0;                         // ring index of the segment's first K tile
-            uint32_t par0 = 0, par1 = 0;        // parity of each Q tile's per-key-tile barriers
+            uint32_t par0 = 0, par1 = 0, par2 = 0;      // parities of the three sets of per-key-tile barriers
             bool ok = true;
             auto wait = [&](int index, uint32_t parity, uint32_t site) { return wait_paged(bar(index), parity, abort_flag, site); };
             auto wait_ring = [&](int i, uint32_t site) {
                 return wait_paged(bar(C::kBarKvFull + i % C::kStages), (i / C::kStages) & 1, abort_flag, site);
             };
-            // A segment's products; two Q tiles or one (separate code: the issuing thread's own instructions count).
-            auto issue_segment = [&](auto both, int count) -> bool {
-                constexpr bool two = decltype(both)::value;
+            // The products of a segment of one Q tile. Its S is double-buffered (key tile j in S_(j & 1)): Q K^T of the
+            // next key tile runs during the softmax of this one.
+            auto issue_one = [&](int count) -> bool {
                 wide_issue_qk<D>(t_s0, q0, in_slot(k_ring, ri));
                 umma_commit(bar(C::kBarSFull + 0));
-                if constexpr (two) {
-                    wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ri));
-                    umma_commit(bar(C::kBarSFull + 1));
+                umma_commit(empty_bar(ri));
+                if (count == 1) umma_commit(bar(C::kBarQEmpty));
+                for (int j = 0; j < count; ++j) {
+                    const int vi = ri + 2 * j + 1, ki = vi + 1;
+                    const bool odd = (j & 1) != 0;
+                    const int set = odd ? 2 : 0;
+                    const uint32_t t_sj = odd ? t_s1 : t_s0, parity = odd ? par2 : par0;
+                    if (j + 1 < count) {
+                        if (!wait_ring(ki, kSiteWideK)) return false;
+                        tc_fence_after();
+                        wide_issue_qk<D>(odd ? t_s0 : t_s1, q0, in_slot(k_ring, ki));
+                        umma_commit(bar(C::kBarSFull + (set ^ 2)));
+                        umma_commit(empty_bar(ki));
+                        if (j + 2 == count) umma_commit(bar(C::kBarQEmpty));
+                    }
+                    if (!wait_ring(vi, kSiteWideV)) return false;
+                    if (!wait(C::kBarPHalf + set, parity, kSiteWideP)) return false;
+                    tc_fence_after();
+                    wide_issue_pv<D, 0, 4>(t_o0, t_sj, in_slot(v_ring, vi), j > 0);
+                    umma_commit(bar(C::kBarPvHalf + 0));
+                    if (!wait(C::kBarPFull + set, parity, kSiteWideP)) return false;
+                    tc_fence_after();
+                    wide_issue_pv<D, 4, 8>(t_o0, t_sj, in_slot(v_ring, vi), true);
+                    umma_commit(empty_bar(vi));
+                    umma_commit(bar(C::kBarPvHalf + 1));
+                    if (j + 1 == count) umma_commit(bar(C::kBarOFull + 0));
+                    if (odd) par2 ^= 1u;
+                    else par0 ^= 1u;
                 }
+                return true;
+            };
+            // The products of a segment of two Q tiles.
+            auto issue_two = [&](int count) -> bool {
+                wide_issue_qk<D>(t_s0, q0, in_slot(k_ring, ri));
+                umma_commit(bar(C::kBarSFull + 0));
+                wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ri));
+                umma_commit(bar(C::kBarSFull + 1));
                 umma_commit(empty_bar(ri));
                 if (count == 1) umma_commit(bar(C::kBarQEmpty));
                 for (int j = 0; j < count; ++j) {
@@ -914,23 +960,19 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                         wide_issue_qk<D>(t_s0, q0, in_slot(k_ring, ki));
                         umma_commit(bar(C::kBarSFull + 0));
                     }
-                    if constexpr (two) {
-                        if (!wait(C::kBarPHalf + 1, par1, kSiteWideP)) return false;
-                        tc_fence_after();
-                        wide_issue_pv<D, 0, 4>(t_o1, t_s1, in_slot(v_ring, vi), j > 0);
-                        umma_commit(bar(C::kBarPvHalf + 1));
-                        if (!wait(C::kBarPFull + 1, par1, kSiteWideP)) return false;
-                        tc_fence_after();
-                        wide_issue_pv<D, 4, 8>(t_o1, t_s1, in_slot(v_ring, vi), true);
-                        par1 ^= 1u;
-                        umma_commit(empty_bar(vi));
-                        if (!more) umma_commit(bar(C::kBarOFull + 1));
-                        if (more) {
-                            wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ki));
-                            umma_commit(bar(C::kBarSFull + 1));
-                        }
-                    } else {
-                        umma_commit(empty_bar(vi));
+                    if (!wait(C::kBarPHalf + 1, par1, kSiteWideP)) return false;
+                    tc_fence_after();
+                    wide_issue_pv<D, 0, 4>(t_o1, t_s1, in_slot(v_ring, vi), j > 0);
+                    umma_commit(bar(C::kBarPvHalf + 1));
+                    if (!wait(C::kBarPFull + 1, par1, kSiteWideP)) return false;
+                    tc_fence_after();
+                    wide_issue_pv<D, 4, 8>(t_o1, t_s1, in_slot(v_ring, vi), true);
+                    par1 ^= 1u;
+                    umma_commit(empty_bar(vi));
+                    if (!more) umma_commit(bar(C::kBarOFull + 1));
+                    if (more) {
+                        wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ki));
+                        umma_commit(bar(C::kBarSFull + 1));
                     }
                     if (more) umma_commit(empty_bar(ki));
                     if (j + 2 == count) umma_commit(bar(C::kBarQEmpty));    // the segment's last S is on its way
@@ -948,7 +990,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     ok = wait(C::kBarQFull, sg & 1, kSiteWideQ) && wait_ring(ri, kSiteWideK);
                     if (ok) {
                         tc_fence_after();
-                        ok = two ? issue_segment(std::true_type{}, count) : issue_segment(std::false_type{}, count);
+                        ok = two ? issue_two(count) : issue_one(count);
                         ri += 2 * count;
                     }
                 }
@@ -960,34 +1002,14 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 drain_paged(bar(C::kBarDrain), 0);
             }
             __syncwarp();
-        } else if (warp == kTail) {
-            // ======================= zeroes behind the last key ================
-            int ri = 0;
-            uint32_t parity = 0;
-            for (int sg = 0; await_segment(sg); ++sg) {
-                const int count = segments[sg & 1].count, from = segments[sg & 1].zero_from, to = segments[sg & 1].zero_to;
-                release_segment(sg);
-                if (count == 0) break;
-                ri += 2 * count;
-                if (from >= to) continue;
-                const int slot = (ri - 1) % C::kStages;
-                if (!__all_sync(0xffffffffu, wait_paged(bar(C::kBarTail + slot), parity >> slot & 1u, abort_flag, kSiteWideTail)))
-                    break;
-                parity ^= 1u << slot;
-                const int bytes = (to - from) * 128;
-                for (int sub = 0; sub < C::kSub; ++sub) {
-                    uint8_t* at = smem + C::kRingOff + slot * C::kTileBytes + sub * C::kSubBytes + from * 128;
-                    for (int i = lane * 16; i < bytes; i += 512) *reinterpret_cast<uint4*>(at + i) = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(C::kBarKvFull + slot));
-            }
         } else {
-            // ======================= the walk along the line ===================
+            // ======================= the walk along the line, and V behind the last key
             const RequestFinder finder(plan, start);
             long long x = begin;
             Merge merge{};
+            int ri = 0;                                     // ring index behind the segment before
+            int zero_from = 0, zero_to = 0, zero_slot = 0;  // of the segment before
+            uint32_t parity = 0;
             for (int sg = 0;; ++sg) {
                 if (sg > 1 && !__all_sync(0xffffffffu, wait_paged(bar(C::kBarSchedEmpty + (sg & 1)), ((sg >> 1) - 1) & 1,
                                                                   abort_flag, kSiteWideSched)))
@@ -995,27 +1017,38 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 WideSegment s;
                 s.count = 0;
                 while (x < end && s.count <= 0) {
-                    s = wide_segment(plan, finder, x, end);
-                    if (s.count <= 0) {
-                        s.count = 0;
-                        x = s.last;
-                    }
+                    s = wide_segment(plan, finder, x, end, share);
+                    x = s.last;
+                    if (s.count < 0) s.count = 0;
                 }
                 if (s.count > 0) {
-                    // A block that began before this CTA's range leaves its part in the CTA's first place, one
-                    // that goes on behind it in the second.
-                    if (s.first < begin) s.part = 2 * static_cast<int>(blockIdx.x);
-                    else if (s.last > end) s.part = 2 * static_cast<int>(blockIdx.x) + 1;
-                    if (s.first >= begin && s.last > end)
-                        merge = {static_cast<int>((s.last - 1) / share) - static_cast<int>(blockIdx.x) + 1, s.token0, s.tokens,
-                                 s.h * group};
-                    x = s.first + s.tile + s.count;
+                    if (s.part == 1) merge = {s.parts, s.token0, s.tokens, s.h * group};
+                    if (s.part >= 0) s.part += 2 * static_cast<int>(blockIdx.x);
                 }
                 if (lane == 0) {
                     segments[sg & 1] = s;
                     mbar_arrive(bar(C::kBarSchedFull + (sg & 1)));
                 }
+                // The segment before: the rows behind the last key of its last V tile.
+                if (zero_from < zero_to) {
+                    if (!__all_sync(0xffffffffu, wait_paged(bar(C::kBarTail + zero_slot), parity >> zero_slot & 1u, abort_flag,
+                                                            kSiteWideTail)))
+                        break;
+                    parity ^= 1u << zero_slot;
+                    const int bytes = (zero_to - zero_from) * 128;
+                    for (int sub = 0; sub < C::kSub; ++sub) {
+                        uint8_t* at = smem + C::kRingOff + zero_slot * C::kTileBytes + sub * C::kSubBytes + zero_from * 128;
+                        for (int i = lane * 16; i < bytes; i += 512) *reinterpret_cast<uint4*>(at + i) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(C::kBarKvFull + zero_slot));
+                }
                 if (s.count == 0) break;
+                ri += 2 * s.count;
+                zero_from = s.zero_from;
+                zero_to = s.zero_to;
+                zero_slot = (ri - 1) % C::kStages;
             }
             if (lane == 0) p.wide_merges[blockIdx.x] = merge;
         }
@@ -1027,13 +1060,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const int quarter = warp % 4;
         const int r = quarter * 32 + lane;         // row within the Q tile == tensor-memory lane
         const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-        const uint32_t t_s = lane_base + (t == 0 ? C::kColS0 : C::kColS1);
+        const uint32_t t_s0 = lane_base + C::kColS0;
         const uint32_t t_o = lane_base + (t == 0 ? C::kColO0 : C::kColO1);
         const int tok = t * per_tile + r / group;       // token of this row within its block
         const float sl2 = p.scale_log2;
         const uint64_t c2 = f2_pack(sl2, sl2);
-        uint32_t phase = 0;                        // parity of this tile's per-key-tile barriers
-        uint32_t o_phase = 0;
+        // Parities: of the barrier sets (one bit each); of PvHalf, which completes once per key tile; of OFull.
+        uint32_t sets = 0, pv_phase = 0, o_phase = 0;
 
         auto rescale_o = [&](float scale) {
             const uint64_t a2 = f2_pack(scale, scale);
@@ -1093,8 +1126,10 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             const WideSegment& seg = segments[sg & 1];
             const int count = seg.count;
             if (count == 0) break;
-            if (t == 1 && seg.tokens <= per_tile) {     // this block has one tile
+            const bool one = seg.tokens <= per_tile;    // this block has one Q tile
+            if (t == 1 && one) {
                 release_segment(sg);
+                pv_phase ^= count & 1;
                 continue;
             }
             const int tile = seg.tile;
@@ -1102,8 +1137,10 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             // First key tile of the stretch that some row of this Q tile must not see all of.
             const int mask_from = (plan.causal ? seg.pos0 + t * per_tile + 1 : seg.kv) / kWideKeys - tile;
             float row_max = -INFINITY, row_sum = 0.0f, m_base = 0.0f;
-            for (int j = 0; j < count; ++j, phase ^= 1u) {
-                ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarSFull + t), phase, abort_flag, kSiteWideS));
+            for (int j = 0; j < count; ++j, pv_phase ^= 1u) {
+                const int set = one ? 2 * (j & 1) : t;
+                const uint32_t t_s = t_s0 + (set ? C::kColS1 - C::kColS0 : 0u);
+                ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarSFull + set), sets >> set & 1u, abort_flag, kSiteWideS));
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t sc[4][32];
@@ -1156,7 +1193,11 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                         } else {
                             // The first-half PV of this tile may be running on the old base: let it finish, then
                             // correct O, its contribution included.
-                            ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarPvHalf + t), phase, abort_flag, kSiteWideO));
+                            if (one && j > 0) {     // (a phase is only told from the one before: that one has to be over)
+                                ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarPvHalf + 1), pv_phase ^ 1u, abort_flag, kSiteWideO));
+                                if (!ok) break;
+                            }
+                            ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarPvHalf + t), pv_phase, abort_flag, kSiteWideO));
                             if (!ok) break;
                             tc_fence_after();
                             rescale_o(alpha);
@@ -1165,16 +1206,24 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     }
                     row_sum += hsum;
                     if (h == 0) {
-                        if (j > 0 && __any_sync(0xffffffffu, o_scale != 1.0f)) rescale_o(o_scale);
+                        if (j > 0 && __any_sync(0xffffffffu, o_scale != 1.0f)) {
+                            if (one) {      // S of this tile can be ready before the PV of the one before is done
+                                ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarPvHalf + 1), pv_phase ^ 1u, abort_flag, kSiteWideO));
+                                if (!ok) break;
+                                tc_fence_after();
+                            }
+                            rescale_o(o_scale);
+                        }
                         tmem_wait_st();
                         tc_fence_before();
-                        mbar_arrive(bar(C::kBarPHalf + t));
+                        mbar_arrive(bar(C::kBarPHalf + set));
                     }
                 }
                 if (!ok) break;
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(bar(C::kBarPFull + t));
+                mbar_arrive(bar(C::kBarPFull + set));
+                sets ^= 1u << set;
             }
             if (!ok) break;
 

@@ -4,7 +4,8 @@
 // A request with n new tokens and a group of G query heads per K/V head has n * G query
 // rows per K/V head (row = token * G + head in group). Requests of at most narrow_rows(plan) rows
 // go to the narrow kernel, whose unit of work is a 64-key tile; all others to the wide kernel,
-// whose unit is a 128-key tile of a block of 2 * tokens_per_tile(G) tokens. Each narrow item (one
+// which takes 128-key tiles of blocks of 2 * tokens_per_tile(G) tokens, at two units each (one if the
+// block has one Q tile). Each narrow item (one
 // K/V head of a request) and each block is preceded by kNarrowGap or kWideGap units without work,
 // about what its set-up and epilogue cost.
 #pragma once
@@ -16,7 +17,7 @@
 namespace fa_sm100 {
 
 constexpr int kNarrowGap = 1;
-constexpr int kWideGap = 2;
+constexpr int kWideGap = 4;
 constexpr int kNarrowKeys = 64;
 constexpr int kWideRows = 128;      // query rows of one tile (tensor-memory lanes)
 constexpr int kWideKeys = 128;
@@ -63,15 +64,19 @@ __host__ __device__ inline long long wide_tiles_of(long long u, long long span, 
     return ceil_div(cached + (causal ? end : n), kWideKeys);
 }
 
+// Units of one of its key tiles: a block of one Q tile takes half the time of a block of two.
+__host__ __device__ inline int wide_weight(long long u, long long span, long long n) { return n - u * span <= span / 2 ? 1 : 2; }
+
 // Units (key tiles and gaps) of the request's first `blocks` token blocks.
 __host__ __device__ inline long long wide_units_through(long long blocks, long long span, long long cached, long long n,
                                                         bool causal)
 {
     if (blocks <= 0) return 0;
-    if (!causal) return blocks * (kWideGap + ceil_div(cached + n, kWideKeys));
     const long long whole = n / span < blocks ? n / span : blocks;      // blocks that end at (u + 1) * span
-    const long long sum = floor_sum_128(whole, span, cached + span + kWideKeys - 1);
-    return sum + blocks * kWideGap + (blocks > whole ? ceil_div(cached + n, kWideKeys) : 0);
+    const long long tiles = causal ? floor_sum_128(whole, span, cached + span + kWideKeys - 1)
+                                   : whole * ceil_div(cached + n, kWideKeys);
+    return blocks * kWideGap + 2 * tiles +
+           (blocks > whole ? wide_weight(whole, span, n) * ceil_div(cached + n, kWideKeys) : 0);
 }
 
 }  // namespace fa_sm100

@@ -55,14 +55,15 @@ def test_plan(cuda_device, lengths, page_size, padding):
 
 
 def _units(cached, new, group, causal):
-    """Attention units of a request: (64-key tiles and an idle unit, 128-key tiles of token blocks and two idle
-    units each)."""
+    """Attention units of a request: (64-key tiles and an idle unit, 128-key tiles of token blocks, two units each or
+    one for a block of at most 128 rows, and four idle units per block)."""
     if new == 0:
         return 0, 0
     if new * group <= 16:
         return 1 + -(-(cached + new) // 64), 0
     span = 2 * (128 // group)
-    return 0, sum(2 + -(-(cached + (min(new, u + span) if causal else new)) // 128) for u in range(0, new, span))
+    return 0, sum(4 + (1 if new - u <= span // 2 else 2) * -(-(cached + (min(new, u + span) if causal else new)) // 128)
+                  for u in range(0, new, span))
 
 
 @pytest.mark.parametrize("group", [1, 2, 3, 5, 7, 16, 33, 64, 127, 128])
