@@ -750,6 +750,17 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
                     } else {
                         // The first-half PV of this tile may be running on the old base: let it
                         // finish, then correct O (including its contribution) now.
+                        if constexpr (kOneTile) {
+                            // S of this tile can be ready before the previous tile's PV is done (its V may be
+                            // late), and a barrier's phase is only told apart from the one before it: wait for
+                            // that PV first, else the next wait could take the phase before it for its own.
+                            if (j > 0) {
+                                ok = __all_sync(0xffffffffu, wait_bounded(bar(C::kBarPvHalf + 1),
+                                                                          static_cast<uint32_t>((j - 1) & 1), abort_flag,
+                                                                          timeout, kSiteSoftO));
+                                if (!ok) break;
+                            }
+                        }
                         ok = __all_sync(0xffffffffu, wait_bounded(bar(C::kBarPvHalf + t), j & 1, abort_flag,
                                                                   timeout, kSiteSoftO));
                         if (!ok) break;
