@@ -58,8 +58,9 @@ constexpr float kRebase = 16.0f;
 // that is absent reads as zeros), with each item's Q and description ahead of its first tile; warps
 // 0-3 share out the keys of every tile (and the two 16-row tiles, if MT, their number, is 2), S = Q K^T
 // and O += P V by warp-level matrix instructions with Q, P and O in registers, a running maximum and
-// sum per warp, and meet only at an item's end, in the ring slot of its last tile. P is rounded to bf16 for the product with V (its sum is taken before);
-// everything else that is kept is 32-bit.
+// sum per warp, and meet only at an item's end, in the ring slot of its last tile. P goes into the
+// product with V as two bf16 numbers (rounded, and the rest), so that it keeps 16 bits; everything
+// else that is kept is 32-bit.
 constexpr int kNarrowWarps = 4;
 constexpr int kNarrowThreads = (kNarrowWarps + 1) * 32;
 constexpr int kNarrowCtasPerSm = 2;
@@ -445,15 +446,19 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     }
                 }
                 const float base0 = m0 == -INFINITY ? 0.0f : m0 * sl2, base1 = m1 == -INFINITY ? 0.0f : m1 * sl2;
-                uint32_t pf[MT][4];
+                // A weight as two bf16 numbers, rounded and rest: V's product is not bound by them, so P keeps 16 bits.
+                uint32_t pf[MT][4], rest[MT][4];
 #pragma unroll
                 for (int j = 0; j < 2 * MT; ++j) {
                     const float a0 = ex2_approx(fmaf(sc[j][0], sl2, -base0)), a1 = ex2_approx(fmaf(sc[j][1], sl2, -base0));
                     const float b0 = ex2_approx(fmaf(sc[j][2], sl2, -base1)), b1 = ex2_approx(fmaf(sc[j][3], sl2, -base1));
                     l0 += a0 + a1;
                     l1 += b0 + b1;
-                    pf[j / 2][2 * (j % 2)] = pack_bf16x2(a0, a1);
-                    pf[j / 2][2 * (j % 2) + 1] = pack_bf16x2(b0, b1);
+                    const uint32_t a = pack_bf16x2(a0, a1), b = pack_bf16x2(b0, b1);
+                    pf[j / 2][2 * (j % 2)] = a;
+                    pf[j / 2][2 * (j % 2) + 1] = b;
+                    rest[j / 2][2 * (j % 2)] = pack_bf16x2(a0 - __uint_as_float(a << 16), a1 - __uint_as_float(a & 0xffff0000u));
+                    rest[j / 2][2 * (j % 2) + 1] = pack_bf16x2(b0 - __uint_as_float(b << 16), b1 - __uint_as_float(b & 0xffff0000u));
                 }
                 // V rows behind the last key may hold anything: they are zeroed in the fragments (fragment
                 // register 0 holds keys 2t and 2t + 1 of 16, register 1 the same plus 8).
@@ -478,6 +483,8 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                         }
                         mma_16816(o[2 * dd], pf[s], b[0], b[1]);
                         mma_16816(o[2 * dd + 1], pf[s], b[2], b[3]);
+                        mma_16816(o[2 * dd], rest[s], b[0], b[1]);
+                        mma_16816(o[2 * dd + 1], rest[s], b[2], b[3]);
                     }
                 }
             }

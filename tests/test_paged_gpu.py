@@ -449,6 +449,26 @@ def test_shared_pages_and_output_over_q(cuda_device):
     assert same[3].isfinite().all()
 
 
+@pytest.mark.parametrize("seed", range(40))
+def test_mixed_batches(cuda_device, seed):
+    """Random batches over all head layouts, page sizes and kinds of requests, with scores that move the rows' maxima."""
+    rng = np.random.RandomState(seed)
+    dim, page_size = int(rng.choice([64, 128])), int(rng.choice([16, 32, 64, 128, 256]))
+    kv_heads = int(rng.choice([1, 2, 3, 8]))
+    heads = kv_heads * int(rng.choice([1, 2, 3, 4, 5, 8, 16, 24]))
+    seqs = int(rng.choice([1, 2, 7, 33, 64]))
+    most = int(rng.choice([1, 4, 9, 40, 300]))
+    cached = [int(x) for x in np.exp(rng.uniform(0, np.log(4000), seqs)).astype(int) - 1]
+    new = [int(x) for x in rng.randint(0, most + 1, seqs)]
+    r = Requests(cached, new, page_size, cuda_device, seed=seed, padding=int(rng.randint(0, 5)))
+    how = {"max_new": most} if seed % 2 else {}
+    q, caches, plan, out = check_attention(r, heads, kv_heads, dim, bool(rng.randint(0, 4)), seed, q_scale=float(rng.choice([1, 4, 12])),
+                                           **how)
+    if sum(new):
+        again = fa.paged_attention(q, *caches, plan)
+        assert torch.equal(again[: sum(new)], out[: sum(new)])
+
+
 def test_same_bits_every_time(cuda_device):
     r = Requests([9000, 17, 4000], [1, 200, 6], 16, cuda_device)
     q, (k, v), plan, want = check_attention(r, 8, 2, 128)
