@@ -64,7 +64,7 @@ constexpr float kRebase = 16.0f;
 constexpr int kNarrowWarps = 4;
 constexpr int kNarrowThreads = (kNarrowWarps + 1) * 32;
 constexpr int kNarrowCtasPerSm = 2;
-constexpr int kNarrowMinTiles = 3;       // units a CTA takes at least
+constexpr int kNarrowMinTiles = 2;       // units a CTA takes at least
 constexpr unsigned long long kTimeoutNs = 1000000000ull;
 
 // What the producer tells the consumers of a stretch of one (request, K/V head).
@@ -198,7 +198,7 @@ private:
 // Units per CTA when `total` are shared out over `ctas`.
 __device__ __forceinline__ long long narrow_share(long long total, int ctas)
 {
-    const long long even = (total + ctas - 1) / ctas;
+    const long long even = ceil_div(total, ctas);
     return even > kNarrowMinTiles ? even : kNarrowMinTiles;
 }
 
@@ -263,9 +263,9 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             NarrowItem item{};
             int b = 0, h = 0;
             if (x < end) {
-                const Request r = finder.find(x / plan.kv_heads);
+                const Request r = finder.find(quotient(x, plan.kv_heads));
                 b = r.b;
-                h = static_cast<int>((x - r.start * plan.kv_heads) / r.units);
+                h = static_cast<int>(quotient(x - r.start * plan.kv_heads, r.units));
                 // The item's tiles lie at [first, last) of the line, behind its gap.
                 const long long first = r.start * plan.kv_heads + h * r.units + kNarrowGap;
                 const long long last = first - kNarrowGap + r.units;
@@ -286,7 +286,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 item.part = first < begin ? 2 * static_cast<int>(blockIdx.x)
                                           : last > end ? 2 * static_cast<int>(blockIdx.x) + 1 : -1;
                 if (first >= begin && last > end)
-                    merge = {static_cast<int>((last - 1) / share) - static_cast<int>(blockIdx.x) + 1, item.token0, item.tokens,
+                    merge = {static_cast<int>(quotient(last - 1, share)) - static_cast<int>(blockIdx.x) + 1, item.token0, item.tokens,
                              item.head0};
                 x = stop;
             }
@@ -596,7 +596,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 // Tensor memory, barriers per key tile and the lazily moved exponent base are those of the dense
 // kernel (fa_sm100.cu); a block of at most 128 rows has its S double-buffered. P is rounded to bf16 for the product with V.
 constexpr int kWideThreads = 384;
-constexpr int kWideMinUnits = 8;        // units a CTA takes at least, more than a tile's
+constexpr int kWideMinUnits = 4;        // units a CTA takes at least, more than a tile's
 constexpr uint32_t kWideRegsLaunch = 168, kWideRegsSoftmax = 200, kWideRegsOther = 104;
 static_assert(2 * 128 * kWideRegsSoftmax + 128 * kWideRegsOther <= kWideThreads * kWideRegsLaunch,
               "the warpgroup register split must fit in the registers the CTA launches with");
@@ -665,44 +665,44 @@ __device__ inline WideSegment wide_segment(const FaPagedPlan& plan, const Reques
                                            long long share)
 {
     WideSegment s;
-    const Request r = finder.find(x / plan.kv_heads);
+    const Request r = finder.find(quotient(x, plan.kv_heads));
     s.b = r.b;
-    s.h = static_cast<int>((x - r.start * plan.kv_heads) / r.units);
+    s.h = static_cast<int>(quotient(x - r.start * plan.kv_heads, r.units));
     const long long head_first = r.start * plan.kv_heads + s.h * r.units;
     const int n = r.tokens;
     s.kv = r.kv;
     const int cached = s.kv - n;
     const int span = 2 * tokens_per_tile(plan.heads / plan.kv_heads);
     const bool causal = plan.causal != 0;
-    const int lane = threadIdx.x % 32;
+    const int lane = threadIdx.x % 32, whole = n / span;
     int lo = 0, blocks = (n - 1) / span + 1;    // the last block in [lo, lo + blocks) whose units begin at or before x
     while (blocks > 1) {
         const int step = (blocks + 31) / 32;
         const bool below = lane * step < blocks &&
-                           head_first + wide_units_through(lo + lane * step, span, cached, n, causal) <= x;
+                           head_first + wide_units_through(lo + lane * step, whole, span, cached, n, causal) <= x;
         const int at = RequestFinder::last_of(below);
         lo += at * step;
         blocks = min(step, blocks - at * step);
     }
     // The block's tiles lie at first, first + weight, ... of the line; a CTA takes those that begin in its range.
-    const long long first = head_first + wide_units_through(lo, span, cached, n, causal) + kWideGap;
+    const long long first = head_first + wide_units_through(lo, whole, span, cached, n, causal) + kWideGap;
     const int weight = wide_weight(lo, span, n);
     const int tiles = static_cast<int>(wide_tiles_of(lo, span, cached, n, causal));
     s.last = first + static_cast<long long>(weight) * tiles;
     s.token0 = r.token0 + lo * span;
     s.tokens = min(span, n - lo * span);
     s.pos0 = cached + lo * span;
-    s.tile = x <= first ? 0 : static_cast<int>(ceil_div(x - first, weight));
-    const int stop = end >= s.last ? tiles : end <= first ? 0 : static_cast<int>(ceil_div(end - first, weight));
+    s.tile = x <= first ? 0 : static_cast<int>((x - first + weight - 1) >> (weight - 1));
+    const int stop = end >= s.last ? tiles : end <= first ? 0 : static_cast<int>((end - first + weight - 1) >> (weight - 1));
     s.count = stop - s.tile;        // 0 or less: no tile of the block begins in the rest of the range
     // A block whose first tile is another CTA's leaves its part in the CTA's first place, one whose last tile is
     // another's in the second.
     s.part = s.tile > 0 ? 0 : stop < tiles ? 1 : -1;
-    s.parts = static_cast<int>((first + static_cast<long long>(weight) * (tiles - 1)) / share - first / share) + 1;
+    s.parts = static_cast<int>(quotient(first + static_cast<long long>(weight) * (tiles - 1), share) - quotient(first, share)) + 1;
     s.reserved = s.reserved2 = 0;
     // Behind the last key: rows of the last page (pages behind it are zero-filled by the copy).
     const int v0 = (s.tile + s.count - 1) * kWideKeys;
-    const int held = (s.kv + plan.page_size - 1) / plan.page_size * plan.page_size;
+    const int held = (s.kv + plan.page_size - 1) & ~(plan.page_size - 1);
     s.zero_from = s.kv - v0;
     s.zero_to = min(kWideKeys, held - v0);
     if (s.zero_from >= s.zero_to) s.zero_from = s.zero_to = 0;
@@ -711,7 +711,7 @@ __device__ inline WideSegment wide_segment(const FaPagedPlan& plan, const Reques
 
 __device__ __forceinline__ long long wide_share(long long total, int ctas)
 {
-    const long long even = (total + ctas - 1) / ctas;
+    const long long even = ceil_div(total, ctas);
     return even > kWideMinUnits ? even : kWideMinUnits;
 }
 

@@ -42,41 +42,50 @@ __host__ __device__ inline int narrow_rows(const FaPagedPlan& plan)
 }
 
 __host__ __device__ inline int tokens_per_tile(int group) { return kWideRows / group; }
-__host__ __device__ inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
-
-// sum over 0 <= i < n of floor((a * i + b) / 128), a, b >= 0. The terms' sum is exact without the
-// floors; what the floors drop, (a * i + b) mod 128, repeats with period P = 128 / gcd(a, 128), and
-// over one period takes each value that is b modulo the gcd once. So P - 1 terms at most are added up.
-__host__ __device__ inline long long floor_sum_128(long long n, long long a, long long b)
+// a / b for a >= 0, b > 0: nearly always in 32 bits, where a division costs a fifth. The kernels find their
+// first work with these, before anything else can start.
+__host__ __device__ inline long long quotient(long long a, long long b)
 {
-    long long g = 128;
-    while (a % g) g >>= 1;
-    const long long period = 128 / g;
-    long long dropped = n / period * (period * (b % g) + g * (period * (period - 1) / 2));
-    for (long long i = 0; i < n % period; ++i) dropped += (a * i + b) & 127;
-    return (n * b + a * (n * (n - 1) / 2) - dropped) / 128;
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+__host__ __device__ inline long long ceil_div(long long a, long long b) { return quotient(a + b - 1, b); }
+__host__ __device__ inline long long key_tiles(long long keys) { return (keys + kWideKeys - 1) >> 7; }
+
+// sum over 0 <= i < n of floor((a * i + b) / 128), a > 0, b >= 0. The terms' sum is exact without the
+// floors; what the floors drop, (a * i + b) mod 128, repeats with period 128 / gcd(a, 128), and over one
+// period takes each value that is b modulo the gcd once. So fewer terms than a period are added up.
+__host__ __device__ inline long long floor_sum_128(long long n, int a, long long b)
+{
+    int log_gcd = 0;
+    while (log_gcd < 7 && (a >> log_gcd & 1) == 0) ++log_gcd;
+    const int period = 128 >> log_gcd, gcd = 1 << log_gcd;
+    const int rest = static_cast<int>(b & 127);
+    long long dropped = (n >> (7 - log_gcd)) * (period * (rest & (gcd - 1)) + gcd * (period * (period - 1) / 2));
+    const int left = static_cast<int>(n & (period - 1));
+    int partial = 0;
+    for (int i = 0; i < left; ++i) partial += (a * i + rest) & 127;
+    dropped += partial;
+    return (n * b + a * (n * (n - 1) / 2) - dropped) >> 7;
 }
 
 // Key tiles of token block u (of `span` tokens) of a request with `cached` + `n` tokens.
-__host__ __device__ inline long long wide_tiles_of(long long u, long long span, long long cached, long long n, bool causal)
+__host__ __device__ inline long long wide_tiles_of(long long u, int span, long long cached, int n, bool causal)
 {
     const long long end = (u + 1) * span < n ? (u + 1) * span : n;
-    return ceil_div(cached + (causal ? end : n), kWideKeys);
+    return key_tiles(cached + (causal ? end : n));
 }
 
 // Units of one of its key tiles: a block of one Q tile takes half the time of a block of two.
-__host__ __device__ inline int wide_weight(long long u, long long span, long long n) { return n - u * span <= span / 2 ? 1 : 2; }
+__host__ __device__ inline int wide_weight(long long u, int span, int n) { return n - u * span <= span / 2 ? 1 : 2; }
 
-// Units (key tiles and gaps) of the request's first `blocks` token blocks.
-__host__ __device__ inline long long wide_units_through(long long blocks, long long span, long long cached, long long n,
+// Units (key tiles and gaps) of the request's first `blocks` token blocks, of which `whole` (n / span) are full.
+__host__ __device__ inline long long wide_units_through(long long blocks, int whole, int span, long long cached, int n,
                                                         bool causal)
 {
-    if (blocks <= 0) return 0;
-    const long long whole = n / span < blocks ? n / span : blocks;      // blocks that end at (u + 1) * span
-    const long long tiles = causal ? floor_sum_128(whole, span, cached + span + kWideKeys - 1)
-                                   : whole * ceil_div(cached + n, kWideKeys);
-    return blocks * kWideGap + 2 * tiles +
-           (blocks > whole ? wide_weight(whole, span, n) * ceil_div(cached + n, kWideKeys) : 0);
+    const long long full = whole < blocks ? whole : blocks;
+    const long long tiles = causal ? floor_sum_128(full, span, cached + span + kWideKeys - 1) : full * key_tiles(cached + n);
+    return blocks * kWideGap + 2 * tiles + (blocks > full ? wide_weight(whole, span, n) * key_tiles(cached + n) : 0);
 }
 
 }  // namespace fa_sm100

@@ -60,7 +60,7 @@ plan_kernel(const PlanParams p)
     const int ps = plan.page_size;
     const int shift = __ffs(ps) - 1;
     const int group = plan.heads / plan.kv_heads;
-    const long long span = 2LL * tokens_per_tile(group);
+    const int span = 2 * tokens_per_tile(group);
     const bool first_cta = blockIdx.x == 0;
 
     __shared__ PlanSums warp_sums[kPlanWarps];
@@ -111,7 +111,9 @@ plan_kernel(const PlanParams p)
         if (!fits && first_cta && b < plan.num_seqs) record_plan_error(FA_ERROR_BAD_LENGTH);
         if (valid && fits && n > 0) {
             if (n * group <= narrow_rows(plan)) narrow_units = kNarrowGap + ceil_div(cached + n, kNarrowKeys);
-            else wide_units = wide_units_through(ceil_div(n, span), span, cached, n, plan.causal != 0);
+            else
+                wide_units = wide_units_through(ceil_div(n, span), static_cast<int>(n) / span, span, cached, static_cast<int>(n),
+                                                plan.causal != 0);
         }
         s_start[tid] = static_cast<int>(tokens_before < total ? tokens_before : total);
         s_page[tid] = static_cast<int>(pages_before - carry.pages < INT_MAX ? pages_before - carry.pages : INT_MAX);
