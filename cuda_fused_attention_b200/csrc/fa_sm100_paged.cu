@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -1459,20 +1460,20 @@ bool page_size_supported(int page_size)
 int current_sm100(int* device, int* sm_count)
 {
     constexpr int kMax = 64;
-    static int counts[kMax];        // SM count of each device once known (written with the same value by any thread)
+    static std::atomic<int> counts[kMax];       // SM count of each device once known
     cudaError_t err = cudaGetDevice(device);
     if (err != cudaSuccess) return static_cast<int>(err);
     if (*device < 0 || *device >= kMax) return FA_STATUS_INVALID_ARGUMENT;
-    if (counts[*device] == 0) {
+    if (counts[*device].load() == 0) {
         int major = 0, count = 0;
         err = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, *device);
         if (err != cudaSuccess) return static_cast<int>(err);
         if (major != 10) return FA_STATUS_NO_SM100;
         err = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, *device);
         if (err != cudaSuccess) return static_cast<int>(err);
-        counts[*device] = count;
+        counts[*device].store(count);
     }
-    *sm_count = counts[*device];
+    *sm_count = counts[*device].load();
     return FA_STATUS_OK;
 }
 

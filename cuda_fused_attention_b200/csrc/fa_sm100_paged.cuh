@@ -5,9 +5,10 @@
 // rows per K/V head (row = token * G + head in group). Requests of at most narrow_rows(plan) rows
 // go to the narrow kernel, whose unit of work is a 64-key tile; all others to the wide kernel,
 // which takes 128-key tiles of blocks of 2 * tokens_per_tile(G) tokens, at two units each (one if the
-// block has one Q tile). Each narrow item (one
-// K/V head of a request) and each block is preceded by kNarrowGap or kWideGap units without work,
-// about what its set-up and epilogue cost.
+// block has one Q tile). Each narrow item (one K/V head of a request) and each block is preceded by
+// kNarrowGap or kWideGap units without work, about what its set-up and epilogue cost. Without the
+// narrow gap 32 ragged requests of up to 4096 keys take 55.0 us instead of 52.4, with two 52.8;
+// without the wide one a causal prompt of 8192 tokens (16 heads) 340 us instead of 300.
 #pragma once
 
 #include <cstdint>
@@ -29,7 +30,8 @@ __host__ __device__ inline long long* narrow_starts(long long* schedule, int) { 
 __host__ __device__ inline long long* wide_starts(long long* schedule, int num_seqs) { return schedule + num_seqs + 1; }
 
 // Query rows per K/V head that any request of the plan can have, and the most that go to the narrow
-// kernel: 32 where no request has more (drafted tokens), else 16, which its faster variant holds.
+// kernel: 32 where no request has more (drafted tokens), else 16, which its faster variant holds. 16
+// requests of 5 to 8 new tokens, 20 to 32 rows, behind up to 8192: 63 us against 84 in the wide kernel.
 __host__ __device__ inline long long most_rows(const FaPagedPlan& plan)
 {
     return static_cast<long long>(plan.max_new < plan.total_tokens ? plan.max_new : plan.total_tokens) *
@@ -42,6 +44,7 @@ __host__ __device__ inline int narrow_rows(const FaPagedPlan& plan)
 }
 
 __host__ __device__ inline int tokens_per_tile(int group) { return kWideRows / group; }
+
 // a / b for a >= 0, b > 0: nearly always in 32 bits, where a division costs a fifth. The kernels find their
 // first work with these, before anything else can start.
 __host__ __device__ inline long long quotient(long long a, long long b)

@@ -286,6 +286,18 @@ PyObject* plan(PyObject* const* args, Py_ssize_t count)
         buffer = tensor(args[10], "plan");
         if (buffer.numel() != words || buffer.scalar_type() != at::kInt || !buffer.is_cuda() || buffer.get_device() != device.index())
             bad_value("plan was made for other sizes or another device");
+        // The kernel's blocks write the plan while others still read the inputs.
+        auto apart = [&](const at::Tensor& t, const char* name) {
+            const auto* from = static_cast<const char*>(buffer.const_data_ptr());
+            const auto* at = static_cast<const char*>(t.const_data_ptr());
+            if (t.numel() > 0 && at < from + 4 * words && at + t.nbytes() > from)
+                bad_value(std::string(name) + " must not be a part of the plan that is written");
+        };
+        apart(cached, "cached_lens");
+        apart(fresh, "new_lens");
+        apart(free_pages, "free_pages");
+        apart(table, "block_table");
+        if (has_cursor) apart(tensor(args[7], "free_cursor"), "free_cursor");
     }
     FaPagedPlan c{};
     c.num_seqs = static_cast<int>(seqs);

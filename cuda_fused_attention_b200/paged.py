@@ -110,7 +110,8 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, total_tokens, sha
     axis, at least the sum of new_lens. num_pages: pages of the cache. max_new: an upper bound of
     new_lens (default total_tokens); a tight one lets calls leave out kernels that have no work.
     plan: an earlier plan of the same B, total_tokens and shape whose buffers are written again
-    (for CUDA graphs). Returns the PagedPlan.
+    (for CUDA graphs); its own arrays cannot be inputs then: copy kv_lens and free_cursor to the next
+    step's tensors first. Returns the PagedPlan.
     """
     ops = _ops or _load()
     seqs = cached_lens.numel()

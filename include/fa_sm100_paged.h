@@ -72,7 +72,8 @@ FA_API size_t fa_sm100_paged_schedule_bytes(int num_seqs);
 /* Extends every request's table row by the pages its new tokens need and writes the
  * plan's arrays. New pages are free_pages[*free_start + k] (free_start may be NULL: 0),
  * handed out in request order; entries behind a request's last page stay as they were.
- * The inputs are not changed, so a call with the same inputs gives the same result. */
+ * The inputs are not changed, so a call with the same inputs gives the same result; they must not
+ * overlap the plan's arrays. */
 FA_API int fa_sm100_paged_plan(const FaPagedPlan* plan, const int* cached_lens, const int* new_lens,
                                const int* free_pages, int num_free, const int* free_start, void* stream);
 

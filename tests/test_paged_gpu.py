@@ -97,6 +97,12 @@ def test_plan_views_are_the_struct_s_pointers(cuda_device):
     assert c.query_start == c.schedule + _lib.load().fa_sm100_paged_schedule_bytes(3)
     with pytest.raises(ValueError):
         r.plan(fa.PagedShape(8, 2, 128, 16), plan=plan)
+    for own in ("cached_lens", "free_cursor"):      # blocks would read what others have written
+        args = dict(cached_lens=r.cached_lens, free_cursor=None)
+        args[own] = plan.kv_lens if own == "cached_lens" else plan.free_cursor
+        with pytest.raises(ValueError, match="part of the plan"):
+            fa.paged_plan(args["cached_lens"], r.new_lens, r.block_table, r.free_pages, r.total, plan.shape, r.num_pages,
+                          free_cursor=args["free_cursor"], plan=plan)
 
 
 def test_plan_steps_through_the_free_list(cuda_device):
