@@ -61,11 +61,14 @@ constexpr float kRebase = 16.0f;
 // and O += P V by warp-level matrix instructions with Q, P and O in registers, a running maximum and
 // sum per warp, and meet only at an item's end, in the ring slot of its last tile. P goes into the
 // product with V as two bf16 numbers (rounded, and the rest), so that it keeps 16 bits; everything
-// else that is kept is 32-bit.
+// else that is kept is 32-bit. Why mma.sync and not tcgen05: a tile of 128 rows would be nearly empty, and
+// its fragments keep up with memory. Measured (B200, 32/8 heads, D = 128): 64 requests of 4095 to
+// 16384 keys 410 us, 6.6 TB/s; 32 of up to 4096 keys 52 us with the merging, 5.3 TB/s; 16 of 5 to 8
+// new tokens behind up to 8192 (MT = 2) 63 us, 4.8 TB/s.
 constexpr int kNarrowWarps = 4;
 constexpr int kNarrowThreads = (kNarrowWarps + 1) * 32;
 constexpr int kNarrowCtasPerSm = 2;
-constexpr int kNarrowMinTiles = 2;       // units a CTA takes at least
+constexpr int kNarrowMinTiles = 2;       // units a CTA takes at least (2048 keys, 8 heads: 8.5 us; 3: 8.8, 5: 10.5, 8: 11.5)
 constexpr unsigned long long kTimeoutNs = 1000000000ull;
 
 // What the producer tells the consumers of a stretch of one (request, K/V head).
@@ -595,9 +598,15 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 // 8 MMA issuer; 9 and 10 TMA producers of Q and K and of V; 11 walks the line, hands out the segments,
 // and zeroes what V's last page holds behind the last key (a weight of zero does not silence a NaN).
 // Tensor memory, barriers per key tile and the lazily moved exponent base are those of the dense
-// kernel (fa_sm100.cu); a block of at most 128 rows has its S double-buffered. P is rounded to bf16 for the product with V.
+// kernel (fa_sm100.cu); a block of at most 128 rows has its S double-buffered. P is rounded to bf16 for
+// the product with V, as in the dense kernel: a second product for the rest would cost the tensor
+// pipe a third more. Measured (B200, 32/8 heads, D = 128): 2048 new tokens behind 14336 cached 445 us,
+// 1158 TFLOP/s; a prompt of 8192 tokens without mask (16 heads) 490 us, as the dense kernel; 16
+// requests of 16 new tokens (64 rows) behind up to 8192 74 us, 4.1 TB/s.
 constexpr int kWideThreads = 384;
-constexpr int kWideMinUnits = 4;        // units a CTA takes at least, more than a tile's
+constexpr int kWideMinUnits = 4;        // units a CTA takes at least, more than a tile's (256 new tokens: 19.4 us; 8: 22.3)
+// 216 / 72 registers made the MMA issuer spill, and a load by it waits for its queued MMAs: 493 us against 462 (chunk
+// of 2048 tokens).
 constexpr uint32_t kWideRegsLaunch = 168, kWideRegsSoftmax = 200, kWideRegsOther = 104;
 static_assert(2 * 128 * kWideRegsSoftmax + 128 * kWideRegsOther <= kWideThreads * kWideRegsLaunch,
               "the warpgroup register split must fit in the registers the CTA launches with");
@@ -1322,7 +1331,8 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 //     sum_i w_i O_i / sum_i w_i l_i,   w_i = 2^((m_i - max_i m_i) log2(e) / sqrt(D)).
 // What to merge was written down by the CTA with the first part. A few round trips to memory bound
 // this, so its blocks are small and launched while the kernel before still runs (programmatic
-// dependent launch).
+// dependent launch): about 3 us behind the narrow kernel; behind the wide one, whose parts are 256 rows,
+// 5 us for 40 MB of parts at D = 128.
 constexpr int kCombineThreads = 128;
 
 // One row per warp; a lane has D / 32 columns.
