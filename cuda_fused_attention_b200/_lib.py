@@ -56,6 +56,7 @@ SIGNATURES = {
                                     _I, _VP, _I, _I, _VP]),
     "fa_sm100_paged_fwd": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, ctypes.c_size_t, _VP]),
     "fa_sm100_paged_workspace_bytes": (ctypes.c_size_t, [_VP]),
+    "fa_sm100_paged_test_arm_stall": (_I, []),
 }
 
 

@@ -28,6 +28,7 @@ struct PagedParams {
     long long k_page, k_head, k_row, v_page, v_head, v_row;
     int page_shift;
     float scale_log2;
+    int inject_stall;           // test only: the warps that hand out work wait on a barrier nothing arrives on
     // Parts of items that cross a border between CTAs' ranges, two places per CTA, and per CTA what is to be
     // merged from the second place on; for the narrow and for the wide kernel.
     float* partial;
@@ -262,7 +263,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         const void* map = is_v ? static_cast<const void*>(&tm_v) : static_cast<const void*>(&tm_k);
         int it = 0, sg = 0;
         Merge merge{};
-        bool ok = true;
+        bool ok = p.inject_stall == 0 || __all_sync(0xffffffffu, wait_paged(item_empty(0), 0, abort_flag, kSiteNarrowItemFree));
         for (long long x = begin; ok;) {
             NarrowItem item{};
             int b = 0, h = 0;
@@ -1027,7 +1028,9 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             int ri = 0;                                     // ring index behind the segment before
             int zero_from = 0, zero_to = 0, zero_slot = 0;  // of the segment before
             uint32_t parity = 0;
-            for (int sg = 0;; ++sg) {
+            const bool go = p.inject_stall == 0 ||
+                            __all_sync(0xffffffffu, wait_paged(bar(C::kBarSchedEmpty), 0, abort_flag, kSiteWideSched));
+            for (int sg = 0; go; ++sg) {
                 if (sg > 1 && !__all_sync(0xffffffffu, wait_paged(bar(C::kBarSchedEmpty + (sg & 1)), ((sg >> 1) - 1) & 1,
                                                                   abort_flag, kSiteWideSched)))
                     break;
@@ -1561,6 +1564,9 @@ int prepare_paged_device(int device)
     return state.status;
 }
 
+// Test only: set by fa_sm100_paged_test_arm_stall for this host thread's next launch.
+thread_local bool t_armed_stall = false;
+
 int narrow_ctas(int sms) { return kNarrowCtasPerSm * sms; }
 
 // Workspace: the parts, then the merges, of each kernel.
@@ -1649,6 +1655,12 @@ int launch_attention(const PagedMaps& maps, const PagedParams& params, bool wide
 
 extern "C" {
 
+int fa_sm100_paged_test_arm_stall(void)
+{
+    t_armed_stall = true;
+    return FA_STATUS_OK;
+}
+
 size_t fa_sm100_paged_workspace_bytes(const FaPagedPlan* plan)
 {
     int device = 0, sms = 0;
@@ -1670,8 +1682,10 @@ int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cac
     uintptr_t any = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) |
                     reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(o);
     if (any & 15u) return FA_STATUS_MISALIGNED;
-    for (int i = 0; i < 10; ++i)
+    for (int i = 0; i < 10; ++i) {
+        if (strides[i] < 0) return FA_STATUS_INVALID_ARGUMENT;
         if (strides[i] & 7) return FA_STATUS_MISALIGNED;
+    }
     int device = 0, sms = 0;
     status = fa_sm100_internal::current_sm100(&device, &sms);
     if (status != FA_STATUS_OK) return status;
@@ -1699,6 +1713,8 @@ int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cac
     params.v_row = strides[9];
     params.page_shift = __builtin_ctz(static_cast<unsigned>(plan->page_size));
     params.scale_log2 = fa_default_scale(plan->head_dim) * 1.4426950408889634f;
+    params.inject_stall = t_armed_stall ? 1 : 0;
+    t_armed_stall = false;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = may_be_wide(*plan), narrow = may_be_narrow(*plan);
     PagedMaps maps;

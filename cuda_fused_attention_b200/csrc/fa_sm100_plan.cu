@@ -451,11 +451,14 @@ namespace {
 
 using namespace fa_sm100;
 
-bool multiple_of_8(const long long* strides, int count)
+// FA_STATUS_OK if all strides are multiples of 8 and none is negative.
+int check_strides(const long long* strides, int count)
 {
-    for (int i = 0; i < count; ++i)
-        if (strides[i] & 7) return false;
-    return true;
+    for (int i = 0; i < count; ++i) {
+        if (strides[i] < 0) return FA_STATUS_INVALID_ARGUMENT;
+        if (strides[i] & 7) return FA_STATUS_MISALIGNED;
+    }
+    return FA_STATUS_OK;
 }
 
 bool misaligned(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) != 0; }
@@ -558,12 +561,13 @@ int fa_sm100_rotary(const void* x, const long long* x_strides, void* out, const 
     if (head_dim != 64 && head_dim != 128) return FA_STATUS_UNSUPPORTED;
     if (rotary_dim <= 0 || rotary_dim > head_dim || rotary_dim % 16) return FA_STATUS_INVALID_ARGUMENT;
     RotaryParams params{};
-    const int status = fill_sections(params, sections, axes, rotary_dim);
+    int status = fill_sections(params, sections, axes, rotary_dim);
     if (status != FA_STATUS_OK) return status;
     if (batch == 0 || heads == 0 || seq_len == 0) return FA_STATUS_OK;
     if (x == nullptr || out == nullptr || positions == nullptr || inv_freq == nullptr) return FA_STATUS_INVALID_ARGUMENT;
-    if (misaligned(x) || misaligned(out) || !multiple_of_8(x_strides, 3) || !multiple_of_8(out_strides, 3))
-        return FA_STATUS_MISALIGNED;
+    if (misaligned(x) || misaligned(out)) return FA_STATUS_MISALIGNED;
+    if ((status = check_strides(x_strides, 3)) != FA_STATUS_OK || (status = check_strides(out_strides, 3)) != FA_STATUS_OK)
+        return status;
     params.src[0] = static_cast<const __nv_bfloat16*>(x);
     params.dst[0] = static_cast<__nv_bfloat16*>(out);
     params.src_batch = x_strides[0];
@@ -599,15 +603,16 @@ int fa_sm100_rotary_append(const void* q, const void* k, const void* v, void* q_
     if (static_cast<long long>(num_pages) * page_size > INT_MAX) return FA_STATUS_INVALID_ARGUMENT;
     if (rotary_dim <= 0 || rotary_dim > head_dim || rotary_dim % 16) return FA_STATUS_INVALID_ARGUMENT;
     RotaryParams params{};
-    const int status = fill_sections(params, sections, axes, rotary_dim);
+    int status = fill_sections(params, sections, axes, rotary_dim);
     if (status != FA_STATUS_OK) return status;
     if (tokens == 0) return FA_STATUS_OK;
     if (q == nullptr || k == nullptr || v == nullptr || q_out == nullptr || k_cache == nullptr || v_cache == nullptr ||
         positions == nullptr || slots == nullptr || inv_freq == nullptr)
         return FA_STATUS_INVALID_ARGUMENT;
     if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(q_out) || misaligned(k_cache) ||
-        misaligned(v_cache) || !multiple_of_8(strides, 14))
+        misaligned(v_cache))
         return FA_STATUS_MISALIGNED;
+    if ((status = check_strides(strides, 14)) != FA_STATUS_OK) return status;
     params.src[0] = static_cast<const __nv_bfloat16*>(q);
     params.src[1] = static_cast<const __nv_bfloat16*>(k);
     params.src[2] = static_cast<const __nv_bfloat16*>(v);

@@ -118,6 +118,12 @@ FA_API int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void
                               void* o, const long long* strides, void* workspace, size_t workspace_bytes,
                               void* stream);
 
+/* Test-only: this host thread's next fa_sm100_paged_fwd stalls on the device: the warps that hand out its
+ * work wait on a barrier nothing arrives on, for the limit of one second. It must give up, report
+ * FA_STATUS_DEVICE_TIMEOUT through fa_sm100_device_status, and leave the context usable; its output is
+ * not written. */
+FA_API int fa_sm100_paged_test_arm_stall(void);
+
 /* Workspace of fa_sm100_paged_fwd for a plan of these sizes on the current device. */
 FA_API size_t fa_sm100_paged_workspace_bytes(const FaPagedPlan* plan);
 

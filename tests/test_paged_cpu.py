@@ -54,6 +54,7 @@ def test_c_refusals(lib):
     plan = ctypes.byref(_plan())
     good = (ctypes.c_longlong * 10)(*[128] * 10)
     odd = (ctypes.c_longlong * 10)(*[128] * 9, 132)
+    back = (ctypes.c_longlong * 10)(*[128] * 9, -128)
     assert lib.fa_sm100_paged_plan(None, 0x1000, 0x1000, 0x1000, 4, None, None) == 1001
     assert lib.fa_sm100_paged_plan(plan, None, 0x1000, 0x1000, 4, None, None) == 1001
     assert lib.fa_sm100_paged_plan(plan, 0x1000, None, 0x1000, 4, None, None) == 1001
@@ -66,6 +67,7 @@ def test_c_refusals(lib):
         assert fwd(plan, *[0x1008 if j == i else 0x1000 for j in range(4)], good, None, 0, None) == 1003
     assert fwd(plan, 0x1000, 0x1000, 0x1000, 0x1000, None, None, 0, None) == 1001
     assert fwd(plan, 0x1000, 0x1000, 0x1000, 0x1000, odd, None, 0, None) == 1003
+    assert fwd(plan, 0x1000, 0x1000, 0x1000, 0x1000, back, None, 0, None) == 1001
     assert fwd(ctypes.byref(_plan(total_tokens=0)), None, None, None, None, good, None, 0, None) == 0
     assert lib.fa_sm100_paged_schedule_bytes(3) == 64 and lib.fa_sm100_paged_schedule_bytes(-1) == 0
 
@@ -85,6 +87,7 @@ def test_c_rotary_refusals(lib):
                 dict(rot=64), dict(sec=(ctypes.c_int * 4)(-8, 48, 24, 0))):
         assert call(**bad) == 1001, bad
     assert call(x=0x1008) == 1003 and call(xs=odd) == 1003
+    assert call(xs=(ctypes.c_longlong * 3)(128, -128, 128)) == 1001
 
     strides = (ctypes.c_longlong * 14)(*[128] * 14)
 

@@ -546,6 +546,22 @@ def test_empty_calls(cuda_device):
         check_attention(Requests(cached, new, 16, cuda_device, padding=padding), 4, 2, 64)
 
 
+@pytest.mark.parametrize("new", [[1, 1], [100, 40], [1, 100]])
+def test_a_stalled_launch_gives_up(cuda_device, new):
+    """A wait that runs out: an error status, nothing written, and the next call is right."""
+    r = Requests([700, 90], new, 16, cuda_device)
+    q, (k, v), plan, want = check_attention(r, 8, 2, 128)
+    out = torch.full_like(want, 9.0)
+    assert _lib.load().fa_sm100_paged_test_arm_stall() == 0
+    fa.paged_attention(q, k, v, plan, out=out)
+    status, word = fa.device_status()
+    assert status == fa.STATUS_DEVICE_TIMEOUT and word & 1
+    assert (out == 9.0).all()
+    status_ok()
+    assert torch.equal(fa.paged_attention(q, k, v, plan), want)
+    status_ok()
+
+
 # ---------------------------------------------------------------------------
 # Streams, graphs, and the operators together
 # ---------------------------------------------------------------------------
