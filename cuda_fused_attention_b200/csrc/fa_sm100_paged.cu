@@ -1337,6 +1337,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 // dependent launch): about 3 us behind the narrow kernel; behind the wide one, whose parts are 256 rows,
 // 5 us for 40 MB of parts at D = 128.
 constexpr int kCombineThreads = 128;
+constexpr int kCombineColumns = 32;         // wide: columns of a thread
 
 // One row per warp; a lane has D / 32 columns.
 template <int D, int MT>
@@ -1394,59 +1395,6 @@ __device__ __forceinline__ void combine_narrow(const PagedParams& p, int cta, in
         *reinterpret_cast<uint32_t*>(out + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
 }
 
-// A thread is a query row and takes 32 columns (group c) of Q tile t.
-template <int D>
-__device__ __forceinline__ void combine_wide(const PagedParams& p, int cta, int t, int c)
-{
-    using C = WideCfg<D>;
-    const Merge merge = p.wide_merges[cta];
-    const int group = p.plan.heads / p.plan.kv_heads, per_tile = tokens_per_tile(group);
-    const int r = threadIdx.x, tok = t * per_tile + r / group;
-    if (merge.parts == 0 || r >= per_tile * group || tok >= merge.tokens) return;
-    const float* first = p.wide_partial + ((2LL * cta + 1) * 2 + t) * C::kPartTileFloats;
-    auto part = [&](int i) { return i == 0 ? first : first + (2LL * i - 1) * 2 * C::kPartTileFloats; };
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int i = 0; i < merge.parts; ++i) top = fmaxf(top, part(i)[D * kWideRows + r]);
-    float4 acc[8] = {};
-    float sum = 0.0f;
-    for (int i = 0; i < merge.parts; ++i) {
-        const float* at = part(i);
-        const float m = at[D * kWideRows + r];
-        const float w = m == -INFINITY ? 0.0f : ex2_approx((m - top) * p.scale_log2);
-        sum += w * at[D * kWideRows + kWideRows + r];
-        const float4* columns = reinterpret_cast<const float4*>(at) + c * 8 * kWideRows + r;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const float4 v = columns[q * kWideRows];
-            acc[q].x += w * v.x;
-            acc[q].y += w * v.y;
-            acc[q].z += w * v.z;
-            acc[q].w += w * v.w;
-        }
-    }
-    const float inv = 1.0f / sum;
-    __nv_bfloat16* out = p.o + static_cast<long long>(merge.token0 + tok) * p.o_token +
-                         static_cast<long long>(merge.head0 + r % group) * p.o_head + c * 32;
-#pragma unroll
-    for (int q = 0; q < 8; q += 2)
-        *reinterpret_cast<uint4*>(out + q * 4) =
-            make_uint4(pack_bf16x2(acc[q].x * inv, acc[q].y * inv), pack_bf16x2(acc[q].z * inv, acc[q].w * inv),
-                       pack_bf16x2(acc[q + 1].x * inv, acc[q + 1].y * inv), pack_bf16x2(acc[q + 1].z * inv, acc[q + 1].w * inv));
-}
-
-// A block per CTA of the wide kernel, Q tile and 32 columns.
-template <int D>
-__global__ void __launch_bounds__(kCombineThreads)
-paged_combine_wide_kernel(const __grid_constant__ PagedParams p)
-{
-    constexpr int kPieces = 2 * (D / 32);
-    const int block = static_cast<int>(blockIdx.x);
-    grid_dependents_launch();
-    grid_dependency_wait();
-    combine_wide<D>(p, block / kPieces, block % kPieces / (D / 32), block % (D / 32));
-}
-
 // A block per CTA of the narrow kernel and four rows.
 template <int D, int MT>
 __global__ void __launch_bounds__(kCombineThreads)
@@ -1456,6 +1404,53 @@ paged_combine_narrow_kernel(const __grid_constant__ PagedParams p)
     const int block = static_cast<int>(blockIdx.x);
     grid_dependency_wait();
     combine_narrow<D, MT>(p, block / kRowBlocks, block % kRowBlocks * kWarps + static_cast<int>(threadIdx.x) / 32);
+}
+
+// A block per CTA of the wide kernel, Q tile and group of columns; a thread is a query row.
+template <int D>
+__global__ void __launch_bounds__(kCombineThreads)
+paged_combine_wide_kernel(const __grid_constant__ PagedParams p)
+{
+    using C = WideCfg<D>;
+    constexpr int kGroups = D / kCombineColumns, kQuads = kCombineColumns / 4;
+    const int block = static_cast<int>(blockIdx.x), cta = block / (2 * kGroups), t = block / kGroups % 2, c = block % kGroups;
+    const int group = p.plan.heads / p.plan.kv_heads, per_tile = tokens_per_tile(group);
+    const int r = threadIdx.x, tok = t * per_tile + r / group;
+    grid_dependents_launch();
+    grid_dependency_wait();
+    const Merge merge = p.wide_merges[cta];
+    if (merge.parts == 0 || r >= per_tile * group || tok >= merge.tokens) return;
+    const float* first = p.wide_partial + ((2LL * cta + 1) * 2 + t) * C::kPartTileFloats;
+    auto part = [&](int i) { return i == 0 ? first : first + (2LL * i - 1) * 2 * C::kPartTileFloats; };
+    float top = -INFINITY;
+#pragma unroll 8
+    for (int i = 0; i < merge.parts; ++i) top = fmaxf(top, part(i)[D * kWideRows + r]);
+    float4 acc[kQuads] = {};
+    float sum = 0.0f;
+#pragma unroll 2
+    for (int i = 0; i < merge.parts; ++i) {
+        const float* at = part(i);
+        const float m = at[D * kWideRows + r];
+        const float w = m == -INFINITY ? 0.0f : ex2_approx((m - top) * p.scale_log2);
+        sum += w * at[D * kWideRows + kWideRows + r];
+        const float4* columns = reinterpret_cast<const float4*>(at) + c * kQuads * kWideRows + r;
+#pragma unroll
+        for (int q = 0; q < kQuads; ++q) {
+            const float4 v = columns[q * kWideRows];
+            acc[q].x += w * v.x;
+            acc[q].y += w * v.y;
+            acc[q].z += w * v.z;
+            acc[q].w += w * v.w;
+        }
+    }
+    const float inv = 1.0f / sum;
+    __nv_bfloat16* out = p.o + static_cast<long long>(merge.token0 + tok) * p.o_token +
+                         static_cast<long long>(merge.head0 + r % group) * p.o_head + c * kCombineColumns;
+#pragma unroll
+    for (int q = 0; q < kQuads; q += 2)
+        *reinterpret_cast<uint4*>(out + q * 4) =
+            make_uint4(pack_bf16x2(acc[q].x * inv, acc[q].y * inv), pack_bf16x2(acc[q].z * inv, acc[q].w * inv),
+                       pack_bf16x2(acc[q + 1].x * inv, acc[q + 1].y * inv), pack_bf16x2(acc[q + 1].z * inv, acc[q + 1].w * inv));
 }
 
 }  // namespace fa_sm100
@@ -1640,7 +1635,8 @@ int launch_attention(const PagedMaps& maps, const PagedParams& params, bool wide
         status = launch(paged_wide_kernel<D>, sms, kWideThreads, WideCfg<D>::kSmemBytes, false, stream, maps.q, maps.wide_k,
                         maps.wide_v, params);
         if (status == FA_STATUS_OK)
-            status = launch(paged_combine_wide_kernel<D>, sms * 2 * (D / 32), kCombineThreads, 0, true, stream, params);
+            status = launch(paged_combine_wide_kernel<D>, sms * 2 * (D / kCombineColumns), kCombineThreads, 0, true, stream,
+                            params);
     }
     if (!narrow || status != FA_STATUS_OK) return status;
     const int ctas = narrow_ctas(sms);
