@@ -47,7 +47,6 @@ struct Merge {
 // A row keeps its exponent base until a score exceeds it by this much in the exp2 domain.
 constexpr float kRebase = 16.0f;
 
-
 // =============================================================================
 // Narrow kernel: requests of few query rows per K/V head (decode steps, drafted tokens)
 // =============================================================================
@@ -583,7 +582,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 }
 
 // =============================================================================
-// Wide kernel: requests of more than 16 query rows per K/V head (chunks of tokens)
+// Wide kernel: requests of more query rows per K/V head than the narrow kernel takes (chunks of tokens)
 // =============================================================================
 // The query rows of a K/V head (token * group + head in group) are taken 128 at a time as the M
 // of tcgen05 products, so that all heads of a group share each K/V tile; a block is two such
@@ -592,8 +591,8 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 // pipe and the exponentials bound it, not memory. The work of all requests, K/V heads and blocks
 // is one line of 128-key tiles (request, head, block, key; each block preceded by kWideGap idle units
 // that stand for its set-up and epilogue) of which each of the grid's CTAs (one per SM, persistent)
-// takes an equal stretch; blocks that cross a border are merged from parts. Within a CTA the K/V ring runs on across blocks, the first products of a
-// block overlap the epilogue of the one before.
+// takes an equal stretch; blocks that cross a border are merged from parts. Within a CTA the K/V ring
+// runs on across blocks, and the first products of a block overlap the epilogue of the one before.
 //
 // Warps: 0-3 and 4-7 softmax, O correction and epilogue of Q tile 0 and 1 (one thread per row);
 // 8 MMA issuer; 9 and 10 TMA producers of Q and K and of V; 11 walks the line, hands out the segments,
@@ -1495,8 +1494,9 @@ int validate_plan(const FaPagedPlan* plan)
     if (plan->num_seqs < 0 || plan->total_tokens < 0 || plan->max_new < 0 || plan->num_pages < 0 ||
         plan->table_width < 0 || plan->table_stride < plan->table_width)
         return FA_STATUS_INVALID_ARGUMENT;
+    // Slots are 32-bit; positions leave room for a tile behind the last key.
     if (static_cast<long long>(plan->num_pages) * plan->page_size > INT_MAX ||
-        static_cast<long long>(plan->table_width) * plan->page_size > INT_MAX)
+        static_cast<long long>(plan->table_width) * plan->page_size > (1 << 30))
         return FA_STATUS_INVALID_ARGUMENT;
     if (plan->query_start == nullptr || plan->free_cursor == nullptr || plan->schedule == nullptr)
         return FA_STATUS_INVALID_ARGUMENT;

@@ -266,8 +266,9 @@ PyObject* plan(PyObject* const* args, Py_ssize_t count)
     if (!PyTuple_Check(args[5]) || PyTuple_GET_SIZE(args[5]) != 4) bad_type("shape must be a PagedShape");
     long long shape[4];
     for (int i = 0; i < 4; ++i) shape[i] = integer(PyTuple_GET_ITEM(args[5], i), "shape");
-    if (num_pages * shape[3] > kIntMax || width * shape[3] > kIntMax || stride > kIntMax || seqs > kIntMax / 4)
-        bad_value("a cache, and a table row, must hold fewer than 2^31 tokens");
+    if (num_pages > kIntMax || num_pages * shape[3] > kIntMax || stride > kIntMax || seqs > kIntMax / 4)
+        bad_value("a cache must hold fewer than 2^31 tokens");
+    if (width * shape[3] > (1LL << 30)) bad_value("a table row must hold at most 2^30 tokens");
     OneDevice device;
     device.add(cached, "cached_lens");
     device.add(fresh, "new_lens");

@@ -50,7 +50,7 @@ typedef struct FaPagedPlan {
     int total_tokens;           /* rows of the packed token axis */
     int max_new;                /* no request brings more new tokens than this */
     int num_pages;              /* pages of the cache; num_pages * page_size < 2^31 */
-    int table_width;            /* pages a table row has room for */
+    int table_width;            /* pages a table row has room for; table_width * page_size <= 2^30 */
     int table_stride;           /* elements between table rows, >= table_width */
     int heads;                  /* query heads */
     int kv_heads;               /* K/V heads; divides heads, heads / kv_heads <= 128 */
