@@ -1003,7 +1003,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 const bool two = segments[sg & 1].tokens > per_tile;
                 release_segment(sg);
                 if (count == 0) break;
-                if (lane == 0) {
+                if (elect_one()) {
                     ok = wait(C::kBarQFull, sg & 1, kSiteWideQ) && wait_ring(ri, kSiteWideK);
                     if (ok) {
                         tc_fence_after();
@@ -1011,9 +1011,9 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                         ri += 2 * count;
                     }
                 }
-                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                ok = __all_sync(0xffffffffu, ok);
             }
-            if (lane == 0) {
+            if (elect_one()) {
                 // Every MMA issued above must finish before tensor memory is released.
                 umma_commit(bar(C::kBarDrain));
                 drain_paged(bar(C::kBarDrain), 0);
