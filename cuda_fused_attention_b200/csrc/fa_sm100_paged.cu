@@ -597,12 +597,16 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 // Warps: 0-3 and 4-7 softmax, O correction and epilogue of Q tile 0 and 1 (one thread per row);
 // 8 MMA issuer; 9 and 10 TMA producers of Q and K and of V; 11 walks the line, hands out the segments,
 // and zeroes what V's last page holds behind the last key (a weight of zero does not silence a NaN).
-// Tensor memory, barriers per key tile and the lazily moved exponent base are those of the dense
-// kernel (fa_sm100.cu); a block of at most 128 rows has its S double-buffered. P is rounded to bf16 for
-// the product with V, as in the dense kernel: a second product for the rest would cost the tensor
-// pipe a third more. Measured (B200, 32/8 heads, D = 128): 2048 new tokens behind 14336 cached 445 us,
-// 1158 TFLOP/s; a prompt of 8192 tokens without mask (16 heads) 490 us, as the dense kernel; 16
-// requests of 16 new tokens (64 rows) behind up to 8192 74 us, 4.1 TB/s.
+// The lazily moved exponent base is that of the dense kernel (fa_sm100.cu); tensor memory is not. A softmax
+// warpgroup reads its whole S into registers at once, so S is free long before P is written. P has columns of its
+// own here, and Q K^T of the next key tile runs during the softmax of this one: at D = 64 each Q tile has its
+// S, at D = 128, where S, P and O of two tiles would not fit, the two take turns with one. What bounds the kernel now is
+// the softmax: about 3400 cycles per key tile of a block of two Q tiles, of which the special-function
+// unit needs 2048 (a part of the exponentials as cubics on the FMA pipe was slower: 403 us against 394). P is rounded to
+// bf16 for the product with V, as in the dense kernel: a second product for the rest would cost the tensor
+// pipe a third more. Measured (B200, 32/8 heads, D = 128): 2048 new tokens behind 14336 cached 390 us,
+// 1320 TFLOP/s, with S and P in the same columns 405; a causal prompt of 8192 tokens 435 us (455); 16
+// requests of 16 new tokens (64 rows) behind up to 8192 71 us, 4.3 TB/s.
 constexpr int kWideThreads = 384;
 constexpr int kWideMinUnits = 4;        // units a CTA takes at least, more than a tile's (256 new tokens: 19.4 us; 8: 22.3)
 // 216 / 72 registers made the MMA issuer spill, and a load by it waits for its queued MMAs: 493 us against 462 (chunk
@@ -626,15 +630,15 @@ struct WideCfg {
     static constexpr int kBarOff = kRingOff + kStages * kTileBytes;
     static constexpr int kBarQFull = 0, kBarQEmpty = 1;
     static constexpr int kBarKvFull = 2, kBarKvEmpty = 2 + kStages;
-    // Three sets of S, P-half and P barriers: Q tile 0's (in a block of one Q tile, its even key tiles'), Q tile
-    // 1's, and that of the odd key tiles of a block of one Q tile. Q tile 1's are its own because a warpgroup that
-    // sits a block out must not have to follow their phases.
+    // Per Q tile, each completed once per key tile: S computed, S read (by a lane of each warp), half of P written,
+    // P written, the product of that half with V done, the whole product done.
     static constexpr int kBarSFull = 2 + 2 * kStages;
-    static constexpr int kBarPHalf = kBarSFull + 3;
-    static constexpr int kBarPFull = kBarPHalf + 3;
-    static constexpr int kBarPvHalf = kBarPFull + 3;            // per Q tile
-    static constexpr int kBarOFull = kBarPvHalf + 2;
-    static constexpr int kBarTail = kBarOFull + 2;              // per ring slot: a V tile to be zeroed in part has landed
+    static constexpr int kBarSRead = kBarSFull + 2;
+    static constexpr int kBarPHalf = kBarSRead + 2;
+    static constexpr int kBarPFull = kBarPHalf + 2;
+    static constexpr int kBarPvHalf = kBarPFull + 2;
+    static constexpr int kBarPvFull = kBarPvHalf + 2;
+    static constexpr int kBarTail = kBarPvFull + 2;              // per ring slot: a V tile to be zeroed in part has landed
     static constexpr int kBarDrain = kBarTail + kStages;
     static constexpr int kBarSchedFull = kBarDrain + 1;
     static constexpr int kBarSchedEmpty = kBarSchedFull + 2;
@@ -645,7 +649,8 @@ struct WideCfg {
     static constexpr int kStageStride = 80;
     static constexpr int kStageOff = kSegOff + 2 * 64;
     static constexpr int kSmemBytes = kStageOff + 8 * 32 * kStageStride + 1024;
-    static constexpr uint32_t kColS0 = 0, kColS1 = 128, kColO0 = 256, kColO1 = 256 + D;
+    static constexpr bool kOwnS = D == 64;                      // S of Q tile 1 in columns of its own
+    static constexpr uint32_t kColS0 = 0, kColS1 = D == 64 ? 384 : 0, kColP0 = 128, kColP1 = 192, kColO0 = 256, kColO1 = 256 + D;
     static constexpr uint32_t kIdescQK = make_idesc_bf16(kWideRows, kWideKeys, false);
     static constexpr uint32_t kIdescPV = make_idesc_bf16(kWideRows, D, true);
     // A part: per Q tile O as [D / 4][128 rows] of float4, then 128 maxima and 128 sums.
@@ -790,6 +795,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     if (warp == 0) {
         for (int i = lane; i < C::kNumBars; i += 32) {
             uint32_t count = 1;
+            if (i >= C::kBarSRead && i < C::kBarPHalf) count = 4;
             if (i >= C::kBarPHalf && i < C::kBarPvHalf) count = 128;
             if (i >= C::kBarSchedEmpty) count = kReaders;
             mbar_init(bar(i), count);
@@ -901,59 +907,57 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             // ======================= MMA issuer ================================
             // Anything but MMAs that this thread does waits until the MMAs it has queued are done, so all it
             // needs is in registers before a segment's loop.
-            const uint32_t t_s0 = tmem_base + C::kColS0, t_s1 = tmem_base + C::kColS1;
+            const uint32_t t_s = tmem_base + C::kColS0, t_s1 = tmem_base + C::kColS1, t_p0 = tmem_base + C::kColP0, t_p1 = tmem_base + C::kColP1;
             const uint32_t t_o0 = tmem_base + C::kColO0, t_o1 = tmem_base + C::kColO1;
             const uint32_t q0 = desc_low(base, 16), q1 = desc_low(base + C::kTileBytes, 16);
             const uint32_t k_ring = desc_low(ring, 16), v_ring = desc_low(ring, C::kSubBytes);
             auto in_slot = [](uint32_t low, int i) { return low + static_cast<uint32_t>(i % C::kStages) * (C::kTileBytes >> 4); };
             auto empty_bar = [&](int i) -> uint32_t { return bar(C::kBarKvEmpty + i % C::kStages); };
             int ri = 0;                         // ring index of the segment's first K tile
-            uint32_t par0 = 0, par1 = 0, par2 = 0;      // parities of the three sets of per-key-tile barriers
+            uint32_t par0 = 0, par1 = 0;        // parities of the Q tiles' barriers
             bool ok = true;
             auto wait = [&](int index, uint32_t parity, uint32_t site) { return wait_paged(bar(index), parity, abort_flag, site); };
             auto wait_ring = [&](int i, uint32_t site) {
                 return wait_paged(bar(C::kBarKvFull + i % C::kStages), (i / C::kStages) & 1, abort_flag, site);
             };
-            // The products of a segment of one Q tile. Its S is double-buffered (key tile j in S_(j & 1)): Q K^T of the
-            // next key tile runs during the softmax of this one.
+            // The products of a segment of one Q tile: Q K^T of the next key tile is issued once S of this one is read.
             auto issue_one = [&](int count) -> bool {
-                wide_issue_qk<D>(t_s0, q0, in_slot(k_ring, ri));
+                wide_issue_qk<D>(t_s, q0, in_slot(k_ring, ri));
                 umma_commit(bar(C::kBarSFull + 0));
                 umma_commit(empty_bar(ri));
                 if (count == 1) umma_commit(bar(C::kBarQEmpty));
                 for (int j = 0; j < count; ++j) {
                     const int vi = ri + 2 * j + 1, ki = vi + 1;
-                    const bool odd = (j & 1) != 0;
-                    const int set = odd ? 2 : 0;
-                    const uint32_t t_sj = odd ? t_s1 : t_s0, parity = odd ? par2 : par0;
                     if (j + 1 < count) {
                         if (!wait_ring(ki, kSiteWideK)) return false;
+                        if (!wait(C::kBarSRead + 0, par0, kSiteWideP)) return false;
                         tc_fence_after();
-                        wide_issue_qk<D>(odd ? t_s0 : t_s1, q0, in_slot(k_ring, ki));
-                        umma_commit(bar(C::kBarSFull + (set ^ 2)));
+                        wide_issue_qk<D>(t_s, q0, in_slot(k_ring, ki));
+                        umma_commit(bar(C::kBarSFull + 0));
                         umma_commit(empty_bar(ki));
                         if (j + 2 == count) umma_commit(bar(C::kBarQEmpty));
                     }
                     if (!wait_ring(vi, kSiteWideV)) return false;
-                    if (!wait(C::kBarPHalf + set, parity, kSiteWideP)) return false;
+                    if (!wait(C::kBarPHalf + 0, par0, kSiteWideP)) return false;
                     tc_fence_after();
-                    wide_issue_pv<D, 0, 4>(t_o0, t_sj, in_slot(v_ring, vi), j > 0);
+                    wide_issue_pv<D, 0, 4>(t_o0, t_p0, in_slot(v_ring, vi), j > 0);
                     umma_commit(bar(C::kBarPvHalf + 0));
-                    if (!wait(C::kBarPFull + set, parity, kSiteWideP)) return false;
+                    if (!wait(C::kBarPFull + 0, par0, kSiteWideP)) return false;
                     tc_fence_after();
-                    wide_issue_pv<D, 4, 8>(t_o0, t_sj, in_slot(v_ring, vi), true);
+                    wide_issue_pv<D, 4, 8>(t_o0, t_p0, in_slot(v_ring, vi), true);
+                    umma_commit(bar(C::kBarPvFull + 0));
                     umma_commit(empty_bar(vi));
-                    umma_commit(bar(C::kBarPvHalf + 1));
-                    if (j + 1 == count) umma_commit(bar(C::kBarOFull + 0));
-                    if (odd) par2 ^= 1u;
-                    else par0 ^= 1u;
+                    par0 ^= 1u;
                 }
                 return true;
             };
-            // The products of a segment of two Q tiles.
+            // The products of a segment of two Q tiles. Where they take turns with S, tile 1's Q K^T follows when tile 0
+            // has read its S, tile 0's of the next key tile when tile 1 has.
             auto issue_two = [&](int count) -> bool {
-                wide_issue_qk<D>(t_s0, q0, in_slot(k_ring, ri));
+                wide_issue_qk<D>(t_s, q0, in_slot(k_ring, ri));
                 umma_commit(bar(C::kBarSFull + 0));
+                if (!C::kOwnS && !wait(C::kBarSRead + 0, par0, kSiteWideP)) return false;
+                tc_fence_after();
                 wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ri));
                 umma_commit(bar(C::kBarSFull + 1));
                 umma_commit(empty_bar(ri));
@@ -961,38 +965,41 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 for (int j = 0; j < count; ++j) {
                     const int vi = ri + 2 * j + 1, ki = vi + 1;
                     const bool more = j + 1 < count;
+                    if (more) {
+                        if (!wait_ring(ki, kSiteWideK)) return false;
+                        if (!wait(C::kBarSRead + (C::kOwnS ? 0 : 1), C::kOwnS ? par0 : par1, kSiteWideP)) return false;
+                        tc_fence_after();
+                        wide_issue_qk<D>(t_s, q0, in_slot(k_ring, ki));
+                        umma_commit(bar(C::kBarSFull + 0));
+                    }
                     if (!wait_ring(vi, kSiteWideV)) return false;
                     if (!wait(C::kBarPHalf + 0, par0, kSiteWideP)) return false;
                     tc_fence_after();
-                    wide_issue_pv<D, 0, 4>(t_o0, t_s0, in_slot(v_ring, vi), j > 0);
+                    wide_issue_pv<D, 0, 4>(t_o0, t_p0, in_slot(v_ring, vi), j > 0);
                     umma_commit(bar(C::kBarPvHalf + 0));
                     if (!wait(C::kBarPFull + 0, par0, kSiteWideP)) return false;
                     tc_fence_after();
-                    wide_issue_pv<D, 4, 8>(t_o0, t_s0, in_slot(v_ring, vi), true);
+                    wide_issue_pv<D, 4, 8>(t_o0, t_p0, in_slot(v_ring, vi), true);
+                    umma_commit(bar(C::kBarPvFull + 0));
                     par0 ^= 1u;
-                    if (!more) umma_commit(bar(C::kBarOFull + 0));
                     if (more) {
-                        if (!wait_ring(ki, kSiteWideK)) return false;
+                        if (!wait(C::kBarSRead + (C::kOwnS ? 1 : 0), C::kOwnS ? par1 : par0, kSiteWideP)) return false;
                         tc_fence_after();
-                        wide_issue_qk<D>(t_s0, q0, in_slot(k_ring, ki));
-                        umma_commit(bar(C::kBarSFull + 0));
+                        wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ki));
+                        umma_commit(bar(C::kBarSFull + 1));
+                        umma_commit(empty_bar(ki));
+                        if (j + 2 == count) umma_commit(bar(C::kBarQEmpty));    // the segment's last S is on its way
                     }
                     if (!wait(C::kBarPHalf + 1, par1, kSiteWideP)) return false;
                     tc_fence_after();
-                    wide_issue_pv<D, 0, 4>(t_o1, t_s1, in_slot(v_ring, vi), j > 0);
+                    wide_issue_pv<D, 0, 4>(t_o1, t_p1, in_slot(v_ring, vi), j > 0);
                     umma_commit(bar(C::kBarPvHalf + 1));
                     if (!wait(C::kBarPFull + 1, par1, kSiteWideP)) return false;
                     tc_fence_after();
-                    wide_issue_pv<D, 4, 8>(t_o1, t_s1, in_slot(v_ring, vi), true);
-                    par1 ^= 1u;
+                    wide_issue_pv<D, 4, 8>(t_o1, t_p1, in_slot(v_ring, vi), true);
+                    umma_commit(bar(C::kBarPvFull + 1));
                     umma_commit(empty_bar(vi));
-                    if (!more) umma_commit(bar(C::kBarOFull + 1));
-                    if (more) {
-                        wide_issue_qk<D>(t_s1, q1, in_slot(k_ring, ki));
-                        umma_commit(bar(C::kBarSFull + 1));
-                    }
-                    if (more) umma_commit(empty_bar(ki));
-                    if (j + 2 == count) umma_commit(bar(C::kBarQEmpty));    // the segment's last S is on its way
+                    par1 ^= 1u;
                 }
                 return true;
             };
@@ -1079,13 +1086,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const int quarter = warp % 4;
         const int r = quarter * 32 + lane;         // row within the Q tile == tensor-memory lane
         const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-        const uint32_t t_s0 = lane_base + C::kColS0;
+        const uint32_t t_s = lane_base + (t == 0 ? C::kColS0 : C::kColS1);
+        const uint32_t t_p = lane_base + (t == 0 ? C::kColP0 : C::kColP1);
         const uint32_t t_o = lane_base + (t == 0 ? C::kColO0 : C::kColO1);
         const int tok = t * per_tile + r / group;       // token of this row within its block
         const float sl2 = p.scale_log2;
         const uint64_t c2 = f2_pack(sl2, sl2);
-        // Parities: of the barrier sets (one bit each); of PvHalf, which completes once per key tile; of OFull.
-        uint32_t sets = 0, pv_phase = 0, o_phase = 0;
+        uint32_t phase = 0;     // parity of this Q tile's barriers
 
         auto rescale_o = [&](float scale) {
             const uint64_t a2 = f2_pack(scale, scale);
@@ -1105,7 +1112,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 tmem_st32(t_o + static_cast<uint32_t>(c * 32), o);
             }
         };
-        // 64 scores on base `mb`: P as bf16 pairs to tensor memory, the 32-bit sum and the raw maximum.
+        // 64 scores on base `mb`: P as bf16 pairs, the 32-bit sum and the raw maximum.
         auto exp_half = [&](const uint32_t (&lo)[32], const uint32_t (&hi)[32], float mb, float& half_sum, float& half_max,
                             uint32_t p_tmem) {
             const uint64_t nb2 = f2_pack(-mb, -mb);
@@ -1148,7 +1155,6 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             const bool one = seg.tokens <= per_tile;    // this block has one Q tile
             if (t == 1 && one) {
                 release_segment(sg);
-                pv_phase ^= count & 1;
                 continue;
             }
             const int tile = seg.tile;
@@ -1156,10 +1162,8 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             // First key tile of the stretch that some row of this Q tile must not see all of.
             const int mask_from = (plan.causal ? seg.pos0 + t * per_tile + 1 : seg.kv) / kWideKeys - tile;
             float row_max = -INFINITY, row_sum = 0.0f, m_base = 0.0f;
-            for (int j = 0; j < count; ++j, pv_phase ^= 1u) {
-                const int set = one ? 2 * (j & 1) : t;
-                const uint32_t t_s = t_s0 + (set ? C::kColS1 - C::kColS0 : 0u);
-                ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarSFull + set), sets >> set & 1u, abort_flag, kSiteWideS));
+            for (int j = 0; j < count; ++j, phase ^= 1u) {
+                ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarSFull + t), phase, abort_flag, kSiteWideS));
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t sc[4][32];
@@ -1172,6 +1176,9 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 reg_fence32(sc[1]);
                 reg_fence32(sc[2]);
                 reg_fence32(sc[3]);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(C::kBarSRead + t));
                 const int key0 = (tile + j) * kWideKeys;
                 if (j >= mask_from && __any_sync(0xffffffffu, limit < key0 + kWideKeys - 1)) {
 #pragma unroll
@@ -1195,11 +1202,17 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     row_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                     m_base = row_max == -INFINITY ? 0.0f : row_max * sl2;
                 }
+                if (j > 0) {
+                    // O and P are the previous tile's until its product with V is done.
+                    ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarPvFull + t), phase ^ 1u, abort_flag, kSiteWideO));
+                    if (!ok) break;
+                    tc_fence_after();
+                }
                 float o_scale = 1.0f;       // O correction owed before the first PV of this tile reads O
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float hsum, hmax;
-                    exp_half(sc[2 * h], sc[2 * h + 1], m_base, hsum, hmax, t_s + static_cast<uint32_t>(32 * h));
+                    exp_half(sc[2 * h], sc[2 * h + 1], m_base, hsum, hmax, t_p + static_cast<uint32_t>(32 * h));
                     const bool need = (hmax - row_max) * sl2 > kRebase;
                     if (__any_sync(0xffffffffu, need)) {
                         const float m_new = need ? hmax : row_max;
@@ -1212,44 +1225,26 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                         } else {
                             // The first-half PV of this tile may be running on the old base: let it finish, then
                             // correct O, its contribution included.
-                            if (one && j > 0) {     // (a phase is only told from the one before: that one has to be over)
-                                ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarPvHalf + 1), pv_phase ^ 1u, abort_flag, kSiteWideO));
-                                if (!ok) break;
-                            }
-                            ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarPvHalf + t), pv_phase, abort_flag, kSiteWideO));
+                            ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarPvHalf + t), phase, abort_flag, kSiteWideO));
                             if (!ok) break;
                             tc_fence_after();
                             rescale_o(alpha);
                         }
-                        exp_half(sc[2 * h], sc[2 * h + 1], m_base, hsum, hmax, t_s + static_cast<uint32_t>(32 * h));
+                        exp_half(sc[2 * h], sc[2 * h + 1], m_base, hsum, hmax, t_p + static_cast<uint32_t>(32 * h));
                     }
                     row_sum += hsum;
-                    if (h == 0) {
-                        if (j > 0 && __any_sync(0xffffffffu, o_scale != 1.0f)) {
-                            if (one) {      // S of this tile can be ready before the PV of the one before is done
-                                ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarPvHalf + 1), pv_phase ^ 1u, abort_flag, kSiteWideO));
-                                if (!ok) break;
-                                tc_fence_after();
-                            }
-                            rescale_o(o_scale);
-                        }
-                        tmem_wait_st();
-                        tc_fence_before();
-                        mbar_arrive(bar(C::kBarPHalf + set));
-                    }
+                    if (h == 0 && j > 0 && __any_sync(0xffffffffu, o_scale != 1.0f)) rescale_o(o_scale);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(bar((h == 0 ? C::kBarPHalf : C::kBarPFull) + t));
                 }
                 if (!ok) break;
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(bar(C::kBarPFull + set));
-                sets ^= 1u << set;
             }
             if (!ok) break;
 
             // ---- epilogue: O from tensor memory, to its rows or to this stretch's part ----
-            ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarOFull + t), o_phase, abort_flag, kSiteWideO));
+            ok = __all_sync(0xffffffffu, wait_paged(bar(C::kBarPvFull + t), phase ^ 1u, abort_flag, kSiteWideO));
             if (!ok) break;
-            o_phase ^= 1u;
             tc_fence_after();
             const int part = seg.part;
             // A row of 32 columns is 64 bytes: staged in shared memory, four lanes write one row, so that a warp's
