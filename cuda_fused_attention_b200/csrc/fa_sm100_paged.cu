@@ -28,6 +28,7 @@ struct PagedParams {
     long long k_page, k_head, k_row, v_page, v_head, v_row;
     int page_shift;
     float scale_log2;
+    int behind_wide;            // narrow kernel: the wide one of the same call was launched before it
     int inject_stall;           // test only: the warps that hand out work wait on a barrier nothing arrives on
     // Parts of items that cross a border between CTAs' ranges, two places per CTA, and per CTA what is to be
     // merged from the second place on; for the narrow and for the wide kernel.
@@ -213,11 +214,8 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 {
     using C = NarrowCfg<D, MT>;
     const FaPagedPlan& plan = p.plan;
-    const long long* start = narrow_starts(plan.schedule, plan.num_seqs);
-    const long long total = start[plan.num_seqs] * plan.kv_heads;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int group = plan.heads / plan.kv_heads;
-    grid_dependents_launch();
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
@@ -238,6 +236,11 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         if (lane == 0) *abort_flag = 0u;
         fence_mbarrier_init();
     }
+    // Behind the wide kernel of the same call, which has waited, there is nothing to wait for before the end.
+    if (!p.behind_wide) grid_dependency_wait();
+    grid_dependents_launch();
+    const long long* start = narrow_starts(plan.schedule, plan.num_seqs);
+    const long long total = start[plan.num_seqs] * plan.kv_heads;
     const RequestFinder finder(plan, start);        // used by the producer
     const long long share = narrow_share(total, gridDim.x);
     const long long begin = share * blockIdx.x;
@@ -768,11 +771,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 {
     using C = WideCfg<D>;
     const FaPagedPlan& plan = p.plan;
+    // In this order: the narrow kernel relies on it.
+    grid_dependency_wait();
+    grid_dependents_launch();
     const long long* start = wide_starts(plan.schedule, plan.num_seqs);
     const long long total = start[plan.num_seqs] * plan.kv_heads;
     const long long share = wide_share(total, gridDim.x);
     const long long begin = share * blockIdx.x;
-    grid_dependents_launch();
     if (begin >= total) {
         if (threadIdx.x == 0) p.wide_merges[blockIdx.x] = Merge{};
         return;
@@ -1396,6 +1401,7 @@ paged_combine_narrow_kernel(const __grid_constant__ PagedParams p)
 {
     constexpr int kWarps = kCombineThreads / 32, kRowBlocks = 16 * MT / kWarps;
     const int block = static_cast<int>(blockIdx.x);
+    grid_dependents_launch();
     grid_dependency_wait();
     combine_narrow<D, MT>(p, block / kRowBlocks, block % kRowBlocks * kWarps + static_cast<int>(threadIdx.x) / 32);
 }
@@ -1596,24 +1602,6 @@ int cache_map(CUtensorMap* map, const void* ptr, const FaPagedPlan& plan, const 
     return fa_sm100_internal::encode_map(map, ptr, 4, dims, bytes, box);
 }
 
-// Launches a kernel; `early`: it may start before the one in front of it in the stream is done, and waits
-// for that one itself (grid_dependency_wait).
-template <typename... Args>
-int launch(void (*kernel)(Args...), int grid, int threads, int shared_bytes, bool early, cudaStream_t stream, const Args&... args)
-{
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(grid));
-    config.blockDim = dim3(static_cast<unsigned>(threads));
-    config.dynamicSmemBytes = static_cast<size_t>(shared_bytes);
-    config.stream = stream;
-    config.attrs = &attribute;
-    config.numAttrs = early ? 1 : 0;
-    return static_cast<int>(cudaLaunchKernelEx(&config, kernel, args...));
-}
-
 struct PagedMaps {
     CUtensorMap q;                          // wide
     CUtensorMap wide_k, wide_v;
@@ -1627,18 +1615,18 @@ int launch_attention(const PagedMaps& maps, const PagedParams& params, bool wide
 {
     int status = FA_STATUS_OK;
     if (wide) {
-        status = launch(paged_wide_kernel<D>, sms, kWideThreads, WideCfg<D>::kSmemBytes, false, stream, maps.q, maps.wide_k,
+        status = fa_sm100_internal::launch_early(paged_wide_kernel<D>, sms, kWideThreads, WideCfg<D>::kSmemBytes, stream, maps.q, maps.wide_k,
                         maps.wide_v, params);
         if (status == FA_STATUS_OK)
-            status = launch(paged_combine_wide_kernel<D>, sms * 2 * (D / kCombineColumns), kCombineThreads, 0, true, stream,
+            status = fa_sm100_internal::launch_early(paged_combine_wide_kernel<D>, sms * 2 * (D / kCombineColumns), kCombineThreads, 0, stream,
                             params);
     }
     if (!narrow || status != FA_STATUS_OK) return status;
     const int ctas = narrow_ctas(sms);
-    status = launch(paged_narrow_kernel<D, MT>, ctas, kNarrowThreads, NarrowCfg<D, MT>::kSmemBytes, wide, stream, maps.narrow_k,
+    status = fa_sm100_internal::launch_early(paged_narrow_kernel<D, MT>, ctas, kNarrowThreads, NarrowCfg<D, MT>::kSmemBytes, stream, maps.narrow_k,
                     maps.narrow_v, params);
     if (status != FA_STATUS_OK) return status;
-    return launch(paged_combine_narrow_kernel<D, MT>, ctas * (16 * MT / (kCombineThreads / 32)), kCombineThreads, 0, true, stream,
+    return fa_sm100_internal::launch_early(paged_combine_narrow_kernel<D, MT>, ctas * (16 * MT / (kCombineThreads / 32)), kCombineThreads, 0, stream,
                   params);
 }
 
@@ -1704,6 +1692,7 @@ int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cac
     params.v_row = strides[9];
     params.page_shift = __builtin_ctz(static_cast<unsigned>(plan->page_size));
     params.scale_log2 = fa_default_scale(plan->head_dim) * 1.4426950408889634f;
+    params.behind_wide = may_be_wide(*plan) ? 1 : 0;
     params.inject_stall = t_armed_stall ? 1 : 0;
     t_armed_stall = false;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

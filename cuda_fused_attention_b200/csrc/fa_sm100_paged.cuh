@@ -13,6 +13,8 @@
 
 #include <cstdint>
 
+#include <cuda_runtime.h>
+
 #include "fa_sm100_paged.h"
 
 namespace fa_sm100 {
@@ -102,6 +104,25 @@ int take_paged_attention_error(unsigned int* word);
 
 int validate_plan(const FaPagedPlan* plan);
 bool page_size_supported(int page_size);
+
+// Launches a kernel that may start before the one in front of it in the stream is done, once that one's CTAs
+// all run, so that its own start-up hides (attention of one request over 2048 keys, plan of 16 requests: 8.9 -> 8.4 us, 4.5 -> 4.2 us).
+// It calls grid_dependency_wait before it touches memory, and grid_dependents_launch for the kernel behind it.
+template <typename... Args>
+int launch_early(void (*kernel)(Args...), int grid, int threads, int shared_bytes, cudaStream_t stream, const Args&... args)
+{
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(grid));
+    config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.dynamicSmemBytes = static_cast<size_t>(shared_bytes);
+    config.stream = stream;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&config, kernel, args...));
+}
 
 // cudaError_t or FA_STATUS_*: the current device, its SM count, and that it is compute capability 10.x.
 int current_sm100(int* device, int* sm_count);

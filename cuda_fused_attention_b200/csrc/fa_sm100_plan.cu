@@ -9,6 +9,7 @@
 
 #include "fa_sm100_paged.h"
 #include "fa_sm100_paged.cuh"
+#include "fa_sm100_ptx.cuh"
 
 namespace fa_sm100 {
 
@@ -54,8 +55,10 @@ __device__ __forceinline__ long long warp_inclusive(long long v, int lane)
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
-plan_kernel(const PlanParams p)
+plan_kernel(const __grid_constant__ PlanParams p)
 {
+    grid_dependents_launch();
+    grid_dependency_wait();
     const FaPagedPlan& plan = p.plan;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const int ps = plan.page_size;
@@ -334,6 +337,8 @@ template <bool kAppend, bool kInterleaved>
 __global__ void __launch_bounds__(kRotaryThreads, 6)
 rotary_kernel(const __grid_constant__ RotaryParams p)
 {
+    grid_dependents_launch();
+    grid_dependency_wait();
     __shared__ __align__(16) float2 turn[kMaxTokensPerCta][64];
     __shared__ long long slots[kMaxTokensPerCta];
     const int group = 1 << p.group_shift;
@@ -413,6 +418,8 @@ template <bool kInterleaved>
 __global__ void __launch_bounds__(kRotaryThreads)
 rotary_long_kernel(const __grid_constant__ RotaryParams p)
 {
+    grid_dependents_launch();
+    grid_dependency_wait();
     const long long index = static_cast<long long>(blockIdx.x) * kRotaryThreads + threadIdx.x;
     const int unit = static_cast<int>(index) & ((1 << p.unit_shift) - 1);
     const long long all = static_cast<long long>(p.tokens) * p.batch, rest = index >> p.unit_shift;
@@ -496,9 +503,8 @@ int launch_rotary(RotaryParams& params, bool interleaved, cudaStream_t stream)
         params.head_split = static_cast<int>(split < rows ? split : rows);
         const long long blocks = ceil_div(units * params.head_split, kRotaryThreads);
         if (blocks > INT_MAX) return FA_STATUS_INVALID_ARGUMENT;
-        if (interleaved) rotary_long_kernel<true><<<static_cast<unsigned>(blocks), kRotaryThreads, 0, stream>>>(params);
-        else rotary_long_kernel<false><<<static_cast<unsigned>(blocks), kRotaryThreads, 0, stream>>>(params);
-        return static_cast<int>(cudaGetLastError());
+        return fa_sm100_internal::launch_early(interleaved ? rotary_long_kernel<true> : rotary_long_kernel<false>,
+                                               static_cast<int>(blocks), kRotaryThreads, 0, stream, params);
     }
     // Tokens share a CTA (and its set-up) once the CTAs would fill the GPU without it, four per SM.
     params.group_shift = 0;
@@ -506,9 +512,8 @@ int launch_rotary(RotaryParams& params, bool interleaved, cudaStream_t stream)
         ++params.group_shift;
     const long long blocks = ceil_div(params.tokens, 1LL << params.group_shift) * params.batch;
     if (blocks > INT_MAX) return FA_STATUS_INVALID_ARGUMENT;
-    if (interleaved) rotary_kernel<kAppend, true><<<static_cast<unsigned>(blocks), kRotaryThreads, 0, stream>>>(params);
-    else rotary_kernel<kAppend, false><<<static_cast<unsigned>(blocks), kRotaryThreads, 0, stream>>>(params);
-    return static_cast<int>(cudaGetLastError());
+    return fa_sm100_internal::launch_early(interleaved ? rotary_kernel<kAppend, true> : rotary_kernel<kAppend, false>,
+                                           static_cast<int>(blocks), kRotaryThreads, 0, stream, params);
 }
 
 }  // namespace
@@ -546,8 +551,8 @@ int fa_sm100_paged_plan(const FaPagedPlan* plan, const int* cached_lens, const i
     long long blocks = ceil_div(plan->total_tokens, kPlanTokensPerCta);
     if (blocks < 1) blocks = 1;
     if (blocks > sms) blocks = sms;
-    plan_kernel<<<static_cast<unsigned>(blocks), kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(params);
-    return static_cast<int>(cudaGetLastError());
+    return fa_sm100_internal::launch_early(plan_kernel, static_cast<int>(blocks), kPlanThreads, 0,
+                                           static_cast<cudaStream_t>(stream), params);
 }
 
 int fa_sm100_rotary(const void* x, const long long* x_strides, void* out, const long long* out_strides, int batch,

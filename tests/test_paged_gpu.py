@@ -679,3 +679,64 @@ def test_captured_steps(cuda_device):
     status_ok()
     for graph in graphs:
         graph.reset()
+
+
+@pytest.mark.parametrize("dim, new", [(64, [1, 1, 3, 1]), (128, [1, 40, 0, 300]), (64, [70, 129, 257, 64])])
+def test_launches_that_overlap(cuda_device, dim, new):
+    """Kernels that start before the one in front of them is done: chains in which each call needs the one before,
+    with copies between, on one stream and over a fork and a join, launched and captured; the inputs change
+    before every pass. Each pass equals calls with a synchronisation behind each."""
+    heads, kv_heads, page_size = 8, 2, 16
+    r = Requests([700, 0, 33, 64], new, page_size, cuda_device, seed=5)
+    shape = fa.PagedShape(heads, kv_heads, dim, page_size)
+    freq = _freq(dim // 2)
+    caches = [normal(s, r.num_pages, kv_heads, page_size, dim) for s in (1, 2)]
+    start = [c.clone() for c in caches]
+    sources = [normal(s, r.total, heads + 2 * kv_heads, dim) for s in (3, 4, 5)]
+    source, qkv = sources[0].clone(), torch.empty_like(sources[0])
+    table = r.block_table.clone()
+    side = torch.cuda.Stream()
+
+    def chain(wait):
+        r.block_table.copy_(table)
+        for c, s in zip(caches, start):
+            c.copy_(s)
+        qkv.copy_(source)
+        q, k, v = qkv.split([heads, kv_heads, kv_heads], dim=1)
+        wait()
+        plan = r.plan(shape)
+        wait()
+        outs = []
+        for _ in range(3):
+            out = _layer(None, plan, q, k, v, caches, freq)
+            wait()
+            main = torch.cuda.current_stream()
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                turned = fa.rotary_embed(out.transpose(0, 1)[None], plan.positions, freq)[0].transpose(0, 1)
+            wait()
+            q = fa.paged_attention(out, *caches, plan)
+            wait()
+            main.wait_stream(side)
+            q = fa.paged_attention(q + turned, *caches, plan)
+            wait()
+            outs += [out, turned, q]
+        return outs
+
+    want = []
+    for s in sources:
+        source.copy_(s)
+        want.append([o.clone() for o in chain(torch.cuda.synchronize)])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = chain(lambda: None)
+    for i in range(9):
+        source.copy_(sources[i % 3])
+        for o, w in zip(chain(lambda: None), want[i % 3]):
+            assert torch.equal(o, w)
+        graph.replay()
+        for o, w in zip(captured, want[i % 3]):
+            assert torch.equal(o, w)
+    graph.reset()
+    status_ok()
