@@ -611,7 +611,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 // 1320 TFLOP/s, with S and P in the same columns 405; a causal prompt of 8192 tokens 435 us (455); 16
 // requests of 16 new tokens (64 rows) behind up to 8192 71 us, 4.3 TB/s.
 constexpr int kWideThreads = 384;
-constexpr int kWideMinUnits = 4;        // units a CTA takes at least, more than a tile's (256 new tokens: 19.4 us; 8: 22.3)
+constexpr int kWideMinUnits = 4;        // units a CTA takes at least, more than a tile's (256 new tokens: 17.8 us; 2: 19.4, 8: 20.7)
 // 216 / 72 registers made the MMA issuer spill, and a load by it waits for its queued MMAs: 493 us against 462 (chunk
 // of 2048 tokens).
 constexpr uint32_t kWideRegsLaunch = 168, kWideRegsSoftmax = 200, kWideRegsOther = 104;

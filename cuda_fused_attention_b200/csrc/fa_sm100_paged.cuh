@@ -8,7 +8,7 @@
 // block has one Q tile). Each narrow item (one K/V head of a request) and each block is preceded by
 // kNarrowGap or kWideGap units without work, about what its set-up and epilogue cost. Without the
 // narrow gap 32 ragged requests of up to 4096 keys take 55.0 us instead of 52.4, with two 52.8;
-// without the wide one a causal prompt of 8192 tokens (16 heads) 340 us instead of 300.
+// without the wide one a causal prompt of 8192 tokens (32/8 heads) 484 us instead of 437, with two 453, with six 441.
 #pragma once
 
 #include <cstdint>
@@ -33,7 +33,7 @@ __host__ __device__ inline long long* wide_starts(long long* schedule, int num_s
 
 // Query rows per K/V head that any request of the plan can have, and the most that go to the narrow
 // kernel: 32 where no request has more (drafted tokens), else 16, which its faster variant holds. 16
-// requests of 5 to 8 new tokens, 20 to 32 rows, behind up to 8192: 63 us against 84 in the wide kernel.
+// requests of 5 to 8 new tokens, 20 to 32 rows, behind up to 8192: 62 us against 71 in the wide kernel, at D = 64 40 against 60.
 __host__ __device__ inline long long most_rows(const FaPagedPlan& plan)
 {
     return static_cast<long long>(plan.max_new < plan.total_tokens ? plan.max_new : plan.total_tokens) *
