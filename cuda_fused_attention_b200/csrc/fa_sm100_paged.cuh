@@ -122,7 +122,9 @@ int launch_early(void (*kernel)(Args...), int grid, int threads, int shared_byte
     config.stream = stream;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    return static_cast<int>(cudaLaunchKernelEx(&config, kernel, args...));
+    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, args...);
+    if (err != cudaSuccess) cudaGetLastError();     // returned here, not left for the caller's next call
+    return static_cast<int>(err);
 }
 
 // cudaError_t or FA_STATUS_*: the current device, its SM count, and that it is compute capability 10.x.

@@ -10,6 +10,8 @@
  * Plain C like fa_sm100.h: pointers, integers and one struct; a stream is a
  * cudaStream_t passed as void*. Every call is asynchronous on its stream, works on
  * the current device, allocates nothing and may be captured into a CUDA graph.
+ * Its kernels may take their places while the one in front of them in the stream still
+ * runs (programmatic dependent launch), but touch memory only when that one is done.
  *
  * Words used below. A step serves num_seqs requests. Request b has cached_lens[b]
  * tokens in the cache and brings new_lens[b] more (zero is allowed for both). The
