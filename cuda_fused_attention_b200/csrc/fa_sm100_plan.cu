@@ -198,14 +198,16 @@ plan_kernel(const __grid_constant__ PlanParams p)
             if (s_cached[r] < 0) continue;
             const int have = static_cast<int>((static_cast<long long>(s_cached[r]) + ps - 1) >> shift);
             const long long from = free_start + carry.pages + k;
+            // Where no page is to be had the entry says so: what it held before may be another request's page.
+            int page = -1;
             if (from < 0 || from >= p.num_free) {
                 record_plan_error(FA_ERROR_OUT_OF_PAGES);
-                continue;
-            }
-            const int page = p.free_pages[from];
-            if (page < 0 || page >= plan.num_pages) {
-                record_plan_error(FA_ERROR_BAD_PAGE);
-                continue;
+            } else {
+                page = p.free_pages[from];
+                if (page < 0 || page >= plan.num_pages) {
+                    record_plan_error(FA_ERROR_BAD_PAGE);
+                    page = -1;
+                }
             }
             plan.block_table[static_cast<long long>(base + r) * plan.table_stride + have + (k - s_page[r])] = page;
         }

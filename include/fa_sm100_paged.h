@@ -25,7 +25,9 @@
  * outside the cache, an empty free list) cannot be refused by the host: the kernels
  * check every index before they use it, skip what is out of range, and record it in
  * the device error word that fa_sm100_device_status reads (FA_STATUS_BAD_REQUEST,
- * FA_STATUS_OUT_OF_PAGES).
+ * FA_STATUS_OUT_OF_PAGES). A page that is not to be had is -1 in the block table, in
+ * this step and the steps behind it: its tokens have slot -1, nothing is written for
+ * them, and attention takes zeros in place of the page's K and V.
  */
 #ifndef FA_SM100_PAGED_H
 #define FA_SM100_PAGED_H
@@ -65,7 +67,7 @@ typedef struct FaPagedPlan {
     int* positions;             /* [total_tokens] position of each new token in its request; 0 for padding */
     int* slots;                 /* [total_tokens] its cache slot; -1 for padding and where no page was to be had */
     int* block_table;           /* [num_seqs][table_stride] */
-    int* free_cursor;           /* [1] free_start plus the pages that this step took */
+    int* free_cursor;           /* [1] free_start plus the pages that this step needed, had or not */
     long long* schedule;        /* fa_sm100_paged_schedule_bytes(num_seqs) bytes, for fa_sm100_paged_fwd */
 } FaPagedPlan;
 
@@ -73,7 +75,8 @@ FA_API size_t fa_sm100_paged_schedule_bytes(int num_seqs);
 
 /* Extends every request's table row by the pages its new tokens need and writes the
  * plan's arrays. New pages are free_pages[*free_start + k] (free_start may be NULL: 0),
- * handed out in request order; entries behind a request's last page stay as they were.
+ * handed out in request order; -1 is written where the list has ended or names a page outside the
+ * cache. Entries behind a request's last page stay as they were.
  * The inputs are not changed, so a call with the same inputs gives the same result; they must not
  * overlap the plan's arrays. */
 FA_API int fa_sm100_paged_plan(const FaPagedPlan* plan, const int* cached_lens, const int* new_lens,
