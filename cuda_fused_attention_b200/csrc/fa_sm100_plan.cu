@@ -69,7 +69,8 @@ plan_kernel(const __grid_constant__ PlanParams p)
 
     __shared__ PlanSums warp_sums[kPlanWarps];
     __shared__ int s_start[kPlanThreads + 1];       // packed row of each request of this round
-    __shared__ int s_page[kPlanThreads + 1];        // new pages before each request of this round
+    __shared__ int s_page[kPlanThreads];            // new pages before each request of this round
+    __shared__ unsigned long long s_unplaced;       // pages of this round's requests that have no rows
     __shared__ int s_cached[kPlanThreads];          // cached tokens, -1 for a request with invalid lengths
     long long* narrow = narrow_starts(plan.schedule, plan.num_seqs);
     long long* wide = wide_starts(plan.schedule, plan.num_seqs);
@@ -99,6 +100,7 @@ plan_kernel(const __grid_constant__ PlanParams p)
         sum.pages = warp_inclusive(need, lane);
         // The tokens of requests past total_tokens have no rows: such a request gets no work.
         if (lane == 31) warp_sums[warp] = {sum.tokens, sum.pages, 0, 0};
+        if (tid == 0) s_unplaced = 0;
         __syncthreads();
         long long tokens_before = carry.tokens + sum.tokens - n, pages_before = carry.pages + sum.pages - need;
         long long round_tokens = 0, round_pages = 0;
@@ -113,6 +115,8 @@ plan_kernel(const __grid_constant__ PlanParams p)
         const long long total = plan.total_tokens;
         const bool fits = tokens_before + n <= total;
         if (!fits && first_cta && b < plan.num_seqs) record_plan_error(FA_ERROR_BAD_LENGTH);
+        // Nor does it get pages. Requests behind it have no rows either, so the sums before those that fit stand.
+        if (!fits && need > 0) atomicAdd(&s_unplaced, static_cast<unsigned long long>(need));
         if (valid && fits && n > 0) {
             if (n * group <= narrow_rows(plan)) narrow_units = kNarrowGap + ceil_div(cached + n, kNarrowKeys);
             else
@@ -125,7 +129,6 @@ plan_kernel(const __grid_constant__ PlanParams p)
         if (tid == 0) {
             const long long end = carry.tokens + round_tokens;
             s_start[kPlanThreads] = static_cast<int>(end < total ? end : total);
-            s_page[kPlanThreads] = static_cast<int>(round_pages < INT_MAX ? round_pages : INT_MAX);
         }
         if (first_cta) {
             // Only one CTA writes the per-request arrays, so only it needs the units' sums.
@@ -188,8 +191,9 @@ plan_kernel(const __grid_constant__ PlanParams p)
             plan.slots[t] = slot;
         }
 
-        // This round's new pages.
-        const int pages = s_page[kPlanThreads];
+        // This round's new pages: at most one per 16 rows and one per request, so k stays far below 2^31.
+        round_pages -= static_cast<long long>(s_unplaced);
+        const int pages = static_cast<int>(round_pages);
         for (int k = blockIdx.x * kPlanThreads + tid; k < pages; k += gridDim.x * kPlanThreads) {
             int r = 0;
 #pragma unroll

@@ -76,7 +76,8 @@ FA_API size_t fa_sm100_paged_schedule_bytes(int num_seqs);
 /* Extends every request's table row by the pages its new tokens need and writes the
  * plan's arrays. New pages are free_pages[*free_start + k] (free_start may be NULL: 0),
  * handed out in request order; -1 is written where the list has ended or names a page outside the
- * cache. Entries behind a request's last page stay as they were.
+ * cache. Entries behind a request's last page stay as they were. A request with invalid lengths, or whose
+ * new tokens and those before it are more than total_tokens, takes no pages.
  * The inputs are not changed, so a call with the same inputs gives the same result; they must not
  * overlap the plan's arrays. */
 FA_API int fa_sm100_paged_plan(const FaPagedPlan* plan, const int* cached_lens, const int* new_lens,

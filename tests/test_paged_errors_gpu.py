@@ -74,3 +74,24 @@ def test_a_request_without_pages_leaves_others_alone(cuda_device, new, free):
     for a, b in zip(outs, other):
         assert torch.equal(a[1:], b[1:]) and not torch.equal(a[:1], b[:1])
     fa.device_status()
+
+
+@pytest.mark.parametrize("seqs,placed", [(3, 1), (3, 2), (512, 511), (600, 100), (600, 512), (1300, 1024), (1300, 1299)])
+def test_requests_without_rows_take_no_pages(cuda_device, seqs, placed):
+    """total_tokens ends inside request `placed`: only the requests before it get pages, and the next step begins in the
+    free list where theirs end."""
+    width = 3
+    cached, new = [(7 * b) % 20 for b in range(seqs)], [1 + (5 * b) % 23 for b in range(seqs)]
+    table = torch.full((seqs, width), -5, dtype=torch.int32, device=cuda_device)
+    free = torch.arange(seqs * width, dtype=torch.int32, device=cuda_device)
+    total = sum(new[:placed]) + new[placed] - 1
+    plan = fa.paged_plan(i32(*cached), i32(*new), table, free, total, fa.PagedShape(HEADS, KV_HEADS, DIM, PAGE), seqs * width)
+    assert fa.device_status()[0] == fa.STATUS_BAD_REQUEST
+    want, taken = [[-5] * width for _ in range(seqs)], 0
+    for b in range(placed):
+        for i in range(-(-cached[b] // PAGE), -(-(cached[b] + new[b]) // PAGE)):
+            want[b][i] = taken
+            taken += 1
+    assert table.tolist() == want
+    assert plan.free_cursor.tolist() == [taken]
+    assert plan.kv_lens.tolist() == [c + n if b < placed else 0 for b, (c, n) in enumerate(zip(cached, new))]
