@@ -29,6 +29,7 @@ struct PagedParams {
     int page_shift;
     float scale_log2;
     int behind_wide;            // narrow kernel: the wide one of the same call was launched before it
+    int narrow_follows;         // wide kernel: the narrow one of the same call is launched behind it
     int inject_stall;           // test only: the warps that hand out work wait on a barrier nothing arrives on
     // Parts of items that cross a border between CTAs' ranges, two places per CTA, and per CTA what is to be
     // merged from the second place on; for the narrow and for the wide kernel.
@@ -200,6 +201,17 @@ private:
     int my_token0_ = 0, my_tokens_ = 0, my_kv_ = 0;
 };
 
+// The plan's arrays may have been written again for other arguments (mask, max_new, table) than a captured call was
+// made with. Its line of units is then another one, and to walk it might never end or leave the tensors: what a
+// kernel finds on the line is compared with its own arguments, and a difference ends the walk.
+__device__ __forceinline__ void record_other_plan() { atomicOr(&g_paged_error_word, FA_ERROR_OTHER_PLAN); }
+
+__device__ __forceinline__ bool request_in_range(const FaPagedPlan& plan, const Request& r)
+{
+    return r.token0 >= 0 && r.tokens > 0 && r.tokens <= plan.total_tokens - r.token0 && r.kv > 0 &&
+           r.kv <= plan.table_width * plan.page_size;
+}
+
 // Units per CTA when `total` are shared out over `ctas`.
 __device__ __forceinline__ long long narrow_share(long long total, int ctas)
 {
@@ -244,7 +256,13 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const RequestFinder finder(plan, start);        // used by the producer
     const long long share = narrow_share(total, gridDim.x);
     const long long begin = share * blockIdx.x;
+    // By one thread that has time: work for a wide kernel that this call has none of.
+    auto check_wide = [&]() {
+        if (blockIdx.x == 0 && threadIdx.x == 0 && !p.behind_wide && wide_starts(plan.schedule, plan.num_seqs)[plan.num_seqs] != 0)
+            record_other_plan();
+    };
     if (begin >= total) {
+        check_wide();
         if (threadIdx.x == 0) p.merges[blockIdx.x] = Merge{};
         grid_dependency_wait();
         return;
@@ -271,6 +289,12 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             int b = 0, h = 0;
             if (x < end) {
                 const Request r = finder.find(quotient(x, plan.kv_heads));
+                if (!request_in_range(plan, r) || r.tokens * static_cast<long long>(group) > 16 * MT ||
+                    r.units != kNarrowGap + (r.kv + kNarrowKeys - 1) / kNarrowKeys) {
+                    if (lane == 0) record_other_plan();
+                    x = end;
+                    continue;
+                }
                 b = r.b;
                 h = static_cast<int>(quotient(x - r.start * plan.kv_heads, r.units));
                 // The item's tiles lie at [first, last) of the line, behind its gap.
@@ -370,6 +394,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     auto swizzled = [](int row, int chunk) -> uint32_t {
         return static_cast<uint32_t>((chunk >> 3) * kNarrowKeys * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
     };
+    check_wide();
     int it = 0;
     bool ok = true;
     for (int sg = 0;; ++sg) {
@@ -707,6 +732,12 @@ __device__ inline WideSegment wide_segment(const FaPagedPlan& plan, const Reques
     const int weight = wide_weight(lo, span, n);
     const int tiles = static_cast<int>(wide_tiles_of(lo, span, cached, n, causal));
     s.last = first + static_cast<long long>(weight) * tiles;
+    if (s.last <= x || s.last > head_first + r.units || !request_in_range(plan, r)) {
+        if (lane == 0) record_other_plan();
+        s.count = 0;
+        s.last = end;
+        return s;
+    }
     s.token0 = r.token0 + lo * span;
     s.tokens = min(span, n - lo * span);
     s.pos0 = cached + lo * span;
@@ -778,7 +809,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const long long total = start[plan.num_seqs] * plan.kv_heads;
     const long long share = wide_share(total, gridDim.x);
     const long long begin = share * blockIdx.x;
+    // By one thread that has time: work for a narrow kernel that this call has none of.
+    auto check_narrow = [&]() {
+        if (blockIdx.x == 0 && threadIdx.x == 0 && !p.narrow_follows && narrow_starts(plan.schedule, plan.num_seqs)[plan.num_seqs] != 0)
+            record_other_plan();
+    };
     if (begin >= total) {
+        check_narrow();
         if (threadIdx.x == 0) p.wide_merges[blockIdx.x] = Merge{};
         return;
     }
@@ -1149,6 +1186,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             half_max = fmaxf(ma, mb_);
         };
 
+        check_narrow();
         bool ok = true;
         for (int sg = 0; ok; ++sg) {
             // The slot stays this segment's until the epilogue has read it.
@@ -1693,6 +1731,7 @@ int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cac
     params.page_shift = __builtin_ctz(static_cast<unsigned>(plan->page_size));
     params.scale_log2 = fa_default_scale(plan->head_dim) * 1.4426950408889634f;
     params.behind_wide = may_be_wide(*plan) ? 1 : 0;
+    params.narrow_follows = may_be_narrow(*plan) ? 1 : 0;
     params.inject_stall = t_armed_stall ? 1 : 0;
     t_armed_stall = false;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

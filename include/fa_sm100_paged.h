@@ -46,6 +46,7 @@ extern "C" {
 #define FA_ERROR_BAD_LENGTH   0x10000u    /* plan: a length is negative or exceeds the table or total_tokens */
 #define FA_ERROR_OUT_OF_PAGES 0x20000u    /* plan: free list exhausted */
 #define FA_ERROR_BAD_PAGE     0x40000u    /* a page id or slot is outside the cache */
+#define FA_ERROR_OTHER_PLAN   0x80000u    /* attention: the plan's arrays were written for another plan than the call's */
 
 /* One step's requests: sizes set by the caller, arrays filled by fa_sm100_paged_plan
  * (block_table is read and extended). All device pointers. */
@@ -119,7 +120,9 @@ FA_API int fa_sm100_rotary_append(const void* q, const void* k, const void* v, v
  * be in the cache. What a cache holds behind a request's last token is never used, whatever it
  * is (NaN included); V of a later token of the same request takes part with weight zero, so it
  * has to be finite. workspace: fa_sm100_paged_workspace_bytes(plan) bytes, 16-byte aligned, not
- * shared with a call that may run at the same time; its contents need no preparation. */
+ * shared with a call that may run at the same time; its contents need no preparation. The plan is the one
+ * that fa_sm100_paged_plan had, unchanged. Where its arrays no longer fit it (a captured call, after they were written
+ * again for another mask, max_new or table), the call records FA_ERROR_OTHER_PLAN and leaves work out. */
 FA_API int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cache, const void* v_cache,
                               void* o, const long long* strides, void* workspace, size_t workspace_bytes,
                               void* stream);

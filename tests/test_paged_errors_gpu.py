@@ -95,3 +95,112 @@ def test_requests_without_rows_take_no_pages(cuda_device, seqs, placed):
     assert table.tolist() == want
     assert plan.free_cursor.tolist() == [taken]
     assert plan.kv_lens.tolist() == [c + n if b < placed else 0 for b, (c, n) in enumerate(zip(cached, new))]
+
+
+def _captured(q, caches, plan, out):
+    """A graph of one attention call with the plan as it is now."""
+    fa.paged_attention(q, *caches, plan, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fa.paged_attention(q, *caches, plan, out=out)
+    return graph
+
+
+OTHER_PLAN = 0x80000
+
+# Heads, K/V heads, rows of the token axis, then (new lengths, causal, max_new) at capture and at replay.
+OTHERS = [
+    (8, 2, 340, ((300, 40), True, None), ((300, 40), False, None)),
+    (8, 2, 340, ((300, 40), False, None), ((300, 40), True, None)),
+    (8, 2, 16, ((1, 1), True, 1), ((8, 8), True, 8)),          # 4, then 32 rows to the narrow kernel
+    (8, 2, 16, ((1, 1), True, 1), ((12, 1), True, 12)),        # no wide kernel, then work for one
+    (8, 2, 16, ((4, 12), True, 16), ((8, 8), True, 8)),        # 16 narrow rows, then 32
+    (8, 2, 40, ((8, 8), True, 8), ((33, 7), True, 33)),        # 32 narrow rows, no wide kernel; then 28 for one
+    (24, 1, 2, ((1, 1), True, 2), ((1, 1), True, 1)),          # no narrow kernel, then work for one
+]
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,total,then,now", OTHERS)
+def test_a_captured_call_meets_another_plan(cuda_device, dim, heads, kv_heads, total, then, now):
+    """The arrays are written again for another mask or max_new while a graph holds a call made for the first: the
+    replay reports it, ends, and is right again once the plan is."""
+    shape = fa.PagedShape(heads, kv_heads, dim, PAGE)
+    table = torch.arange(128, dtype=torch.int32, device=cuda_device).view(2, 64).contiguous()
+    free = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    cached = i32(0, 500)
+    # Every page is in the table, so plans hand out none: all of a request's tokens count as cached but the last new ones.
+    kv = i32(900, 1000)
+
+    def plan_of(which, plan=None):
+        new, causal, max_new = which
+        cached.copy_(kv - i32(*new))
+        return fa.paged_plan(cached, i32(*new), table, free, total, shape, 128, causal=causal, max_new=max_new, plan=plan)
+
+    caches = [normal(s, 128, kv_heads, PAGE, dim) for s in (1, 2)]
+    q = normal(3, total, heads, dim)
+    # Pages of the new tokens come from the free list; give the list what the table holds.
+    entries = table.clone()
+    plan = plan_of(then)
+    table.copy_(entries)
+    fa.device_status()
+    out = torch.zeros_like(q)
+    graph = _captured(q, caches, plan, out)
+    want = out.clone()
+    assert fa.device_status() == (fa.STATUS_OK, 0)
+    plan_of(now, plan)
+    table.copy_(entries)
+    fa.device_status()
+    graph.replay()
+    status, word = fa.device_status()
+    assert status == fa.STATUS_BAD_REQUEST and word == OTHER_PLAN
+    plan_of(then, plan)
+    table.copy_(entries)
+    fa.device_status()
+    out.zero_()
+    graph.replay()
+    assert torch.equal(out, want)
+    assert fa.device_status() == (fa.STATUS_OK, 0)
+    graph.reset()
+
+
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("change", ["table", "kv_lens", "query_start"])
+def test_a_call_whose_arrays_do_not_fit(cuda_device, new, change):
+    """A table of a captured call that is shorter than what the plan was written for again, and arrays of a plan that
+    somebody else wrote to."""
+    shape = fa.PagedShape(HEADS, KV_HEADS, DIM, PAGE)
+    pages, total = 256, 2 * new
+    long_table = torch.arange(pages, dtype=torch.int32, device=cuda_device).view(2, 128).contiguous()
+    table = long_table[:, :8].contiguous()
+    free = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    caches = [normal(s, pages, KV_HEADS, PAGE, DIM) for s in (1, 2)]
+    q = normal(3, total, HEADS, DIM)
+
+    def plan_of(kv, block_table, plan=None):
+        entries = block_table.clone()
+        plan = fa.paged_plan(i32(kv - new, kv - new), i32(new, new), block_table, free, total, shape, pages, plan=plan)
+        block_table.copy_(entries)
+        fa.device_status()
+        return plan
+
+    plan = plan_of(128, table)
+    out = torch.zeros_like(q)
+    graph = _captured(q, caches, plan, out)
+    want = out.clone()
+    if change == "table":
+        plan_of(1500, long_table, plan)
+    elif change == "kv_lens":
+        plan.kv_lens.add_(1000)
+    else:
+        plan.query_start[1:].add_(10 ** 6)
+    graph.replay()
+    status, word = fa.device_status()
+    assert status == fa.STATUS_BAD_REQUEST and word == OTHER_PLAN
+    plan_of(128, table, plan)
+    out.zero_()
+    graph.replay()
+    assert torch.equal(out, want)
+    assert fa.device_status() == (fa.STATUS_OK, 0)
+    graph.reset()
