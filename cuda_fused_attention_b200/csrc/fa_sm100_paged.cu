@@ -347,7 +347,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 // num_pages is out of the map's range: such a box reads as zeros.
                 const int i = ((tile * kNarrowKeys) >> p.page_shift) + page_of_tile;
                 if (!active || i >= held) return plan.num_pages;
-                const int page = __ldg(table + i);
+                const int page = table[i];     // an ordinary load: the plan may have been written while this CTA was here
                 if (page >= 0 && page < plan.num_pages) return page;
                 atomicOr(&g_paged_error_word, FA_ERROR_BAD_PAGE);
                 return plan.num_pages;
@@ -911,7 +911,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                     // num_pages is out of the map's range: such a box reads as zeros.
                     const int i = ((tile * kWideKeys) >> p.page_shift) + page_of_tile;
                     if (!active || i >= held) return plan.num_pages;
-                    const int page = __ldg(table + i);
+                    const int page = table[i];     // an ordinary load, as in the narrow kernel
                     if (page >= 0 && page < plan.num_pages) return page;
                     atomicOr(&g_paged_error_word, FA_ERROR_BAD_PAGE);
                     return plan.num_pages;
