@@ -256,14 +256,15 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const RequestFinder finder(plan, start);        // used by the producer
     const long long share = narrow_share(total, gridDim.x);
     const long long begin = share * blockIdx.x;
-    // By one thread that has time: work for a wide kernel that this call has none of.
+    // By one thread: work for a wide kernel that this call has none of.
     auto check_wide = [&]() {
-        if (blockIdx.x == 0 && threadIdx.x == 0 && !p.behind_wide && wide_starts(plan.schedule, plan.num_seqs)[plan.num_seqs] != 0)
-            record_other_plan();
+        if (blockIdx.x == 0 && !p.behind_wide && wide_starts(plan.schedule, plan.num_seqs)[plan.num_seqs] != 0) record_other_plan();
     };
     if (begin >= total) {
-        check_wide();
-        if (threadIdx.x == 0) p.merges[blockIdx.x] = Merge{};
+        if (threadIdx.x == 0) {
+            check_wide();
+            p.merges[blockIdx.x] = Merge{};
+        }
         grid_dependency_wait();
         return;
     }
@@ -372,7 +373,10 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             for (int i = sg > C::kQSlots ? sg - C::kQSlots : 0; i < sg; ++i)
                 drain_paged(item_full(i % C::kQSlots), (i / C::kQSlots) & 1);
         }
-        if (lane == 0) p.merges[blockIdx.x] = merge;
+        if (lane == 0) {
+            p.merges[blockIdx.x] = merge;
+            check_wide();
+        }
         grid_dependency_wait();     // what was launched before this kernel is done when this one is
         return;
     }
@@ -394,7 +398,6 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     auto swizzled = [](int row, int chunk) -> uint32_t {
         return static_cast<uint32_t>((chunk >> 3) * kNarrowKeys * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
     };
-    check_wide();
     int it = 0;
     bool ok = true;
     for (int sg = 0;; ++sg) {
@@ -809,14 +812,15 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const long long total = start[plan.num_seqs] * plan.kv_heads;
     const long long share = wide_share(total, gridDim.x);
     const long long begin = share * blockIdx.x;
-    // By one thread that has time: work for a narrow kernel that this call has none of.
+    // By one thread: work for a narrow kernel that this call has none of.
     auto check_narrow = [&]() {
-        if (blockIdx.x == 0 && threadIdx.x == 0 && !p.narrow_follows && narrow_starts(plan.schedule, plan.num_seqs)[plan.num_seqs] != 0)
-            record_other_plan();
+        if (blockIdx.x == 0 && !p.narrow_follows && narrow_starts(plan.schedule, plan.num_seqs)[plan.num_seqs] != 0) record_other_plan();
     };
     if (begin >= total) {
-        check_narrow();
-        if (threadIdx.x == 0) p.wide_merges[blockIdx.x] = Merge{};
+        if (threadIdx.x == 0) {
+            check_narrow();
+            p.wide_merges[blockIdx.x] = Merge{};
+        }
         return;
     }
     const long long end = begin + share < total ? begin + share : total;
@@ -1118,7 +1122,10 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 zero_to = s.zero_to;
                 zero_slot = (ri - 1) % C::kStages;
             }
-            if (lane == 0) p.wide_merges[blockIdx.x] = merge;
+            if (lane == 0) {
+                p.wide_merges[blockIdx.x] = merge;
+                check_narrow();
+            }
         }
         __syncwarp();
     } else {
@@ -1186,7 +1193,6 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             half_max = fmaxf(ma, mb_);
         };
 
-        check_narrow();
         bool ok = true;
         for (int sg = 0; ok; ++sg) {
             // The slot stays this segment's until the epilogue has read it.
