@@ -21,11 +21,8 @@ __device__ unsigned int g_paged_error_word;
 struct PagedParams {
     FaPagedPlan plan;
     const __nv_bfloat16* q;
-    const __nv_bfloat16* k;
-    const __nv_bfloat16* v;
     __nv_bfloat16* o;
-    long long q_token, q_head, o_token, o_head;
-    long long k_page, k_head, k_row, v_page, v_head, v_row;
+    long long q_token, q_head, o_token, o_head;     // K and V are read through tensor maps
     int page_shift;
     float scale_log2;
     int behind_wide;            // narrow kernel: the wide one of the same call was launched before it
@@ -251,7 +248,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     // Behind the wide kernel of the same call, which has waited, there is nothing to wait for before the end.
     if (!p.behind_wide) grid_dependency_wait();
     grid_dependents_launch();
-    const long long* start = narrow_starts(plan.schedule, plan.num_seqs);
+    const long long* start = narrow_starts(plan.schedule);
     const long long total = start[plan.num_seqs] * plan.kv_heads;
     const RequestFinder finder(plan, start);        // used by the producer
     const long long share = narrow_share(total, gridDim.x);
@@ -814,7 +811,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const long long begin = share * blockIdx.x;
     // By one thread: work for a narrow kernel that this call has none of.
     auto check_narrow = [&]() {
-        if (blockIdx.x == 0 && !p.narrow_follows && narrow_starts(plan.schedule, plan.num_seqs)[plan.num_seqs] != 0) record_other_plan();
+        if (blockIdx.x == 0 && !p.narrow_follows && narrow_starts(plan.schedule)[plan.num_seqs] != 0) record_other_plan();
     };
     if (begin >= total) {
         if (threadIdx.x == 0) {
@@ -1721,19 +1718,11 @@ int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cac
     PagedParams params{};
     params.plan = *plan;
     params.q = static_cast<const __nv_bfloat16*>(q);
-    params.k = static_cast<const __nv_bfloat16*>(k_cache);
-    params.v = static_cast<const __nv_bfloat16*>(v_cache);
     params.o = static_cast<__nv_bfloat16*>(o);
     params.q_token = strides[0];
     params.q_head = strides[1];
     params.o_token = strides[2];
     params.o_head = strides[3];
-    params.k_page = strides[4];
-    params.k_head = strides[5];
-    params.k_row = strides[6];
-    params.v_page = strides[7];
-    params.v_head = strides[8];
-    params.v_row = strides[9];
     params.page_shift = __builtin_ctz(static_cast<unsigned>(plan->page_size));
     params.scale_log2 = fa_default_scale(plan->head_dim) * 1.4426950408889634f;
     params.behind_wide = may_be_wide(*plan) ? 1 : 0;

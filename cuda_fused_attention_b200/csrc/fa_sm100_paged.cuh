@@ -28,7 +28,7 @@ static_assert(kWideKeys == 128, "floor_sum_128 counts key tiles");
 
 // plan->schedule: narrow_start[num_seqs + 1], then wide_start[num_seqs + 1]: prefix sums of the
 // requests' units for one K/V head.
-__host__ __device__ inline long long* narrow_starts(long long* schedule, int) { return schedule; }
+__host__ __device__ inline long long* narrow_starts(long long* schedule) { return schedule; }
 __host__ __device__ inline long long* wide_starts(long long* schedule, int num_seqs) { return schedule + num_seqs + 1; }
 
 // Query rows per K/V head that any request of the plan can have, and the most that go to the narrow
@@ -108,7 +108,9 @@ bool page_size_supported(int page_size);
 // Launches a kernel that may start before the one in front of it in the stream is done, once that one's CTAs
 // all run, so that its own start-up hides (attention of one request over 2048 keys 8.9 -> 8.4 us, plan of 16
 // requests 4.5 -> 4.2 us). It calls grid_dependency_wait before it touches memory, and
-// grid_dependents_launch for the kernel behind it.
+// grid_dependents_launch for the kernel behind it. One does not wait at its start: the narrow attention kernel behind
+// the wide one. That one waited before it let any other start, and what the merging kernel between them
+// reads and writes is not the narrow kernel's; it waits at its end, so that the call is done when it is.
 template <typename... Args>
 int launch_early(void (*kernel)(Args...), int grid, int threads, int shared_bytes, cudaStream_t stream, const Args&... args)
 {

@@ -72,7 +72,7 @@ plan_kernel(const __grid_constant__ PlanParams p)
     __shared__ int s_page[kPlanThreads];            // new pages before each request of this round
     __shared__ unsigned long long s_unplaced;       // pages of this round's requests that have no rows
     __shared__ int s_cached[kPlanThreads];          // cached tokens, -1 for a request with invalid lengths
-    long long* narrow = narrow_starts(plan.schedule, plan.num_seqs);
+    long long* narrow = narrow_starts(plan.schedule);
     long long* wide = wide_starts(plan.schedule, plan.num_seqs);
 
     const long long free_start = p.free_start ? *p.free_start : 0;
