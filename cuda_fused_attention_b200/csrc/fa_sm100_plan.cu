@@ -624,6 +624,7 @@ int fa_sm100_rotary_append(const void* q, const void* k, const void* v, void* q_
         misaligned(v_cache))
         return FA_STATUS_MISALIGNED;
     if ((status = check_strides(strides, 14)) != FA_STATUS_OK) return status;
+    if (k_cache == v_cache) return FA_STATUS_INVALID_ARGUMENT;
     params.src[0] = static_cast<const __nv_bfloat16*>(q);
     params.src[1] = static_cast<const __nv_bfloat16*>(k);
     params.src[2] = static_cast<const __nv_bfloat16*>(v);

@@ -17,8 +17,11 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <optional>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "fa_sm100_paged.h"
 
@@ -122,6 +125,35 @@ void need_distinct(const at::Tensor& t, const char* name)
         if (stride < reach) bad_value(std::string(name) + " has elements that share memory (strides " + shown(t.strides()) + ")");
         reach = stride * (size - 1) + reach;
     }
+}
+
+// Whether two tensors of one shape and strides, each without shared elements, have an element in common: whether
+// `apart`, the distance of their first elements, is a sum of differences of indexes times strides. Taken from
+// the widest stride down, only the two multiples around what is left can be part of one.
+bool meet(const std::vector<std::pair<int64_t, int64_t>>& widest_first, size_t at, int64_t apart)
+{
+    if (at == widest_first.size()) return apart == 0;
+    const auto [stride, size] = widest_first[at];
+    const int64_t low = apart >= 0 ? apart / stride : -((-apart + stride - 1) / stride);
+    for (int64_t index : {low, low + 1})
+        if (index > -size && index < size && meet(widest_first, at + 1, apart - index * stride)) return true;
+    return false;
+}
+
+// Two caches that are written in one call.
+void need_apart(const at::Tensor& a, const at::Tensor& b, const char* names)
+{
+    if (a.numel() == 0 || a.strides() != b.strides()) return;
+    const auto *pa = static_cast<const char*>(a.const_data_ptr()), *pb = static_cast<const char*>(b.const_data_ptr());
+    const int64_t distance = (pb - pa) / static_cast<int64_t>(a.element_size());
+    int64_t reach = 0;
+    for (int64_t i = 0; i < a.dim(); ++i) reach += (a.size(i) - 1) * a.stride(i);
+    if (distance > reach || distance < -reach) return;
+    std::vector<std::pair<int64_t, int64_t>> spans;
+    for (int64_t i = 0; i < a.dim(); ++i)
+        if (a.size(i) > 1) spans.emplace_back(a.stride(i), a.size(i));
+    std::sort(spans.rbegin(), spans.rend());
+    if (meet(spans, 0, distance)) bad_value(std::string(names) + " must not share memory");
 }
 
 // All tensors on one CUDA device; its index.
@@ -418,6 +450,7 @@ PyObject* append(PyObject* const* args, Py_ssize_t count)
     need_rows(v_cache, "v_cache", cache, s + 11);
     need_distinct(k_cache, "k_cache");
     need_distinct(v_cache, "v_cache");
+    need_apart(k_cache, v_cache, "k_cache and v_cache");
     int sections[kMaxAxes], axes;
     const int rotary_dim = need_frequencies(inv_freq, dim, args[8], sections, axes);
     const int64_t dims = positions.dim();

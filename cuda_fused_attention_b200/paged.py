@@ -152,7 +152,8 @@ def rotary_append(q, k, v, k_cache, v_cache, positions, slots, inv_freq, section
     may be passed as they are. q is rotated into out (returned; may be q itself), k into k_cache and v
     copied into v_cache at slots[token]; caches are [num_pages, kv_heads, page_size, D] in any stride
     order with contiguous rows. positions: int32 [tokens] or [axes, tokens]. A token with a negative
-    slot (padding) is skipped, its row of out included. Slots must be distinct. inv_freq, sections,
+    slot (padding) is skipped, its row of out included. Slots must be distinct, and the caches must not
+    share memory. inv_freq, sections,
     interleaved: as in rotary_embed.
     """
     out = (_ops or _load()).append(q, k, v, k_cache, v_cache, positions, slots, inv_freq, sections, interleaved, out,

@@ -103,7 +103,8 @@ FA_API int fa_sm100_rotary(const void* x, const long long* x_strides, void* out,
  * rotated into k_cache and v copied into v_cache at slots[token]. strides: 14 element strides,
  * multiples of 8: q (token, head), q_out (token, head), k (token, head), v (token, head),
  * k_cache (page, head, row), v_cache (page, head, row). q_out may be q. A token whose slot is
- * negative is skipped: its q_out row is not written either. Slots must be distinct. positions:
+ * negative is skipped: its q_out row is not written either. Slots must be distinct, and the two caches
+ * must not share memory (nor may what is written share memory with another input). positions:
  * int32 [axes][tokens] with element stride position_stride between axes. */
 FA_API int fa_sm100_rotary_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache,
                                   void* v_cache, const long long* strides, int tokens, int heads, int kv_heads,

@@ -173,3 +173,30 @@ def test_python_refusals():
 def test_status_strings(lib):
     for code in (fa.STATUS_BAD_REQUEST, fa.STATUS_OUT_OF_PAGES, fa.STATUS_WORKSPACE):
         assert b"unknown" not in lib.fa_sm100_status_string(code)
+
+
+def test_append_refuses_caches_that_share_memory(lib):
+    """K and V would be written over each other."""
+    q, k = _bf16(5, 4, 64), _bf16(5, 2, 64)
+    rest = dict(positions=_i32(5), slots=_i32(5), inv_freq=torch.ones(32))
+
+    def refusal(k_cache, v_cache):
+        with pytest.raises((ValueError, TypeError)) as caught:
+            fa.rotary_append(q, k, k, k_cache, v_cache, **rest)
+        return str(caught.value)
+
+    pages = _bf16(6, 2, 16, 64)
+    rows = _bf16(6, 16, 2, 64).transpose(1, 2)
+    halves, both = _bf16(6, 2, 2, 16, 64), _bf16(6, 16, 2, 2, 64).permute(0, 2, 3, 1, 4)
+    wide = _bf16(6, 2, 16, 128)
+    for a, b in [(pages, pages), (rows, rows), (pages[:4], pages[2:]), (pages[1:], pages[:-1]), (halves[:, 0], halves[:, 0]),
+                 (both[:, 1], both[:, 1]), (halves[1:, 0], halves[:-1, 0]), (wide[..., :64], wide[..., 32:96])]:
+        assert "must not share memory" in refusal(a, b) and "must not share memory" in refusal(b, a)
+    for a, b in [(pages, pages.clone()), (pages[:3], pages[3:]), (halves[:, 0], halves[:, 1]), (halves[:, 1], halves[:, 0]),
+                 (both[:, 0], both[:, 1]), (wide[..., :64], wide[..., 64:]), (pages[:1], pages[1:2])]:
+        assert "must be a CUDA tensor" in refusal(a, b) and "must be a CUDA tensor" in refusal(b, a)
+
+    sections = (ctypes.c_int * 1)(32)
+    strides = (ctypes.c_longlong * 14)(*[64] * 14)
+    assert lib.fa_sm100_rotary_append(0x1000, 0x2000, 0x2000, 0x1000, 0x3000, 0x3000, strides, 2, 4, 2, 64, 16, 8, 0x1000, 2,
+                                      0x1000, 0x1000, 64, sections, 1, 0, None) == 1001
