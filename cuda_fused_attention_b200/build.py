@@ -15,8 +15,10 @@ whose kernel also dumps its intermediate tiles for layout checks
 
 lib/_paged.so is the CPython binding of the paged-cache operators for torch tensors
 (csrc/paged_binding.cpp). It is the one part that is compiled against torch's headers
-and needs torch at run time; the two libraries above do not.
+and needs torch at run time; the two libraries above do not, and without torch they
+alone are built.
 """
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -58,8 +60,12 @@ def binding_command(output=BINDING_PATH):
             "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-ldl", "-o", output]
 
 
+def have_torch():
+    return importlib.util.find_spec("torch") is not None
+
+
 def needs_build():
-    outputs = (LIB_PATH, DEBUG_LIB_PATH, BINDING_PATH)
+    outputs = (LIB_PATH, DEBUG_LIB_PATH, *((BINDING_PATH,) if have_torch() else ()))
     if not all(os.path.exists(path) for path in outputs):
         return True
     lib_time = min(os.path.getmtime(path) for path in outputs)
@@ -75,7 +81,11 @@ def build(force=False, verbose=True, ptxas_verbose=False):
     os.makedirs(LIB_DIR, exist_ok=True)
     extra = ["-Xptxas", "-v"] if ptxas_verbose else []
     cmds = [compile_command(extra=extra),
-            compile_command(output=DEBUG_LIB_PATH, extra=["-DFA_SM100_DEBUG_DUMP"]), binding_command()]
+            compile_command(output=DEBUG_LIB_PATH, extra=["-DFA_SM100_DEBUG_DUMP"])]
+    if have_torch():
+        cmds.append(binding_command())
+    elif verbose:
+        print("torch is not installed: the binding of the paged-cache operators is not built", flush=True)
     procs = []
     for cmd in cmds:
         if verbose:

@@ -1,0 +1,56 @@
+"""What the build recipe compiles, without running a compiler on the kernels."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+from cuda_fused_attention_b200 import build as recipe
+
+
+class Recorded:
+    """In place of subprocess.Popen: a compiler that succeeds and writes nothing."""
+    commands = []
+
+    def __init__(self, command, **_):
+        Recorded.commands.append(command)
+        self.returncode = 0
+
+    def communicate(self):
+        return "", ""
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    Recorded.commands = []
+    monkeypatch.setattr(subprocess, "Popen", Recorded)
+    return Recorded
+
+
+def _outputs(recorded):
+    return [os.path.basename(command[command.index("-o") + 1]) for command in recorded.commands]
+
+
+def test_libraries_are_built_without_torch(recorded, monkeypatch, capsys):
+    monkeypatch.setitem(sys.modules, "torch", None)         # as if it were not installed
+    assert recipe.build(force=True) == recipe.LIB_PATH
+    assert _outputs(recorded) == ["libfa_sm100.so", "libfa_sm100_debug.so"]
+    assert "binding of the paged-cache operators is not built" in capsys.readouterr().out
+
+
+def test_everything_is_built_with_torch(recorded):
+    recipe.build(force=True, verbose=False)
+    outputs = _outputs(recorded)
+    assert outputs[:2] == ["libfa_sm100.so", "libfa_sm100_debug.so"] and len(outputs) == 3 and outputs[2].startswith("_paged")
+
+
+def test_a_missing_binding_asks_for_a_build_only_with_torch(monkeypatch, tmp_path):
+    for name in ("LIB_PATH", "DEBUG_LIB_PATH"):
+        path = tmp_path / name
+        path.write_text("")
+        os.utime(path, (2 ** 32, 2 ** 32))
+        monkeypatch.setattr(recipe, name, str(path))
+    monkeypatch.setattr(recipe, "BINDING_PATH", str(tmp_path / "absent"))
+    assert recipe.needs_build()
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert not recipe.needs_build()
