@@ -13,11 +13,13 @@ The same sources compiled with FA_SM100_DEBUG_DUMP give lib/libfa_sm100_debug.so
 whose kernel also dumps its intermediate tiles for layout checks
 (fa_sm100_debug_read); only tests load it.
 
-lib/_paged.so is the CPython binding of the paged-cache operators for torch tensors
+lib/_paged.<python>-torch<version>.so is the CPython binding of the paged-cache operators for torch tensors
 (csrc/paged_binding.cpp). It is the one part that is compiled against torch's headers
 and needs torch at run time; the two libraries above do not, and without torch they
-alone are built.
+alone are built. Its name holds the versions that it was compiled for, so that after an
+upgrade it is missing, and built again, instead of being loaded with another binary interface.
 """
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -30,7 +32,18 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libfa_sm100.so")
 DEBUG_LIB_PATH = os.path.join(LIB_DIR, "libfa_sm100_debug.so")
-BINDING_PATH = os.path.join(LIB_DIR, "_paged.so")
+
+
+def binding_name():
+    """File name of the binding for this Python and the installed torch."""
+    try:
+        torch_version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        torch_version = "unknown"
+    return f"_paged.{sys.implementation.cache_tag}-torch{torch_version}.so"
+
+
+BINDING_PATH = os.path.join(LIB_DIR, binding_name())
 SOURCES = ["fa_sm100.cu", "fa_sm100_host.cu", "fa_sm100_api.cu", "fa_sm100_static.cu",
            "fa_sm100_plan.cu", "fa_sm100_paged.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

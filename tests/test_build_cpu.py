@@ -54,3 +54,18 @@ def test_a_missing_binding_asks_for_a_build_only_with_torch(monkeypatch, tmp_pat
     assert recipe.needs_build()
     monkeypatch.setitem(sys.modules, "torch", None)
     assert not recipe.needs_build()
+
+
+def test_the_binding_is_named_after_what_it_was_compiled_for(monkeypatch):
+    """Another torch or Python looks for another file, and asks for a build."""
+    torch = pytest.importorskip("torch")
+    import importlib.metadata
+    name = os.path.basename(recipe.BINDING_PATH)
+    assert name == recipe.binding_name() and torch.__version__ in name and sys.implementation.cache_tag in name
+    assert recipe.binding_command()[-1] == recipe.BINDING_PATH
+    with monkeypatch.context() as other:
+        other.setattr(importlib.metadata, "version", lambda package: "0.1")
+        assert recipe.binding_name() != name
+    with monkeypatch.context() as other:
+        other.setattr(sys.implementation, "cache_tag", "cpython-0")
+        assert recipe.binding_name() != name
