@@ -1348,6 +1348,10 @@ int forward(const void* q, const void* k, const void* v, void* o, int batch, int
 
 namespace fa_sm100_internal {
 
+// Weak: a program may be linked from the dense forward's sources alone, without the paged-cache operators'.
+int take_plan_error(unsigned int* word) __attribute__((weak));
+int take_paged_attention_error(unsigned int* word) __attribute__((weak));
+
 int encode_map(CUtensorMap* map, const void* ptr, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
                const cuuint32_t* box)
 {
@@ -1510,8 +1514,10 @@ int fa_sm100_device_status(unsigned int* detail)
     if (err != cudaSuccess) return static_cast<int>(err);
     // The paged-cache operators keep words of their own: what they recorded joins this one.
     unsigned int plan_word = 0, paged_word = 0;
-    int status = fa_sm100_internal::take_plan_error(&plan_word);
-    if (status == FA_STATUS_OK) status = fa_sm100_internal::take_paged_attention_error(&paged_word);
+    int status = FA_STATUS_OK;
+    if (fa_sm100_internal::take_plan_error != nullptr) status = fa_sm100_internal::take_plan_error(&plan_word);
+    if (status == FA_STATUS_OK && fa_sm100_internal::take_paged_attention_error != nullptr)
+        status = fa_sm100_internal::take_paged_attention_error(&paged_word);
     if (status != FA_STATUS_OK) return status;
     const unsigned int paged = plan_word | paged_word;
     if (word == 0 || (paged & 1u) == 0) word |= paged;

@@ -69,3 +69,17 @@ def test_the_binding_is_named_after_what_it_was_compiled_for(monkeypatch):
     with monkeypatch.context() as other:
         other.setattr(sys.implementation, "cache_tag", "cpython-0")
         assert recipe.binding_name() != name
+
+
+def test_the_dense_forward_links_without_the_paged_sources(tmp_path):
+    """A target that lists the dense forward's four sources alone (front end only: no GPU code is assembled)."""
+    import ctypes
+    dense = [os.path.join(recipe.CSRC, name) for name in ("fa_sm100.cu", "fa_sm100_host.cu", "fa_sm100_api.cu", "fa_sm100_static.cu")]
+    output = str(tmp_path / "dense.so")
+    done = subprocess.run([recipe.nvcc_path(), "-std=c++17", "-gencode", "arch=compute_100a,code=compute_100a", "-shared",
+                           "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-Xlinker", "--no-undefined",
+                           "-I", os.path.join(recipe.ROOT, "include"), "-I", recipe.CSRC, *dense, "-o", output],
+                          capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr[-2000:]
+    lib = ctypes.CDLL(output, mode=os.RTLD_NOW)
+    assert lib.fa_sm100_supported(128) == 1 and not hasattr(lib, "fa_sm100_paged_plan")
