@@ -1536,6 +1536,8 @@ int validate_plan(const FaPagedPlan* plan)
     if (plan->num_seqs < 0 || plan->total_tokens < 0 || plan->max_new < 0 || plan->num_pages < 0 ||
         plan->table_width < 0 || plan->table_stride < plan->table_width)
         return FA_STATUS_INVALID_ARGUMENT;
+    // The kernels count requests and rows in 32 bits, in steps of up to a block of threads.
+    if (plan->num_seqs >= (1 << 30) || plan->total_tokens >= (1 << 30)) return FA_STATUS_INVALID_ARGUMENT;
     // Slots are 32-bit; positions leave room for a tile behind the last key.
     if (static_cast<long long>(plan->num_pages) * plan->page_size > INT_MAX ||
         static_cast<long long>(plan->table_width) * plan->page_size > (1 << 30))

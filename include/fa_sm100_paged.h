@@ -51,8 +51,8 @@ extern "C" {
 /* One step's requests: sizes set by the caller, arrays filled by fa_sm100_paged_plan
  * (block_table is read and extended). All device pointers. */
 typedef struct FaPagedPlan {
-    int num_seqs;               /* requests, 0 or more */
-    int total_tokens;           /* rows of the packed token axis */
+    int num_seqs;               /* requests, 0 or more, fewer than 2^30 */
+    int total_tokens;           /* rows of the packed token axis, fewer than 2^30 */
     int max_new;                /* no request brings more new tokens than this */
     int num_pages;              /* pages of the cache; num_pages * page_size < 2^31 */
     int table_width;            /* pages a table row has room for; table_width * page_size <= 2^30 */

@@ -200,3 +200,13 @@ def test_append_refuses_caches_that_share_memory(lib):
     strides = (ctypes.c_longlong * 14)(*[64] * 14)
     assert lib.fa_sm100_rotary_append(0x1000, 0x2000, 0x2000, 0x1000, 0x3000, 0x3000, strides, 2, 4, 2, 64, 16, 8, 0x1000, 2,
                                       0x1000, 0x1000, 64, sections, 1, 0, None) == 1001
+
+
+@pytest.mark.parametrize("changes", [dict(num_seqs=2 ** 30), dict(num_seqs=2 ** 31 - 1), dict(total_tokens=2 ** 30),
+                                     dict(total_tokens=2 ** 31 - 1)], ids=str)
+def test_c_plan_refuses_more_than_the_kernels_can_count(lib, changes):
+    plan = ctypes.byref(_plan(**changes))
+    strides = (ctypes.c_longlong * 10)(*[128] * 10)
+    assert lib.fa_sm100_paged_plan(plan, 0x1000, 0x1000, 0x1000, 4, None, None) == 1001
+    assert lib.fa_sm100_paged_fwd(plan, 0x1000, 0x1000, 0x1000, 0x1000, strides, 0x1000, 1 << 40, None) == 1001
+    assert lib.fa_sm100_paged_workspace_bytes(plan) == 0
