@@ -270,6 +270,18 @@ void need_arguments(Py_ssize_t given, Py_ssize_t expected)
 
 constexpr long long kIntMax = 2147483647LL;
 
+// No element of a vector may be one of the table's, whose rows of `width` begin `stride` apart.
+void need_outside_table(const at::Tensor& vector, const char* name, const at::Tensor& table, int64_t width, int64_t stride)
+{
+    const int64_t rows = table.size(0), size = vector.numel();
+    if (rows == 0 || width == 0 || size == 0) return;
+    const auto bytes = static_cast<const char*>(vector.const_data_ptr()) - static_cast<const char*>(table.const_data_ptr());
+    const int64_t from = bytes >= 0 ? bytes / 4 : -((3 - bytes) / 4);       // element of the table at which it begins
+    if (from + size <= 0) return;
+    const int64_t row = from < width ? 0 : (from - width) / stride + 1;     // the first row that ends behind it
+    if (row < rows && row * stride < from + size) bad_value(std::string(name) + " must not share memory with block_table");
+}
+
 // plan(cached_lens, new_lens, block_table, free_pages, total_tokens, (heads, kv_heads, head_dim, page_size),
 //      num_pages, free_cursor, causal, max_new, buffer or None, stream)
 //   -> (buffer, FaPagedPlan as bytes, workspace bytes, device index)
@@ -301,6 +313,11 @@ PyObject* plan(PyObject* const* args, Py_ssize_t count)
     if (num_pages > kIntMax || num_pages * shape[3] > kIntMax || stride > kIntMax || seqs > kIntMax / 4)
         bad_value("a cache must hold fewer than 2^31 tokens");
     if (width * shape[3] > (1LL << 30)) bad_value("a table row must hold at most 2^30 tokens");
+    // The kernel's blocks extend the table while others still read the inputs.
+    need_outside_table(cached, "cached_lens", table, width, stride);
+    need_outside_table(fresh, "new_lens", table, width, stride);
+    need_outside_table(free_pages, "free_pages", table, width, stride);
+    if (has_cursor) need_outside_table(tensor(args[7], "free_cursor"), "free_cursor", table, width, stride);
     OneDevice device;
     device.add(cached, "cached_lens");
     device.add(fresh, "new_lens");

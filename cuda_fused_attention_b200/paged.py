@@ -104,12 +104,13 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, total_tokens, sha
     """Block tables, slots, positions and schedule of a step, built on the GPU.
 
     cached_lens, new_lens: int32 [B], tokens that each request has in the cache and brings now.
-    block_table: int32 [B, W], extended in place by the pages that the new tokens need; they are
-    free_pages[free_cursor + k], handed out in request order, and plan.free_cursor is where the
-    next step begins (free_cursor: int32 [1], default 0). Where the list has ended the table gets -1: tokens
-    of such a page have slot -1, are not written, and count as zeros in attention; device_status() reports it. total_tokens: rows of the packed token
-    axis, at least the sum of new_lens. num_pages: pages of the cache. max_new: an upper bound of
-    new_lens (default total_tokens); a tight one lets calls leave out kernels that have no work.
+    block_table: int32 [B, W], extended in place by the pages that the new tokens need (it shares memory
+    with no input); they are free_pages[free_cursor + k], handed out in request order, and
+    plan.free_cursor is where the next step begins (free_cursor: int32 [1], default 0). Where the list has
+    ended the table gets -1: tokens of such a page have slot -1, are not written, and count as zeros in
+    attention; device_status() reports it. total_tokens: rows of the packed token axis, at least the sum
+    of new_lens. num_pages: pages of the cache. max_new: an upper bound of new_lens (default
+    total_tokens); a tight one lets calls leave out kernels that have no work.
     plan: an earlier plan of the same B, total_tokens and shape whose buffers are written again
     (for CUDA graphs); its own arrays cannot be inputs then: copy kv_lens and free_cursor to the next
     step's tensors first. A captured attention call keeps the causal, max_new and table of the plan that it

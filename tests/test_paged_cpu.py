@@ -210,3 +210,26 @@ def test_c_plan_refuses_more_than_the_kernels_can_count(lib, changes):
     assert lib.fa_sm100_paged_plan(plan, 0x1000, 0x1000, 0x1000, 4, None, None) == 1001
     assert lib.fa_sm100_paged_fwd(plan, 0x1000, 0x1000, 0x1000, 0x1000, strides, 0x1000, 1 << 40, None) == 1001
     assert lib.fa_sm100_paged_workspace_bytes(plan) == 0
+
+
+def test_plan_refuses_inputs_inside_the_table():
+    """One block would read what another has written."""
+    shape = fa.PagedShape(8, 2, 64, 16)
+    pool = _i32(64)
+    good = dict(cached_lens=_i32(2), new_lens=_i32(2), block_table=pool[16:48].view(2, 16)[:, :6], free_pages=_i32(3),
+                total_tokens=5, shape=shape, num_pages=9, free_cursor=_i32(1))
+
+    def refusal(**change):
+        with pytest.raises((ValueError, TypeError)) as caught:
+            fa.paged_plan(**{**good, **change})
+        return str(caught.value)
+
+    # The table's elements are 16 to 21 and 32 to 37 of the pool.
+    for name, size in (("cached_lens", 2), ("new_lens", 2), ("free_pages", 9), ("free_cursor", 1)):
+        for at in range(64 - size):
+            inside = any(at <= e < at + size for e in (*range(16, 22), *range(32, 38)))
+            text = refusal(**{name: pool[at: at + size]})
+            assert (f"{name} must not share memory with block_table" in text) == inside, (name, at)
+            assert inside or "must be a CUDA tensor" in text
+    one = refusal(cached_lens=pool[3:4], new_lens=_i32(1), block_table=pool[:4].view(1, 4))
+    assert "cached_lens must not share" in one
