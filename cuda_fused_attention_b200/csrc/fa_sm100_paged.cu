@@ -63,7 +63,7 @@ constexpr float kRebase = 16.0f;
 // else that is kept is 32-bit. Why mma.sync and not tcgen05: a tile of 128 rows would be nearly empty, and
 // its fragments keep up with memory. Measured (B200, 32/8 heads, D = 128): 64 requests of 4095 to
 // 16384 keys 410 us, 6.6 TB/s; 32 of up to 4096 keys 52 us with the merging, 5.3 TB/s; 16 of 5 to 8
-// new tokens behind up to 8192 (MT = 2) 63 us, 4.8 TB/s.
+// new tokens behind up to 8192 (MT = 2) 62 to 66 us, 4.6 to 4.9 TB/s, and 69 us a call.
 constexpr int kNarrowWarps = 4;
 constexpr int kNarrowThreads = (kNarrowWarps + 1) * 32;
 constexpr int kNarrowCtasPerSm = 2;
@@ -632,8 +632,10 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 // the softmax: about 3400 cycles per key tile of a block of two Q tiles, of which the special-function
 // unit needs 2048 (a part of the exponentials as cubics on the FMA pipe was slower: 403 us against 394). P is rounded to
 // bf16 for the product with V, as in the dense kernel: a second product for the rest would cost the tensor
-// pipe a third more. Measured (B200, 32/8 heads, D = 128): 2048 new tokens behind 14336 cached 390 us,
-// 1320 TFLOP/s, with S and P in the same columns 405; a causal prompt of 8192 tokens 435 us (455); 16
+// pipe a third more, and at D = 128 tensor memory has no room for it. The result is off by 0.0024 of its size,
+// against 0.0017 where it alone is rounded. Measured (B200, 32/8 heads, D = 128): 2048 new tokens behind 14336 cached
+// 385 to 400 us in short runs, up to 1340 TFLOP/s (457 us a call in long ones, at the power limit), with S and P in
+// the same columns 405; a causal prompt of 8192 tokens 435 us (455); 16
 // requests of 16 new tokens (64 rows) behind up to 8192 71 us, 4.3 TB/s.
 constexpr int kWideThreads = 384;
 constexpr int kWideMinUnits = 4;        // units a CTA takes at least, more than a tile's (256 new tokens: 17.8 us; 2: 19.4, 8: 20.7)

@@ -29,7 +29,7 @@ __device__ __forceinline__ void record_plan_error(unsigned int bits) { atomicOr(
 // (B200): 4.4 us for 16 decoding requests, 8.0 us for 512 requests with 99k new tokens.
 constexpr int kPlanThreads = 512;
 constexpr int kPlanWarps = kPlanThreads / 32;
-constexpr int kPlanTokensPerCta = 2048;     // tokens per CTA before another CTA is launched
+constexpr int kPlanTokensPerCta = 2048;     // tokens before another CTA is launched (99k tokens: 7.9 us; 4096: 10.0, 1024: 7.5, 512: 6.4)
 
 struct PlanParams {
     FaPagedPlan plan;

@@ -102,8 +102,11 @@ FA_API float fa_default_scale(int head_dim);
 
 /* Reads and clears the device-side error word of the current device after a
  * device synchronisation. FA_STATUS_OK, FA_STATUS_DEVICE_TIMEOUT, or a
- * cudaError_t from the synchronisation. `detail` (may be NULL) receives the raw
- * word: bit 0 set by any timeout, bits 8..15 the id of the wait that gave up.
+ * cudaError_t from the synchronisation; what the paged-cache operators recorded
+ * (fa_sm100_paged.h) is read and cleared with it: FA_STATUS_OUT_OF_PAGES, or
+ * FA_STATUS_BAD_REQUEST. A timeout comes first, then missing pages. `detail` (may
+ * be NULL) receives the raw word: bit 0 set by any timeout, bits 8..15 the id of
+ * the wait that gave up, bits 16 and up the FA_ERROR_* of fa_sm100_paged.h.
  * There is one word per device, shared by every launch, stream and host thread
  * on it: with concurrent callers, a timeout is reported to whichever caller
  * reads the word first (this call, or fa_sm100_fwd_host /

@@ -53,7 +53,7 @@ extern "C" {
 typedef struct FaPagedPlan {
     int num_seqs;               /* requests, 0 or more, fewer than 2^30 */
     int total_tokens;           /* rows of the packed token axis, fewer than 2^30 */
-    int max_new;                /* no request brings more new tokens than this */
+    int max_new;                /* no request brings more new tokens than this; a tight bound leaves out kernels */
     int num_pages;              /* pages of the cache; num_pages * page_size < 2^31 */
     int table_width;            /* pages a table row has room for; table_width * page_size <= 2^30 */
     int table_stride;           /* elements between table rows, >= table_width */
@@ -120,7 +120,9 @@ FA_API int fa_sm100_rotary_append(const void* q, const void* k, const void* v, v
  * k_cache (page, head, row), v_cache (page, head, row). o may be q. The new tokens' K and V must
  * be in the cache. What a cache holds behind a request's last token is never used, whatever it
  * is (NaN included); V of a later token of the same request takes part with weight zero, so it
- * has to be finite. workspace: fa_sm100_paged_workspace_bytes(plan) bytes, 16-byte aligned, not
+ * has to be finite. Scores, weights and sums are in 32 bits; for the product with V a weight is rounded to bf16,
+ * as in fa_sm100_fwd, in requests of more than 16 query rows per K/V head (32 if max_new and total_tokens allow no
+ * request more than 32), and to two bf16 numbers, 16 bits, in the others. workspace: fa_sm100_paged_workspace_bytes(plan) bytes, 16-byte aligned, not
  * shared with a call that may run at the same time; its contents need no preparation. The plan is the one
  * that fa_sm100_paged_plan had, unchanged. Where its arrays no longer fit it (a captured call, after they were written
  * again for another mask, max_new or table), the call records FA_ERROR_OTHER_PLAN and leaves work out. */
