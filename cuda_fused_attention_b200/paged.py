@@ -117,8 +117,8 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, total_tokens, sha
     plan: an earlier plan of the same B, total_tokens and shape whose buffers are written again
     (for CUDA graphs); its own arrays cannot be inputs then: copy kv_lens and free_cursor to the next
     step's tensors first. A captured attention call keeps the causal, max_new and table of the plan that it
-    saw; replayed after the plan was written with others it leaves out work, which device_status() reports
-    (STATUS_BAD_REQUEST). Returns the PagedPlan.
+    saw; replayed after the plan was written with others its output is of no use, which device_status()
+    reports (STATUS_BAD_REQUEST). Returns the PagedPlan.
     """
     ops = _ops or _load()
     seqs = cached_lens.numel()

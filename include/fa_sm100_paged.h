@@ -125,7 +125,7 @@ FA_API int fa_sm100_rotary_append(const void* q, const void* k, const void* v, v
  * request more than 32), and to two bf16 numbers, 16 bits, in the others. workspace: fa_sm100_paged_workspace_bytes(plan) bytes, 16-byte aligned, not
  * shared with a call that may run at the same time; its contents need no preparation. The plan is the one
  * that fa_sm100_paged_plan had, unchanged. Where its arrays no longer fit it (a captured call, after they were written
- * again for another mask, max_new or table), the call records FA_ERROR_OTHER_PLAN and leaves work out. */
+ * again for another mask, max_new or table), the call records FA_ERROR_OTHER_PLAN and ends; its output is of no use. */
 FA_API int fa_sm100_paged_fwd(const FaPagedPlan* plan, const void* q, const void* k_cache, const void* v_cache,
                               void* o, const long long* strides, void* workspace, size_t workspace_bytes,
                               void* stream);
